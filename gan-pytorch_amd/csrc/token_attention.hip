@@ -1,0 +1,756 @@
+// Attention of query rows over key rows with shared key heads and ragged lengths, forward and backward.
+//
+//   s = scale q k^T (key j takes part if j < k_len[b], query t if t < q_len[b])     p = softmax(s)     o = p v
+//   delta = sum_d go o      gv = p^T go      ds = p (go v^T - delta)      gq = scale ds k      gk = scale ds^T q
+//
+// One pass over the keys with the running maximum and sum of the softmax; nothing of size Tq x Tk is ever stored. The
+// backward pass rebuilds p = exp(s - lse) from the row's log-sum.
+//
+// Rows. The G = Hq / Hk query heads of a key head and its Tq queries are the R = Tq G rows of one problem (b, hk), row
+// r = t G + g: keys and values are read once for the whole group, the gradients of a shared head are sums over rows of
+// the same problem (no atomics, a fixed order), and a single query still fills G rows of a tile.
+//
+// Layout of the products. Every product is taken transposed or not so that its result feeds the next one from the
+// registers it lies in. A 32 x 32 product leaves lane (c, h) = (lane % 32, lane / 32) with column c and the 16 rows
+// 8 (i / 4) + 4 h + i % 4. The forward pass takes S^T = K Q^T (column = query), so a lane owns 16 keys of one query: the
+// softmax needs one exchange between lanes c and c + 32, and the probabilities are the B operand of O^T = V^T P^T as
+// they are, if the keys of a k-slice are numbered in the order in which the lane holds them - which only says which
+// rows of V the A operand reads. bf16 reads them with the transposing LDS load (4 keys of one column per lane), f32 with
+// 4-byte loads. Queries' gradients use the same shape; the gradients of keys and values its mirror image (column = key).
+#include <float.h>
+#include <math.h>
+
+#include "token_common.h"
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTileRows = 32 * kWaves;     // rows (forward, queries' gradient) or keys (keys' gradient) of a block
+
+struct AttnParams {
+  vg_attention_geom g;
+  const void *q, *k, *v, *o, *go;
+  void *out, *gq, *gk, *gv;
+  const float *lse_in, *delta;
+  float* lse;
+  const int *q_len, *k_len;
+  float* part;               // split launches: f32 partial results
+  float* part_ml;            // forward: running maximum and sum of every row and split
+  int G, R, splits, chunk;   // chunk: keys (forward, queries' gradient) or rows (keys' gradient) of a split
+  unsigned g_magic;          // ceil(2^32 / G)
+  int row_tiles, key_tiles;
+  float cs;                  // scale * log2(e)
+};
+
+__device__ __forceinline__ int row_query(const AttnParams& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.g_magic); }
+
+template <class T>
+__device__ __forceinline__ const T* row_at(const void* base, const vg_heads_layout& l, const AttnParams& p, int b, int hk, int r) {
+  const int t = row_query(p, r), g = r - t * p.G;
+  return (const T*)base + b * l.sb + t * l.st + (int64_t)(hk * p.G + g) * l.sh;
+}
+
+__device__ __forceinline__ int clamped(const int* len, int b, int most) {
+  if (!len) return most;
+  const int n = len[b];
+  return n < 0 ? 0 : n > most ? most : n;
+}
+
+// ---- fragments ------------------------------------------------------------------------------------------------------
+// LD: elements of an LDS row. 16 bytes of padding spread the rows of a fragment over the banks.
+template <class T, int DP>
+struct Tile {
+  static constexpr int V = TokNum<T>::V;
+  static constexpr int LD = DP + V;
+};
+
+// Registers of a 32-row operand whose contraction index is d: bf16 holds 8 d of each 16 (8 h ..), f32 4 of each 8.
+template <class T, int DP>
+struct RowFrag;
+template <int DP>
+struct RowFrag<__bf16, DP> {
+  bf16x8 f[DP / 16];
+  __device__ __forceinline__ void load(const __bf16* row, int D, int h, bool ok) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = 16 * s + 8 * h;
+      const u32x4 raw = ok && d < D ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0, 0, 0, 0};
+      f[s] = __builtin_bit_cast(bf16x8, raw);
+    }
+  }
+};
+template <int DP>
+struct RowFrag<float, DP> {
+  f32x4 f[DP / 8];
+  __device__ __forceinline__ void load(const float* row, int D, int h, bool ok) {
+#pragma unroll
+    for (int s = 0; s < DP / 8; ++s) {
+      const int d = 8 * s + 4 * h;
+      f[s] = ok && d < D ? *reinterpret_cast<const f32x4*>(row + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// C[row of the LDS tile][column] += sum_d tile[row0 + row][d] * frag(column)[d]
+template <int DP>
+__device__ __forceinline__ f32x16 mul_rows(const __bf16* tile, const RowFrag<__bf16, DP>& b, int row0, int c, int h) {
+  f32x16 acc = zero16();
+  const __bf16* a = tile + (row0 + c) * Tile<__bf16, DP>::LD + 8 * h;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(a + 16 * s), b.f[s], acc, 0, 0, 0);
+  return acc;
+}
+template <int DP>
+__device__ __forceinline__ f32x16 mul_rows(const float* tile, const RowFrag<float, DP>& b, int row0, int c, int h) {
+  f32x16 acc = zero16();
+  const float* a = tile + (row0 + c) * Tile<float, DP>::LD + 4 * h;
+#pragma unroll
+  for (int s = 0; s < DP / 8; ++s) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a + 8 * s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], b.f[s][e], acc, 0, 0, 0);
+  }
+  return acc;
+}
+
+// acc[j] (rows d = 32 j + row) += sum over the 32 tile rows k0.. of tile[k][d] * w[k][column], w as a product left it
+template <int DP>
+__device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
+  constexpr int LD = Tile<__bf16, DP>::LD;
+  const int h = lane >> 5, q = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const u32x4 pk = {tok_pack2(w[8 * s], w[8 * s + 1]), tok_pack2(w[8 * s + 2], w[8 * s + 3]), tok_pack2(w[8 * s + 4], w[8 * s + 5]),
+                      tok_pack2(w[8 * s + 6], w[8 * s + 7])};
+    const bf16x8 b = __builtin_bit_cast(bf16x8, pk);
+    const __bf16* a = tile + (k0 + 16 * s + 4 * h + q) * LD + col;
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) {
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 32 * j));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 32 * j + 8 * LD));
+      const s16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), b, acc[j], 0, 0, 0);
+    }
+  }
+}
+template <int DP>
+__device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
+  constexpr int LD = Tile<float, DP>::LD;
+  const int h = lane >> 5, c = lane & 31;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float* a = tile + (k0 + 8 * (i / 4) + 4 * h + i % 4) * LD + c;
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[32 * j], w[i], acc[j], 0, 0, 0);
+  }
+}
+
+// Stages ROWS rows of up to DP elements in registers on their way to an LDS tile; what is out of range becomes zero.
+template <class T, int DP, int ROWS>
+struct Stage {
+  static constexpr int V = TokNum<T>::V, VPR = DP / V, N = ROWS * VPR / (64 * kWaves);
+  static_assert(ROWS * VPR % (64 * kWaves) == 0, "whole vectors per thread");
+  u32x4 r[N];
+  template <class At>
+  __device__ __forceinline__ void load(int D, int rows, At at) {     // at(row) -> pointer to its first element
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = threadIdx.x + i * 64 * kWaves, row = id / VPR, d = (id % VPR) * V;
+      r[i] = row < rows && d < D ? *reinterpret_cast<const u32x4*>(at(row) + d) : u32x4{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = threadIdx.x + i * 64 * kWaves, row = id / VPR, d = (id % VPR) * V;
+      *reinterpret_cast<u32x4*>(tile + row * Tile<T, DP>::LD + d) = r[i];
+    }
+  }
+};
+
+// keys (rows) of a staged tile: two buffers of two tiles fit the 160 KB of a CU
+template <class T, int DP>
+constexpr int tile_len() {
+  return sizeof(T) == 2 ? 64 : DP >= 128 ? 32 : 64;
+}
+
+template <class T>
+__device__ __forceinline__ void store_cols(T* row, const f32x16& a, int j, int h, int D, float f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = 32 * j + 8 * i + 4 * h;
+    if (d < D) tok_store4(row + d, a[4 * i] * f, a[4 * i + 1] * f, a[4 * i + 2] * f, a[4 * i + 3] * f);
+  }
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+// Grid: (row tile, split, problem), the row tiles of a problem on one XCD. SPLIT: every split leaves its unnormalised
+// rows, maximum and sum for the joining kernel.
+template <class T, int DP, bool SPLIT>
+__global__ void __launch_bounds__(256) attn_fwd_kernel(const AttnParams p) {
+  constexpr int KT = tile_len<T, DP>(), LD = Tile<T, DP>::LD;
+  __shared__ __attribute__((aligned(16))) T smem[2][2][KT * LD];
+  const vg_attention_geom& g = p.g;
+  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
+  const int rt = id % p.row_tiles, sp = (id / p.row_tiles) % p.splits, prob = id / (p.row_tiles * p.splits);
+  const int b = prob / g.Hk, hk = prob - b * g.Hk;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+  const int rows = clamped(p.q_len, b, g.Tq) * p.G;
+  const int kl = clamped(p.k_len, b, g.Tk);
+  const int r = rt * kTileRows + wid * 32 + c;
+  const int kbeg = sp * p.chunk, kend = rt * kTileRows < rows ? min(kl, kbeg + p.chunk) : 0;
+
+  RowFrag<T, DP> qf;
+  qf.load(row_at<T>(p.q, g.q, p, b, hk, r < rows ? r : 0), g.D, h, r < rows);
+  const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
+  const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
+  Stage<T, DP, KT> sk, sv;
+  auto fetch = [&](int j) {
+    sk.load(g.D, kend - j, [&](int row) { return kb + (int64_t)(j + row) * g.k.st; });
+    sv.load(g.D, kend - j, [&](int row) { return vb + (int64_t)(j + row) * g.v.st; });
+  };
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int j = 0; j < DP / 32; ++j) o[j] = zero16();
+  float m = -FLT_MAX, l = 0.f;       // finite: a row whose scores are all -inf sums to zero, not to NaN
+  int buf = 0;
+  if (kbeg < kend) {
+    fetch(kbeg);
+    sk.store(smem[0][0]);
+    sv.store(smem[0][1]);
+  }
+  __syncthreads();
+  for (int j = kbeg; j < kend; j += KT) {
+    const bool more = j + KT < kend;
+    if (more) fetch(j + KT);
+    f32x16 s[KT / 32];
+    float top = m;
+#pragma unroll
+    for (int kk = 0; kk < KT / 32; ++kk) {
+      s[kk] = mul_rows<DP>(smem[buf][0], qf, 32 * kk, c, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kk][i] *= p.cs;
+        if (j + KT > kend && j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) s[kk][i] = -INFINITY;
+        top = fmaxf(top, s[kk][i]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float alpha = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    float sum = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KT / 32; ++kk)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kk][i] = __builtin_amdgcn_exp2f(s[kk][i] - m);
+        sum += s[kk][i];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+#pragma unroll
+    for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP>(smem[buf][1], s[kk], 32 * kk, lane, o);
+    if (more) {
+      sk.store(smem[buf ^ 1][0]);
+      sv.store(smem[buf ^ 1][1]);
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (r >= rows) l = 0.f;       // (took part as a row of zeros)
+  if (r >= p.R) return;
+  if constexpr (SPLIT) {
+    const size_t at = ((size_t)prob * p.splits + sp) * p.R + r;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) store_cols(p.part + at * DP, r < rows ? o[d] : zero16(), d, h, DP, 1.f);
+    if (h == 0) {
+      p.part_ml[2 * at] = m;
+      p.part_ml[2 * at + 1] = l;
+    }
+  } else {
+    const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+    T* out = const_cast<T*>(row_at<T>(p.out, g.o, p, b, hk, r));
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) store_cols(out, r < rows ? o[d] : zero16(), d, h, g.D, f);
+    // a row without keys: +inf, so that the backward pass finds p = exp(s - inf) = 0
+    if (h == 0 && p.lse) p.lse[(size_t)prob * p.R + r] = f != 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+  }
+}
+
+// Joins the splits of a row: D / 4 lanes a row (rounded up to a power of two), 4 elements each.
+template <class T, int DP>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
+  constexpr int LPR = DP / 4;
+  const vg_attention_geom& g = p.g;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int d = (threadIdx.x % LPR) * 4;
+  if (row >= (long long)g.B * g.Hk * p.R) return;
+  const int prob = (int)(row / p.R), r = (int)(row - (long long)prob * p.R);
+  const int b = prob / g.Hk, hk = prob - b * g.Hk;
+  const size_t first = (size_t)prob * p.splits * p.R + r;
+  float m = -FLT_MAX;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (first + (size_t)s * p.R)]);
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const size_t at = first + (size_t)s * p.R;
+    const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - m);
+    l += f * p.part_ml[2 * at + 1];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * DP + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+  }
+  const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+  if (d < g.D) tok_store4(const_cast<T*>(row_at<T>(p.out, g.o, p, b, hk, r)) + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+  if (d == 0 && p.lse) p.lse[row] = f != 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+// delta[row] = sum_d go o: eight lanes a row
+template <class T>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, float* delta) {
+  constexpr int V = TokNum<T>::V;
+  const vg_attention_geom& g = p.g;
+  const long long row = (long long)blockIdx.x * 32 + threadIdx.x / 8;
+  float sum = 0.f;
+  if (row < (long long)g.B * g.Hk * p.R) {
+    const int prob = (int)(row / p.R), r = (int)(row - (long long)prob * p.R);
+    const int b = prob / g.Hk, hk = prob - b * g.Hk;
+    if (r < clamped(p.q_len, b, g.Tq) * p.G) {
+      const T* go = row_at<T>(p.go, g.go, p, b, hk, r);
+      const T* o = row_at<T>(p.o, g.o, p, b, hk, r);
+      for (int d = (threadIdx.x % 8) * V; d < g.D; d += 8 * V) {
+        float x[V], y[V];
+        tok_widen(*reinterpret_cast<const u32x4*>(go + d), x);
+        tok_widen(*reinterpret_cast<const u32x4*>(o + d), y);
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum = __builtin_fmaf(x[e], y[e], sum);
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (threadIdx.x % 8 == 0 && row < (long long)g.B * g.Hk * p.R) delta[row] = sum;
+}
+
+// Queries' gradient: the forward kernel's walk with p rebuilt from lse.
+template <class T, int DP, bool SPLIT>
+__global__ void __launch_bounds__(256) attn_gq_kernel(const AttnParams p) {
+  constexpr int KT = tile_len<T, DP>(), LD = Tile<T, DP>::LD;
+  __shared__ __attribute__((aligned(16))) T smem[2][2][KT * LD];
+  const vg_attention_geom& g = p.g;
+  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
+  const int rt = id % p.row_tiles, sp = (id / p.row_tiles) % p.splits, prob = id / (p.row_tiles * p.splits);
+  const int b = prob / g.Hk, hk = prob - b * g.Hk;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+  const int rows = clamped(p.q_len, b, g.Tq) * p.G;
+  const int kl = clamped(p.k_len, b, g.Tk);
+  const int r = rt * kTileRows + wid * 32 + c;
+  const int kbeg = sp * p.chunk, kend = rt * kTileRows < rows ? min(kl, kbeg + p.chunk) : 0;
+
+  RowFrag<T, DP> qf, gf;
+  qf.load(row_at<T>(p.q, g.q, p, b, hk, r < rows ? r : 0), g.D, h, r < rows);
+  gf.load(row_at<T>(p.go, g.go, p, b, hk, r < rows ? r : 0), g.D, h, r < rows);
+  const float lse = r < rows ? p.lse_in[(size_t)prob * p.R + r] : INFINITY;
+  const float delta = r < rows ? p.delta[(size_t)prob * p.R + r] : 0.f;
+  const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
+  const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
+  Stage<T, DP, KT> sk, sv;
+  auto fetch = [&](int j) {
+    sk.load(g.D, kend - j, [&](int row) { return kb + (int64_t)(j + row) * g.k.st; });
+    sv.load(g.D, kend - j, [&](int row) { return vb + (int64_t)(j + row) * g.v.st; });
+  };
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int j = 0; j < DP / 32; ++j) acc[j] = zero16();
+  int buf = 0;
+  if (kbeg < kend) {
+    fetch(kbeg);
+    sk.store(smem[0][0]);
+    sv.store(smem[0][1]);
+  }
+  __syncthreads();
+  for (int j = kbeg; j < kend; j += KT) {
+    const bool more = j + KT < kend;
+    if (more) fetch(j + KT);
+#pragma unroll
+    for (int kk = 0; kk < KT / 32; ++kk) {
+      const f32x16 s = mul_rows<DP>(smem[buf][0], qf, 32 * kk, c, h);
+      f32x16 dp = mul_rows<DP>(smem[buf][1], gf, 32 * kk, c, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.cs, -lse));
+        if (j + KT > kend && j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) w = 0.f;
+        dp[i] = w * (dp[i] - delta);
+      }
+      mul_cols<DP>(smem[buf][0], dp, 32 * kk, lane, acc);
+    }
+    if (more) {
+      sk.store(smem[buf ^ 1][0]);
+      sv.store(smem[buf ^ 1][1]);
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (r >= p.R) return;
+  if constexpr (SPLIT) {
+    float* out = p.part + (((size_t)prob * p.splits + sp) * p.R + r) * DP;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) store_cols(out, acc[d], d, h, DP, 1.f);
+  } else {
+    T* out = const_cast<T*>(row_at<T>(p.gq, g.gq, p, b, hk, r));
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) store_cols(out, acc[d], d, h, g.D, g.scale);
+  }
+}
+
+// Gradients of keys and values: a block owns kTileRows keys (32 a wave, in registers) and walks the problem's rows.
+template <class T, int DP>
+constexpr int row_len() {
+  return sizeof(T) == 2 ? 64 : 32;
+}
+template <class T, int DP, bool SPLIT>
+__global__ void __launch_bounds__(256, 1) attn_gkv_kernel(const AttnParams p) {
+  constexpr int RT = row_len<T, DP>(), LD = Tile<T, DP>::LD;
+  __shared__ __attribute__((aligned(16))) T smem[2][2][RT * LD];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][RT];
+  const vg_attention_geom& g = p.g;
+  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
+  const int kt = id % p.key_tiles, sp = (id / p.key_tiles) % p.splits, prob = id / (p.key_tiles * p.splits);
+  const int b = prob / g.Hk, hk = prob - b * g.Hk;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+  const int rows = clamped(p.q_len, b, g.Tq) * p.G;
+  const int kl = clamped(p.k_len, b, g.Tk);
+  const int key = kt * kTileRows + wid * 32 + c;
+  const int rbeg = sp * p.chunk, rend = kt * kTileRows < kl ? min(rows, rbeg + p.chunk) : 0;
+
+  RowFrag<T, DP> kf, vf;
+  kf.load((const T*)p.k + b * g.k.sb + hk * g.k.sh + (int64_t)(key < kl ? key : 0) * g.k.st, g.D, h, key < kl);
+  vf.load((const T*)p.v + b * g.v.sb + hk * g.v.sh + (int64_t)(key < kl ? key : 0) * g.v.st, g.D, h, key < kl);
+  Stage<T, DP, RT> sq, sg;
+  float st_l = INFINITY, st_d = 0.f;
+  auto fetch = [&](int j) {
+    sq.load(g.D, rend - j, [&](int row) { return row_at<T>(p.q, g.q, p, b, hk, j + row); });
+    sg.load(g.D, rend - j, [&](int row) { return row_at<T>(p.go, g.go, p, b, hk, j + row); });
+    if (threadIdx.x < RT) {
+      const bool ok = j + (int)threadIdx.x < rend;
+      st_l = ok ? p.lse_in[(size_t)prob * p.R + j + threadIdx.x] : INFINITY;
+      st_d = ok ? p.delta[(size_t)prob * p.R + j + threadIdx.x] : 0.f;
+    }
+  };
+  auto put = [&](int buf) {
+    sq.store(smem[buf][0]);
+    sg.store(smem[buf][1]);
+    if (threadIdx.x < RT) {
+      stat[buf][0][threadIdx.x] = st_l;
+      stat[buf][1][threadIdx.x] = st_d;
+    }
+  };
+  f32x16 gk[DP / 32], gv[DP / 32];
+#pragma unroll
+  for (int j = 0; j < DP / 32; ++j) gk[j] = gv[j] = zero16();
+  int buf = 0;
+  if (rbeg < rend) {
+    fetch(rbeg);
+    put(0);
+  }
+  __syncthreads();
+  for (int j = rbeg; j < rend; j += RT) {
+    const bool more = j + RT < rend;
+    if (more) fetch(j + RT);
+#pragma unroll
+    for (int rr = 0; rr < RT / 32; ++rr) {
+      f32x16 w = mul_rows<DP>(smem[buf][0], kf, 32 * rr, c, h);
+      f32x16 dp = mul_rows<DP>(smem[buf][1], vf, 32 * rr, c, h);
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[buf][0][32 * rr + 8 * i4 + 4 * h]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][1][32 * rr + 8 * i4 + 4 * h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * i4 + e;
+          w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[i], p.cs, -lse[e]));
+          dp[i] = w[i] * (dp[i] - delta[e]);
+        }
+      }
+      mul_cols<DP>(smem[buf][1], w, 32 * rr, lane, gv);
+      mul_cols<DP>(smem[buf][0], dp, 32 * rr, lane, gk);
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (key >= g.Tk) return;
+  // keys that take no part went through the products as zeros: their columns are not used
+  const float live = key < kl ? 1.f : 0.f;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) {
+    if (key >= kl) gk[d] = gv[d] = zero16();
+    if constexpr (SPLIT) {
+      const size_t at = (((size_t)prob * p.splits + sp) * g.Tk + key) * DP;
+      const size_t half = (size_t)g.B * g.Hk * p.splits * g.Tk * DP;
+      store_cols(p.part + at, gk[d], d, h, DP, 1.f);
+      store_cols(p.part + half + at, gv[d], d, h, DP, 1.f);
+    } else {
+      store_cols((T*)p.gk + b * g.gk.sb + hk * g.gk.sh + (int64_t)key * g.gk.st, gk[d], d, h, g.D, g.scale);
+      store_cols((T*)p.gv + b * g.gv.sb + hk * g.gv.sh + (int64_t)key * g.gv.st, gv[d], d, h, g.D, 1.f);
+    }
+  }
+}
+
+// out = factor * sum over splits of part[prob][split][n][DP]; which = 0 queries' rows, 1 keys, 2 values
+template <class T, int DP>
+__global__ void __launch_bounds__(256) attn_sum_kernel(const AttnParams p, const float* part, int which) {
+  constexpr int LPR = DP / 4;
+  const vg_attention_geom& g = p.g;
+  const int n = which == 0 ? p.R : g.Tk;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int d = (threadIdx.x % LPR) * 4;
+  if (row >= (long long)g.B * g.Hk * n || d >= g.D) return;
+  const int prob = (int)(row / n), r = (int)(row - (long long)prob * n);
+  const int b = prob / g.Hk, hk = prob - b * g.Hk;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part + (((size_t)prob * p.splits + s) * n + r) * DP + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += x[e];
+  }
+  const float f = which == 2 ? 1.f : g.scale;
+  T* out = which == 0   ? const_cast<T*>(row_at<T>(p.gq, g.gq, p, b, hk, r))
+           : which == 1 ? (T*)p.gk + b * g.gk.sb + hk * g.gk.sh + (int64_t)r * g.gk.st
+                        : (T*)p.gv + b * g.gv.sb + hk * g.gv.sh + (int64_t)r * g.gv.st;
+  tok_store4(out + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+int check_geom(const vg_attention_geom* g) {
+  VG_REQUIRE(g, "attention: null geometry");
+  VG_REQUIRE(g->B >= 0 && g->Tq >= 0 && g->Tk >= 0 && g->Hq >= 1 && g->Hk >= 1, "attention: bad sizes B=%d Tq=%d Tk=%d Hq=%d Hk=%d", g->B,
+             g->Tq, g->Tk, g->Hq, g->Hk);
+  VG_REQUIRE(g->Hq % g->Hk == 0, "attention: %d query heads are not a multiple of %d key heads", g->Hq, g->Hk);
+  VG_REQUIRE(g->D >= 8 && g->D <= 128 && g->D % 8 == 0, "attention: head width %d is not a multiple of 8 from 8 to 128", g->D);
+  const long long G = g->Hq / g->Hk, R = (long long)g->Tq * G;
+  // r / G by a 32-bit product; block counts of 31 bits
+  VG_REQUIRE((R + kTileRows) * G < (1ll << 32) && R < (1ll << 30) && g->Tk < (1 << 30), "attention: %d queries of %lld heads a group are too many",
+             g->Tq, G);
+  VG_REQUIRE(((R + kTileRows - 1) / kTileRows + 1) * g->B * (long long)g->Hk < (1ll << 31) / 64 &&
+                 (((long long)g->Tk + kTileRows - 1) / kTileRows + 1) * g->B * (long long)g->Hk < (1ll << 31) / 64,
+             "attention: too many blocks");
+  VG_REQUIRE(isfinite(g->scale), "attention: scale is not finite");
+  return VG_OK;
+}
+
+// A walk over `len` (keys, or rows) is split where the blocks alone leave compute units idle: towards 512 blocks (two
+// for each of the 256), but no split shorter than 256, below which a split's own start and its partial results cost
+// more than the walk it saves.
+int splits_for(long long blocks, long long len) {
+  if (blocks >= 256 || blocks == 0) return 1;
+  long long s = 512 / blocks, most = len / 256;
+  if (s > most) s = most;
+  return s < 1 ? 1 : (int)s;
+}
+
+struct Plan {
+  int G, R, row_tiles, key_tiles, probs, fwd_splits, gkv_splits;
+};
+Plan plan_of(const vg_attention_geom* g) {
+  Plan q;
+  q.G = g->Hq / g->Hk;
+  q.R = g->Tq * q.G;
+  q.probs = g->B * g->Hk;
+  q.row_tiles = ceil_div(q.R, kTileRows);
+  q.key_tiles = ceil_div(g->Tk, kTileRows);
+  q.fwd_splits = splits_for((long long)q.row_tiles * q.probs, g->Tk);
+  q.gkv_splits = splits_for((long long)q.key_tiles * q.probs, q.R);
+  return q;
+}
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+size_t fwd_bytes(const vg_attention_geom* g, const Plan& q) {
+  if (q.fwd_splits == 1) return 0;
+  const size_t rows = (size_t)q.probs * q.fwd_splits * q.R;
+  return align256(rows * padded_width(g->D) * 4) + rows * 8;
+}
+size_t bwd_bytes(const vg_attention_geom* g, const Plan& q) {
+  const size_t dp = padded_width(g->D);
+  size_t a = q.fwd_splits == 1 ? 0 : (size_t)q.probs * q.fwd_splits * q.R * dp * 4;
+  const size_t b = q.gkv_splits == 1 ? 0 : 2 * (size_t)q.probs * q.gkv_splits * g->Tk * dp * 4;
+  if (b > a) a = b;       // one after the other on one stream: they share the space
+  return align256((size_t)q.probs * q.R * 4) + a;
+}
+
+AttnParams params_of(const vg_attention_geom* g, const Plan& q) {
+  AttnParams p = {};
+  p.g = *g;
+  p.G = q.G;
+  p.R = q.R;
+  p.g_magic = (unsigned)(((1ull << 32) + q.G - 1) / q.G);
+  p.row_tiles = q.row_tiles;
+  p.key_tiles = q.key_tiles;
+  p.cs = g->scale * 1.44269504088896341f;
+  return p;
+}
+int chunk_of(int len, int splits) { return ((len + splits - 1) / splits + 63) & ~63; }
+
+template <class T, int DP>
+void launch_fwd(AttnParams& p, const Plan& q, hipStream_t st) {
+  p.splits = q.fwd_splits;
+  p.chunk = chunk_of(p.g.Tk, p.splits);
+  const int grid = q.row_tiles * p.splits * q.probs;
+  if (p.splits == 1) {
+    attn_fwd_kernel<T, DP, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    attn_fwd_kernel<T, DP, true><<<grid, 256, 0, st>>>(p);
+    attn_join_kernel<T, DP><<<ceil_div((long long)q.probs * q.R, 256 / (DP / 4)), 256, 0, st>>>(p);
+  }
+}
+template <class T, int DP>
+void launch_bwd(AttnParams& p, const Plan& q, float* delta, hipStream_t st) {
+  if (q.probs * (long long)q.R > 0) attn_delta_kernel<T><<<ceil_div((long long)q.probs * q.R, 32), 256, 0, st>>>(p, delta);
+  if (q.row_tiles > 0 && p.gq) {
+    p.splits = q.fwd_splits;
+    p.chunk = chunk_of(p.g.Tk, p.splits);
+    const int grid = q.row_tiles * p.splits * q.probs;
+    if (p.splits == 1) {
+      attn_gq_kernel<T, DP, false><<<grid, 256, 0, st>>>(p);
+    } else {
+      attn_gq_kernel<T, DP, true><<<grid, 256, 0, st>>>(p);
+      attn_sum_kernel<T, DP><<<ceil_div((long long)q.probs * q.R, 256 / (DP / 4)), 256, 0, st>>>(p, p.part, 0);
+    }
+  }
+  if (q.key_tiles > 0 && p.gk) {
+    p.splits = q.gkv_splits;
+    p.chunk = chunk_of(q.R, p.splits);
+    const int grid = q.key_tiles * p.splits * q.probs;
+    if (p.splits == 1) {
+      attn_gkv_kernel<T, DP, false><<<grid, 256, 0, st>>>(p);
+    } else {
+      attn_gkv_kernel<T, DP, true><<<grid, 256, 0, st>>>(p);
+      const int blocks = ceil_div((long long)q.probs * p.g.Tk, 256 / (DP / 4));
+      attn_sum_kernel<T, DP><<<blocks, 256, 0, st>>>(p, p.part, 1);
+      attn_sum_kernel<T, DP><<<blocks, 256, 0, st>>>(p, p.part + (size_t)q.probs * p.splits * p.g.Tk * DP, 2);
+    }
+  }
+}
+
+template <class T>
+int attention_fwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len,
+                  void* o, float* lse, void* ws, size_t ws_bytes, void* stream) {
+  const int rc = check_geom(g);
+  if (rc) return rc;
+  const Plan pl = plan_of(g);
+  if (pl.probs == 0 || pl.R == 0) return VG_OK;
+  VG_REQUIRE(q && o && (g->Tk == 0 || (k && v)), "attention: null tensor");
+  VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->Tq, g->Hq) && tok_layout_ok<T>(g->o, o, g->B, g->Tq, g->Hq) &&
+                 tok_layout_ok<T>(g->k, k, g->B, g->Tk, g->Hk) && tok_layout_ok<T>(g->v, v, g->B, g->Tk, g->Hk),
+             "attention: a head does not start on a 16-byte border");
+  const size_t need = fwd_bytes(g, pl);
+  if (need && (!ws || ws_bytes < need)) return vg_fail(VG_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu are needed", ws_bytes, need);
+  VG_REQUIRE(!need || vg_aligned16(ws), "attention: workspace is not 16-byte aligned");
+  AttnParams p = params_of(g, pl);
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = o;
+  p.lse = lse;
+  p.q_len = q_len;
+  p.k_len = k_len;
+  p.part = (float*)ws;
+  if (need) p.part_ml = (float*)((char*)ws + align256((size_t)pl.probs * pl.fwd_splits * pl.R * padded_width(g->D) * 4));
+  hipStream_t st = (hipStream_t)stream;
+  switch (padded_width(g->D)) {
+    case 32: launch_fwd<T, 32>(p, pl, st); break;
+    case 64: launch_fwd<T, 64>(p, pl, st); break;
+    default: launch_fwd<T, 128>(p, pl, st);
+  }
+  VG_CHECK_LAUNCH("attention");
+  return VG_OK;
+}
+
+template <class T>
+int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* go,
+                  const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* ws, size_t ws_bytes, void* stream) {
+  const int rc = check_geom(g);
+  if (rc) return rc;
+  const Plan pl = plan_of(g);
+  if (pl.probs == 0 || (pl.R == 0 && g->Tk == 0)) return VG_OK;
+  VG_REQUIRE((pl.R == 0 || (q && o && lse && go)) && (g->Tk == 0 || (k && v)) && !gk == !gv, "attention backward: null tensor");
+  VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->Tq, g->Hq) && tok_layout_ok<T>(g->o, o, g->B, g->Tq, g->Hq) &&
+                 tok_layout_ok<T>(g->go, go, g->B, g->Tq, g->Hq) && tok_layout_ok<T>(g->gq, gq, g->B, g->Tq, g->Hq) &&
+                 tok_layout_ok<T>(g->k, k, g->B, g->Tk, g->Hk) && tok_layout_ok<T>(g->v, v, g->B, g->Tk, g->Hk) &&
+                 tok_layout_ok<T>(g->gk, gk, g->B, g->Tk, g->Hk) && tok_layout_ok<T>(g->gv, gv, g->B, g->Tk, g->Hk),
+             "attention backward: a head does not start on a 16-byte border");
+  const size_t need = bwd_bytes(g, pl);
+  if (need && (!ws || ws_bytes < need))
+    return vg_fail(VG_ERR_WORKSPACE, "attention backward: workspace of %zu bytes, %zu are needed", ws_bytes, need);
+  VG_REQUIRE(!need || vg_aligned16(ws), "attention backward: workspace is not 16-byte aligned");
+  AttnParams p = params_of(g, pl);
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.o = o;
+  p.go = go;
+  p.lse_in = lse;
+  p.q_len = q_len;
+  p.k_len = k_len;
+  p.gq = gq;
+  p.gk = gk;
+  p.gv = gv;
+  float* delta = (float*)ws;
+  p.delta = delta;
+  p.part = (float*)((char*)ws + align256((size_t)pl.probs * pl.R * 4));
+  hipStream_t st = (hipStream_t)stream;
+  switch (padded_width(g->D)) {
+    case 32: launch_bwd<T, 32>(p, pl, delta, st); break;
+    case 64: launch_bwd<T, 64>(p, pl, delta, st); break;
+    default: launch_bwd<T, 128>(p, pl, delta, st);
+  }
+  VG_CHECK_LAUNCH("attention backward");
+  return VG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vg_attention_workspace_bytes(const vg_attention_geom* g, int backward) {
+  if (check_geom(g)) return 0;
+  const Plan q = plan_of(g);
+  if (q.probs == 0) return 0;
+  return backward ? bwd_bytes(g, q) : fwd_bytes(g, q);
+}
+int vg_attention_fwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const int32_t* q_len, const int32_t* k_len,
+                     float* o, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_fwd<float>(g, q, k, v, q_len, k_len, o, lse, workspace, workspace_bytes, stream);
+}
+int vg_attention_fwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len,
+                       void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_fwd<__bf16>(g, q, k, v, q_len, k_len, o, lse, workspace, workspace_bytes, stream);
+}
+int vg_attention_bwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const float* o, const float* lse,
+                     const float* go, const int32_t* q_len, const int32_t* k_len, float* gq, float* gk, float* gv, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  return attention_bwd<float>(g, q, k, v, o, lse, go, q_len, k_len, gq, gk, gv, workspace, workspace_bytes, stream);
+}
+int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                       const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return attention_bwd<__bf16>(g, q, k, v, o, lse, go, q_len, k_len, gq, gk, gv, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

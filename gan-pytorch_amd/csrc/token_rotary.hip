@@ -1,0 +1,316 @@
+// Per-head RMS norm of queries and keys and their rotation by positions on several axes, one pass over the data.
+//
+//   r = 1 / sqrt(mean(x^2) + eps)      n = x r w           (w null: n = x)
+//   section a of a head (width[a] elements, pairs (2i, 2i+1)):  theta = pos[a] base^(-2i / width[a])
+//   y0 = n0 cos - n1 sin    y1 = n0 sin + n1 cos           (elements behind the sections: y = n)
+// backward:  gn = R^T gy     gw = sum gn x r     gx = r (w gn - x r mean(w gn x r))
+//
+// Bound by HBM: one read and one write per element forward, two reads and one write backward. A thread holds one
+// 16-byte vector of a head, a power of two of neighbouring lanes the head, and a wave one token (or several, where its
+// heads do not fill it) whose heads it walks: the angles depend on the token and the lane's place in the head only, so
+// the sine and cosine are worked out once per token and thread, not per head. The angle is formed in 64 bits, in
+// turns, and reduced to half a turn before it becomes an f32, so far positions keep their accuracy.
+#include "token_common.h"
+
+namespace {
+
+struct RotaryParams {
+  vg_rotary_geom g;
+  const void *q, *k, *gq, *gk;
+  void *oq, *ok;
+  const float *wq, *wk;
+  const void* pos;
+  float* part;            // backward: [blocks][2][D] partial sums of the weight gradients
+  int lph, hps;           // lanes of a head, head slots of a wave's token group
+  int wave_tokens;        // tokens a wave works on at once
+};
+
+constexpr int kUnroll = 4;          // head steps whose loads are in flight together
+constexpr int kBwdBlocks = 512;     // rows of partial weight-gradient sums at most
+
+template <int V>
+__device__ __forceinline__ void angles(const RotaryParams& p, long long token, int t, int b, const double (&freq)[V / 2],
+                                       const int (&axis)[V / 2], float (&c)[V / 2], float (&s)[V / 2]) {
+  const long long at = (long long)b * p.g.pos_sb + (long long)t * p.g.axes;
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+    if (axis[i] >= 0) {
+      const double x = p.g.pos_wide ? (double)((const long long*)p.pos)[at + axis[i]] : (double)((const int*)p.pos)[at + axis[i]];
+      const double turn = x * freq[i];
+      sincospif(2.f * (float)(turn - rint(turn)), &s[i], &c[i]);
+    }
+  }
+}
+
+template <class T, bool BWD>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+  constexpr int V = TokNum<T>::V;
+  const vg_rotary_geom& g = p.g;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int lh = lane & (p.lph - 1);                   // lane in the head
+  const int slot = (lane / p.lph) & (p.hps - 1);       // head slot
+  const int sub = lane / (p.lph * p.hps);              // token of the group
+  const int d0 = lh * V;
+  const bool in = d0 < g.D;
+
+  // the lane's pairs: axis and frequency (in turns per position)
+  double freq[V / 2];
+  int axis[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    axis[i] = -1;
+    freq[i] = 0.0;
+    int d = d0 + 2 * i;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (a < g.axes && axis[i] < 0) {
+        if (d < g.width[a]) {
+          axis[i] = a;
+          freq[i] = exp2(-(double)d / (double)g.width[a] * log2(g.base)) * 0.15915494309189533577;
+        }
+        d -= g.width[a];
+      }
+    }
+    if (!in) axis[i] = -1;
+  }
+  float wq[V], wk[V], sq[V], sk[V];                    // weights, and (backward) sums of their gradients
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    wq[e] = in && p.wq ? p.wq[d0 + e] : 1.f;
+    wk[e] = in && p.wk ? p.wk[d0 + e] : 1.f;
+    sq[e] = sk[e] = 0.f;
+  }
+  const float inv_d = 1.f / (float)g.D;
+  const long long tokens = (long long)g.B * g.T;
+  const long long step = (long long)gridDim.x * 4 * p.wave_tokens;
+  for (long long base = ((long long)blockIdx.x * 4 + wid) * p.wave_tokens; base < tokens; base += step) {
+    const long long token = base + sub;
+    const bool tok = token < tokens;
+    const int b = tok ? (int)(token / g.T) : 0, t = tok ? (int)(token - (long long)b * g.T) : 0;
+    float c[V / 2], s[V / 2];
+    angles<V>(p, token, t, b, freq, axis, c, s);
+    // one side (queries, keys) after the other; kUnroll head steps of loads at a time
+    auto side = [&](const T* x, const vg_heads_layout& lx, const T* gy, const vg_heads_layout& lg, T* out, const vg_heads_layout& lo,
+                    int heads, const float (&w)[V], bool normed, float (&sum)[V]) {
+      const T* xb = x + b * lx.sb + t * lx.st + d0;
+      const T* gb = BWD ? gy + b * lg.sb + t * lg.st + d0 : nullptr;
+      T* ob = out + b * lo.sb + t * lo.st + d0;
+      for (int h0 = 0; h0 < heads; h0 += p.hps * kUnroll) {
+        u32x4 rx[kUnroll], rg[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int h = h0 + u * p.hps + slot;
+          const bool ok = tok && in && h < heads;
+          rx[u] = ok && (!BWD || normed) ? *reinterpret_cast<const u32x4*>(xb + h * lx.sh) : u32x4{0, 0, 0, 0};
+          if constexpr (BWD) rg[u] = ok ? *reinterpret_cast<const u32x4*>(gb + h * lg.sh) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (h0 + u * p.hps >= heads) break;          // uniform over the wave
+          const int h = h0 + u * p.hps + slot;
+          const bool ok = tok && in && h < heads;
+          float xv[V], y[V];
+          tok_widen(rx[u], xv);
+          float r = 1.f;
+          if (normed) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) ss = __builtin_fmaf(xv[e], xv[e], ss);
+            for (int o = p.lph >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            r = 1.f / sqrtf(__builtin_fmaf(ss, inv_d, g.eps));
+          }
+          if constexpr (!BWD) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+              const float n0 = xv[2 * i] * r * w[2 * i], n1 = xv[2 * i + 1] * r * w[2 * i + 1];
+              y[2 * i] = n0 * c[i] - n1 * s[i];
+              y[2 * i + 1] = n0 * s[i] + n1 * c[i];
+            }
+          } else {
+            float gv[V], inner = 0.f;
+            tok_widen(rg[u], gv);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+              const float g0 = gv[2 * i] * c[i] + gv[2 * i + 1] * s[i], g1 = gv[2 * i + 1] * c[i] - gv[2 * i] * s[i];
+              y[2 * i] = g0;
+              y[2 * i + 1] = g1;
+            }
+            if (normed) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float xh = xv[e] * r, wg = w[e] * y[e];
+                if (ok) sum[e] = __builtin_fmaf(y[e], xh, sum[e]);
+                inner = __builtin_fmaf(wg, xh, inner);
+                xv[e] = xh;
+                y[e] = wg;
+              }
+              for (int o = p.lph >> 1; o > 0; o >>= 1) inner += __shfl_xor(inner, o, 64);
+              inner *= inv_d;
+#pragma unroll
+              for (int e = 0; e < V; ++e) y[e] = r * __builtin_fmaf(-xv[e], inner, y[e]);
+            }
+          }
+          if (ok) *reinterpret_cast<u32x4*>(ob + h * lo.sh) = tok_narrow(y);
+        }
+      }
+    };
+    side((const T*)p.q, g.q, (const T*)p.gq, g.gq, (T*)p.oq, g.oq, g.Hq, wq, p.wq != nullptr, sq);
+    if (g.Hk) side((const T*)p.k, g.k, (const T*)p.gk, g.gk, (T*)p.ok, g.ok, g.Hk, wk, p.wk != nullptr, sk);
+  }
+  if constexpr (BWD) {
+    if (!p.part) return;
+    // sums of the block's waves and of the lanes that hold the same elements, in a fixed order
+    __shared__ float red[2][4][64][V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      red[0][wid][lane][e] = sq[e];
+      red[1][wid][lane][e] = sk[e];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * g.D; i += 256) {
+      const int which = i >= g.D, d = which ? i - g.D : i;
+      float v = 0.f;
+      for (int w = 0; w < 4; ++w)
+        for (int l = d / V; l < 64; l += p.lph) v += red[which][w][l][d % V];
+      p.part[(size_t)blockIdx.x * 2 * g.D + i] = v;
+    }
+  }
+}
+
+// gw[which][d] = sum over blocks of part[block][which][d]: 32 columns and 8 row lanes per workgroup
+__global__ void __launch_bounds__(256) rotary_weight_kernel(const float* part, int rows, int D, float* gwq, float* gwk) {
+  __shared__ float red[8][32];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + col;
+  float v = 0.f;
+  if (i < 2 * D)
+    for (int r = row; r < rows; r += 8) v += part[(size_t)r * 2 * D + i];
+  red[row][col] = v;
+  __syncthreads();
+  if (row == 0 && i < 2 * D) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) v += red[r][col];
+    float* out = i < D ? gwq : gwk;
+    if (out) out[i < D ? i : i - D] = v;
+  }
+}
+
+int check_geom(const vg_rotary_geom* g, const void* pos) {
+  VG_REQUIRE(g, "rotary: null geometry");
+  VG_REQUIRE(g->B >= 0 && g->T >= 0 && g->Hq >= 1 && g->Hk >= 0, "rotary: bad sizes B=%d T=%d Hq=%d Hk=%d", g->B, g->T, g->Hq, g->Hk);
+  VG_REQUIRE(g->D >= 8 && g->D <= 256 && g->D % 8 == 0, "rotary: head width %d is not a multiple of 8 from 8 to 256", g->D);
+  VG_REQUIRE(g->axes >= 0 && g->axes <= 4, "rotary: %d axes, 0 to 4 are supported", g->axes);
+  VG_REQUIRE(g->axes == 0 || pos, "rotary: null positions");
+  int64_t total = 0;
+  for (int a = 0; a < g->axes; ++a) {
+    VG_REQUIRE(g->width[a] >= 2 && g->width[a] % 2 == 0, "rotary: axis width %d is not even and positive", g->width[a]);
+    total += g->width[a];
+  }
+  VG_REQUIRE(total <= g->D, "rotary: axis widths sum to %lld, more than the head width %d", (long long)total, g->D);
+  VG_REQUIRE(g->axes == 0 || g->base > 0.0, "rotary: base must be positive");
+  return VG_OK;
+}
+
+void plan(RotaryParams& p, int V) {
+  auto pow2 = [](int n) {
+    int r = 1;
+    while (r < n) r *= 2;
+    return r;
+  };
+  p.lph = pow2((p.g.D + V - 1) / V);
+  const int heads = p.g.Hq > p.g.Hk ? p.g.Hq : p.g.Hk;
+  p.hps = pow2(heads) < 64 / p.lph ? pow2(heads) : 64 / p.lph;
+  p.wave_tokens = 64 / (p.lph * p.hps);
+}
+
+long long wave_groups(const RotaryParams& p) { return ((long long)p.g.B * p.g.T + p.wave_tokens - 1) / p.wave_tokens; }
+
+template <class T>
+int rotary_fwd(const vg_rotary_geom* g, const void* q, const void* k, const float* wq, const float* wk, const void* pos, void* yq,
+               void* yk, void* stream) {
+  const int rc = check_geom(g, pos);
+  if (rc) return rc;
+  if ((long long)g->B * g->T == 0) return VG_OK;
+  VG_REQUIRE(q && yq && (g->Hk == 0 || (k && yk)), "rotary: null tensor");
+  VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->T, g->Hq) && tok_layout_ok<T>(g->oq, yq, g->B, g->T, g->Hq) &&
+                 (g->Hk == 0 || (tok_layout_ok<T>(g->k, k, g->B, g->T, g->Hk) && tok_layout_ok<T>(g->ok, yk, g->B, g->T, g->Hk))),
+             "rotary: a head does not start on a 16-byte border");
+  RotaryParams p = {*g, q, k, nullptr, nullptr, yq, yk, wq, wk, pos, nullptr, 0, 0, 0};
+  plan(p, TokNum<T>::V);
+  long long blocks = (wave_groups(p) + 3) / 4;
+  if (blocks > 4096) blocks = 4096;
+  rotary_kernel<T, false><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(p);
+  VG_CHECK_LAUNCH("rotary");
+  return VG_OK;
+}
+
+int bwd_blocks(const RotaryParams& p) {
+  const long long blocks = (wave_groups(p) + 3) / 4;
+  return (int)(blocks < kBwdBlocks ? blocks : kBwdBlocks);
+}
+
+template <class T>
+int rotary_bwd(const vg_rotary_geom* g, const void* q, const void* k, const float* wq, const float* wk, const void* pos,
+               const void* gyq, const void* gyk, void* gq, void* gk, float* gwq, float* gwk, void* workspace, size_t workspace_bytes,
+               void* stream) {
+  const int rc = check_geom(g, pos);
+  if (rc) return rc;
+  VG_REQUIRE((!gwq || wq) && (!gwk || wk), "rotary: gradient of a weight that is not there");
+  const bool sums = gwq || gwk;
+  hipStream_t st = (hipStream_t)stream;
+  RotaryParams p = {*g, q, k, gyq, gyk, gq, gk, wq, wk, pos, nullptr, 0, 0, 0};
+  plan(p, TokNum<T>::V);
+  int blocks = 0;
+  if ((long long)g->B * g->T != 0) {
+    VG_REQUIRE(gyq && gq && (g->Hk == 0 || (gyk && gk)) && (!wq || q) && (!wk || g->Hk == 0 || k), "rotary: null tensor");
+    VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->T, g->Hq) && tok_layout_ok<T>(g->gq, gyq, g->B, g->T, g->Hq) &&
+                   tok_layout_ok<T>(g->oq, gq, g->B, g->T, g->Hq) &&
+                   (g->Hk == 0 || (tok_layout_ok<T>(g->k, k, g->B, g->T, g->Hk) && tok_layout_ok<T>(g->gk, gyk, g->B, g->T, g->Hk) &&
+                                   tok_layout_ok<T>(g->ok, gk, g->B, g->T, g->Hk))),
+               "rotary: a head does not start on a 16-byte border");
+    blocks = bwd_blocks(p);
+    if (sums) {
+      if (!workspace || workspace_bytes < (size_t)blocks * 2 * g->D * sizeof(float))
+        return vg_fail(VG_ERR_WORKSPACE, "rotary: workspace of %zu bytes is too small", workspace_bytes);
+      p.part = (float*)workspace;
+    }
+    rotary_kernel<T, true><<<blocks, 256, 0, st>>>(p);
+    VG_CHECK_LAUNCH("rotary backward");
+  }
+  if (sums) {      // (no tokens: zeros)
+    rotary_weight_kernel<<<(2 * g->D + 31) / 32, 256, 0, st>>>(p.part, blocks, g->D, gwq, gwk);
+    VG_CHECK_LAUNCH("rotary weight gradient");
+  }
+  return VG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vg_qk_norm_rotary_workspace_bytes(const vg_rotary_geom* g) {
+  if (check_geom(g, g)) return 0;
+  return (size_t)kBwdBlocks * 2 * g->D * sizeof(float);
+}
+int vg_qk_norm_rotary_fwd(const vg_rotary_geom* g, const float* q, const float* k, const float* wq, const float* wk, const void* pos,
+                          float* yq, float* yk, void* stream) {
+  return rotary_fwd<float>(g, q, k, wq, wk, pos, yq, yk, stream);
+}
+int vg_qk_norm_rotary_fwd_h(const vg_rotary_geom* g, const void* q, const void* k, const float* wq, const float* wk, const void* pos,
+                            void* yq, void* yk, void* stream) {
+  return rotary_fwd<__bf16>(g, q, k, wq, wk, pos, yq, yk, stream);
+}
+int vg_qk_norm_rotary_bwd(const vg_rotary_geom* g, const float* q, const float* k, const float* wq, const float* wk, const void* pos,
+                          const float* gyq, const float* gyk, float* gq, float* gk, float* gwq, float* gwk, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  return rotary_bwd<float>(g, q, k, wq, wk, pos, gyq, gyk, gq, gk, gwq, gwk, workspace, workspace_bytes, stream);
+}
+int vg_qk_norm_rotary_bwd_h(const vg_rotary_geom* g, const void* q, const void* k, const float* wq, const float* wk, const void* pos,
+                            const void* gyq, const void* gyk, void* gq, void* gk, float* gwq, float* gwk, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  return rotary_bwd<__bf16>(g, q, k, wq, wk, pos, gyq, gyk, gq, gk, gwq, gwk, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

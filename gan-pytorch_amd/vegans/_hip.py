@@ -7,7 +7,7 @@ the call raises.
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libvegans_hip.so")
 
 ACT_NONE, ACT_RELU, ACT_LRELU, ACT_TANH, ACT_SIGMOID = 0, 1, 2, 3, 4
+GATES = {"sigmoid": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 
 class ConvGeom(Structure):
@@ -41,8 +42,28 @@ class SgdCfg(Structure):
                 ("clamp_lo", c_float), ("clamp_hi", c_float)]
 
 
+class HeadsLayout(Structure):
+    """Mirror of vg_heads_layout: element strides of batch, token and head."""
+    _fields_ = [(n, c_int64) for n in ("sb", "st", "sh")]
+
+
+class RotaryGeom(Structure):
+    """Mirror of vg_rotary_geom."""
+    _fields_ = ([(n, c_int32) for n in ("B", "T", "Hq", "Hk", "D", "axes")] + [("width", c_int32 * 4), ("pos_wide", c_int32),
+                ("eps", c_float), ("base", c_double), ("pos_sb", c_int64)] +
+                [(n, HeadsLayout) for n in ("q", "k", "oq", "ok", "gq", "gk")])
+
+
+class AttentionGeom(Structure):
+    """Mirror of vg_attention_geom."""
+    _fields_ = ([(n, c_int32) for n in ("B", "Tq", "Tk", "Hq", "Hk", "D")] + [("scale", c_float)] +
+                [(n, HeadsLayout) for n in ("q", "k", "v", "o", "go", "gq", "gk", "gv")])
+
+
 _P = c_void_p  # device pointers and the stream travel as void*
 _G = POINTER(ConvGeom)
+_RG = POINTER(RotaryGeom)
+_AG = POINTER(AttentionGeom)
 
 # name -> (restype, argtypes); kept in one table so tests can compare it with the header.
 SIGNATURES = {
@@ -159,6 +180,30 @@ SIGNATURES = {
     "vg_act_fwd_h": (c_int, [_P, _P, c_size_t, c_int, c_float, _P]),
     "vg_act_bwd_h": (c_int, [_P, _P, _P, c_size_t, c_int, c_float, _P]),
     "vg_act_dbwd_ref_h": (c_int, [_P, _P, _P, _P, c_size_t, c_int, _P]),
+    # token operators
+    "vg_qk_norm_rotary_workspace_bytes": (c_size_t, [_RG]),
+    "vg_qk_norm_rotary_fwd": (c_int, [_RG] + [_P] * 8),
+    "vg_qk_norm_rotary_fwd_h": (c_int, [_RG] + [_P] * 8),
+    "vg_qk_norm_rotary_bwd": (c_int, [_RG] + [_P] * 12 + [c_size_t, _P]),
+    "vg_qk_norm_rotary_bwd_h": (c_int, [_RG] + [_P] * 12 + [c_size_t, _P]),
+    "vg_attention_workspace_bytes": (c_size_t, [_AG, c_int]),
+    "vg_attention_fwd": (c_int, [_AG] + [_P] * 8 + [c_size_t, _P]),
+    "vg_attention_fwd_h": (c_int, [_AG] + [_P] * 8 + [c_size_t, _P]),
+    "vg_attention_bwd": (c_int, [_AG] + [_P] * 12 + [c_size_t, _P]),
+    "vg_attention_bwd_h": (c_int, [_AG] + [_P] * 12 + [c_size_t, _P]),
+    "vg_gated_linear_fwd": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
+    "vg_gated_linear_fwd_h": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
+    "vg_gated_linear_bwd": (c_int, [c_int] * 2 + [_P] * 4 + [c_int, _P]),
+    "vg_gated_linear_bwd_h": (c_int, [c_int] * 2 + [_P] * 4 + [c_int, _P]),
+    "vg_gated_linear_partial_rows": (c_int, [c_int, c_int]),
+    "vg_gated_linear_recomputes_h": (c_int, [c_int] * 3),
+    "vg_gated_linear_rebwd_h": (c_int, [c_int] * 3 + [_P] * 6 + [c_int, _P]),
+    "vg_gated_linear_gx_workspace_bytes": (c_size_t, [c_int] * 3),
+    "vg_gated_linear_gw_workspace_bytes": (c_size_t, [c_int] * 3),
+    "vg_gated_linear_gx": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
+    "vg_gated_linear_gx_h": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
+    "vg_gated_linear_gw": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
+    "vg_gated_linear_gw_h": (c_int, [c_int] * 3 + [_P] * 3 + [c_int, _P, c_size_t, _P]),
 }
 
 _lib = None

@@ -19,7 +19,10 @@ are kept channels_last as well ([Co][kh][kw][Ci] in memory).  Tensors that arriv
 re-laid-out by the layout kernels, never by torch.
 """
 import collections
+import contextlib
 import ctypes
+import functools
+import math
 import os
 from ctypes import c_float, c_int, c_size_t
 
@@ -1819,3 +1822,422 @@ def flatten(x):
     if getattr(x, "_vg_no_grad_sink", False):
         out._vg_no_grad_sink = True
     return out
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# token operators: per-head norm with rotation, attention, gated linear layer
+# ----------------------------------------------------------------------------------------------------------------
+# Their scratch is allocated per call (the caching allocator keeps it to the calling stream, a capture keeps it in its
+# graph's pool), so calls on any streams and graphs replayed side by side share none. Their gradients cannot be
+# differentiated again: the backward pass of a gradient penalty through a critic that contains one raises.
+class _FirstOrderFn(Function):
+    """A gradient as computed, tied to the tensors it depends on: differentiating it raises (left untied it would
+    silently count as a constant)."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise _hip.HipError("second derivatives of the token operators (qk_norm_rotary, attention, self_attention, gated_linear) "
+                            "are not implemented: a critic under a gradient penalty cannot contain them")
+
+
+def _first_order(backward):
+    """Backward passes of the token operators: checked against captures (_check_capture), run without recording, results
+    tied to their sources where a graph is being built (create_graph=True)."""
+
+    @functools.wraps(backward)
+    def run(ctx, *gouts):
+        _check_capture(ctx)
+        with torch.no_grad():
+            found = backward(ctx, *gouts)
+        if not torch.is_grad_enabled():
+            return found
+        sources = [t for t in ctx.saved_tensors + getattr(ctx, "params", ()) + gouts if torch.is_tensor(t) and t.requires_grad]
+        return tuple(_FirstOrderFn.apply(g, *sources) if torch.is_tensor(g) and sources else g for g in found)
+
+    return run
+
+
+def _on(t):
+    """Context in which calls for `t` are enqueued: its device, when that is not the current one."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _scratch(nbytes, device):
+    """(pointer, size) arguments and the buffer behind them, which the caller keeps until its calls are enqueued."""
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return (ctypes.c_void_p(buf.data_ptr()) if nbytes else None, c_size_t(nbytes)), buf
+
+
+def _token_tensor(t, what, dims):
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise _hip.HipError("%s must be a tensor on the GPU: the engine only runs on the GPU" % what)
+    if t.dtype not in (F32, BF16):
+        raise _hip.HipError("%s is %s: expected float32 or bfloat16" % (what, t.dtype))
+    if t.dim() != dims:
+        raise _hip.HipError("%s must be %d-d, got shape %s" % (what, dims, tuple(t.shape)))
+
+
+def _heads_ok(t):
+    """Whether the kernels can read [batch, tokens, heads, width] tensor `t` as it lies: contiguous heads that start on
+    16-byte borders. (What the strides of a dimension of size one are does not matter.)"""
+    vec = 16 // t.element_size()
+    return ((t.shape[3] == 1 or t.stride(3) == 1) and t.data_ptr() % 16 == 0 and
+            all(t.shape[i] <= 1 or t.stride(i) % vec == 0 for i in range(3)))
+
+
+def _heads_in(t, what):
+    _token_tensor(t, what, 4)
+    if t.numel() and not _heads_ok(t):
+        raise _hip.HipError("%s with strides %s: a head's elements must be contiguous and start on a 16-byte border" %
+                            (what, tuple(t.stride())))
+    return t
+
+
+def _heads_grad(g):
+    """A gradient as the kernels read it (autograd may hand back expanded or sliced ones)."""
+    return g if _heads_ok(g) else g.contiguous()
+
+
+def _layout(t):
+    return _hip.HeadsLayout(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _same_kind(first, *others):
+    for t in others:
+        if t is not None and (t.dtype != first.dtype or t.device != first.device):
+            raise _hip.HipError("tensors of one call differ in type or device: %s on %s and %s on %s" %
+                                (first.dtype, first.device, t.dtype, t.device))
+
+
+def _channel_param(t, size, like, what):
+    """f32 vector of `size` channel parameters on the device of `like` (None stays None)."""
+    if t is None:
+        return
+    if not t.is_cuda or t.device != like.device or t.dtype != F32 or tuple(t.shape) != (size,) or not t.is_contiguous():
+        raise _hip.HipError("%s must be a contiguous float32 vector of %d elements on %s, got %s %s on %s" %
+                            (what, size, like.device, t.dtype, tuple(t.shape), t.device))
+
+
+# A gradient that autograd itself accumulates into a leaf goes through that leaf's accumulation node, which belongs to
+# the stream it was made on and lives as long as any graph over the leaf. A backward pass captured into a HIP graph
+# while an eager graph of the same leaf is alive would pull that eager stream into the capture, which ends the
+# process. The nodes are therefore marked when an operator first sees them, and such a backward pass raises instead.
+# (Inside a training iteration the gradient ledger takes the parameters' gradients and no such node runs.)
+def _mark_leaves(ctx, *tensors):
+    ctx.leaf_nodes = []
+    for t in tensors:
+        if t is not None and t.requires_grad and t.is_leaf:
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            node.metadata.setdefault("vg_captured", torch.cuda.is_current_stream_capturing())
+            ctx.leaf_nodes.append((t, node))
+
+
+def _check_capture(ctx):
+    if not ctx.leaf_nodes or not torch.cuda.is_current_stream_capturing():
+        return
+    for t, node in ctx.leaf_nodes:
+        if not grads.accepts(t) and not node.metadata.get("vg_captured", True):
+            raise _hip.HipError("backward pass captured while an eager graph of the same leaf tensor is alive: drop the "
+                                "eager outputs (and losses) before the capture")
+
+
+def _rotary_geom(q, k, pos, axes, base, eps):
+    """Checked geometry of a norm-and-rotate call: q, k [B, T, heads, D] (as they will be read)."""
+    b, t, hq, d = q.shape
+    if k.shape[0] != b or k.shape[1] != t or k.shape[3] != d:
+        raise _hip.HipError("queries %s and keys %s differ in batch, tokens or head width" % (tuple(q.shape), tuple(k.shape)))
+    if d % 8 or not 8 <= d <= 256:
+        raise _hip.HipError("head width %d is not a multiple of 8 from 8 to 256" % d)
+    axes = tuple(int(a) for a in axes)
+    if len(axes) > 4 or any(a < 2 or a % 2 for a in axes) or sum(axes) > d:
+        raise _hip.HipError("axes %s: at most four even widths whose sum is at most the head width %d" % (axes, d))
+    if not base > 0 or not eps >= 0:
+        raise _hip.HipError("base must be positive and eps not negative, got %s and %s" % (base, eps))
+    g = _hip.RotaryGeom(B=b, T=t, Hq=hq, Hk=k.shape[2], D=d, axes=len(axes), eps=eps, base=base)
+    for i, a in enumerate(axes):
+        g.width[i] = a
+    if axes:
+        if pos is None or not pos.is_cuda or pos.device != q.device or pos.dtype not in (torch.int32, torch.int64):
+            raise _hip.HipError("positions must be an int32 or int64 tensor on the device of the queries")
+        if tuple(pos.shape) not in ((t, len(axes)), (b, t, len(axes))) or not pos.is_contiguous():
+            raise _hip.HipError("positions must be contiguous [tokens, axes] or [batch, tokens, axes], got %s for %d tokens, "
+                                "%d axes" % (tuple(pos.shape), t, len(axes)))
+        g.pos_wide = int(pos.dtype == torch.int64)
+        g.pos_sb = t * len(axes) if pos.dim() == 3 else 0
+    return g
+
+
+def _raw_rotary_fwd(g, q, k, wq, wk, pos, yq, yk):
+    g.q, g.k, g.oq, g.ok = _layout(q), _layout(k), _layout(yq), _layout(yk)
+    call(_A("vg_qk_norm_rotary_fwd", q), ctypes.byref(g), _p(q), _p(k), _ptr(wq), _ptr(wk),
+         ctypes.c_void_p(pos.data_ptr()) if pos is not None else None, _p(yq), _p(yk), _stream())
+
+
+def _raw_rotary_bwd(g, q, k, wq, wk, pos, gyq, gyk, gq, gk, want_weights):
+    """Writes gq, gk; returns the gradients of the weights (None where there is no weight or none is wanted)."""
+    g.q, g.k, g.gq, g.gk, g.oq, g.ok = (_layout(t) for t in (q, k, gyq, gyk, gq, gk))
+    gwq, gwk = (torch.empty_like(w) if w is not None and want else None for w, want in zip((wq, wk), want_weights))
+    scratch, keep = _scratch(_hip.load().vg_qk_norm_rotary_workspace_bytes(ctypes.byref(g)) if gwq is not None or gwk is not None else 0,
+                             q.device)
+    call(_A("vg_qk_norm_rotary_bwd", q), ctypes.byref(g), _p(q), _p(k), _ptr(wq), _ptr(wk),
+         ctypes.c_void_p(pos.data_ptr()) if pos is not None else None, _p(gyq), _p(gyk), _p(gq), _p(gk), _ptr(gwq), _ptr(gwk),
+         *scratch, _stream())
+    return gwq, gwk
+
+
+class QkNormRotaryFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pos, axes, base, eps):
+        g = _rotary_geom(q, k, pos, axes, base, eps)
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        with _on(q):
+            _raw_rotary_fwd(g, q, k, wq, wk, pos, yq, yk)
+        ctx.g, ctx.label = g, grads.ticket()
+        _mark_leaves(ctx, q, k, wq, wk)
+        ctx.save_for_backward(q, k, wq, wk, pos)
+        return yq, yk
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, gyq, gyk):
+        q, k, wq, wk, pos = ctx.saved_tensors
+        lab, need = ctx.label, ctx.needs_input_grad
+        gyq, gyk = _heads_grad(gyq), _heads_grad(gyk)
+        gq, gk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        params = not inputs_only.active
+        with _on(q):
+            gwq, gwk = _raw_rotary_bwd(ctx.g, q, k, wq, wk, pos, gyq, gyk, gq, gk, (params and need[2], params and need[3]))
+        return (gq if need[0] else None, gk if need[1] else None, grads.route(wq, lab + (0,), gwq) if wq is not None else None,
+                grads.route(wk, lab + (1,), gwk) if wk is not None else None, None, None, None, None)
+
+
+def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, axes=(), base=10000.0, eps=1e-6):
+    """Root-mean-square norm of every query and key head and the rotation of the heads by the tokens' positions, in one
+    pass. q [batch, tokens, heads, width] and k [batch, tokens, key heads, width] may be slices of one packed projection.
+
+    q_weight / k_weight [width] (float32): scale of the norm, shared by the heads; None: that side is not normalised.
+    positions [tokens, len(axes)] or [batch, tokens, len(axes)] (int32 / int64): a token's place on every axis (row and
+    column of a feature map, frame of a clip). axes: how many elements of a head belong to each axis, in order; pair
+    (2i, 2i+1) of a section of width d turns by position * base^(-2i / d); elements behind the sections are not turned."""
+    _heads_in(q, "queries")
+    _heads_in(k, "keys")
+    _same_kind(q, k)
+    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _channel_param(w, q.shape[3], q, what)
+    return QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, tuple(axes), float(base), float(eps))
+
+
+def _attention_geom(q, k, v, q_lengths, k_lengths, scale):
+    b, tq, hq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise _hip.HipError("queries %s, keys %s and values %s do not belong together" %
+                            (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if not hq or not k.shape[2] or hq % k.shape[2]:
+        raise _hip.HipError("%d query heads are not a multiple of %d key heads" % (hq, k.shape[2]))
+    if d % 8 or not 8 <= d <= 128:
+        raise _hip.HipError("head width %d is not a multiple of 8 from 8 to 128" % d)
+    for n, what in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths")):
+        if n is not None and (not n.is_cuda or n.device != q.device or n.dtype != torch.int32 or tuple(n.shape) != (b,) or
+                              not n.is_contiguous()):
+            raise _hip.HipError("%s must be a contiguous int32 tensor [%d] on the device of the queries" % (what, b))
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise _hip.HipError("scale must be finite, got %s" % scale)
+    return _hip.AttentionGeom(B=b, Tq=tq, Tk=k.shape[1], Hq=hq, Hk=k.shape[2], D=d, scale=scale)
+
+
+def _lengths_ptr(t):
+    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def _raw_attention_fwd(g, q, k, v, q_lengths, k_lengths, o, save):
+    """Writes o; returns the row sums' logarithms when `save`."""
+    g.q, g.k, g.v, g.o = (_layout(t) for t in (q, k, v, o))
+    lse = torch.empty((g.B, g.Hk, g.Tq * (g.Hq // g.Hk)), dtype=F32, device=q.device) if save else None
+    scratch, keep = _scratch(_hip.load().vg_attention_workspace_bytes(ctypes.byref(g), 0), q.device)
+    call(_A("vg_attention_fwd", q), ctypes.byref(g), _p(q), _p(k), _p(v), _lengths_ptr(q_lengths), _lengths_ptr(k_lengths), _p(o),
+         _ptr(lse), *scratch, _stream())
+    return lse
+
+
+def _raw_attention_bwd(g, q, k, v, o, lse, go, q_lengths, k_lengths, gq, gk, gv):
+    g.q, g.k, g.v, g.o, g.go = (_layout(t) for t in (q, k, v, o, go))
+    none = _hip.HeadsLayout(0, 0, 0)
+    g.gq, g.gk, g.gv = (_layout(t) if t is not None else none for t in (gq, gk, gv))
+    scratch, keep = _scratch(_hip.load().vg_attention_workspace_bytes(ctypes.byref(g), 1), q.device)
+    call(_A("vg_attention_bwd", q), ctypes.byref(g), _p(q), _p(k), _p(v), _p(o), _ptr(lse), _p(go), _lengths_ptr(q_lengths),
+         _lengths_ptr(k_lengths), _p(gq), _p(gk), _p(gv), *scratch, _stream())
+
+
+class AttentionFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_lengths, k_lengths, scale):
+        g = _attention_geom(q, k, v, q_lengths, k_lengths, scale)
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        with _on(q):
+            lse = _raw_attention_fwd(g, q, k, v, q_lengths, k_lengths, o, any(ctx.needs_input_grad))
+        ctx.g = g
+        _mark_leaves(ctx, q, k, v)
+        ctx.save_for_backward(q, k, v, o, lse, q_lengths, k_lengths)
+        return o
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, go):
+        q, k, v, o, lse, q_lengths, k_lengths = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        gq = new(q) if need[0] else None
+        gk, gv = (new(k), new(v)) if need[1] or need[2] else (None, None)
+        with _on(q):
+            _raw_attention_bwd(ctx.g, q, k, v, o, lse, _heads_grad(go), q_lengths, k_lengths, gq, gk, gv)
+        return gq, gk if need[1] else None, gv if need[2] else None, None, None, None
+
+
+def attention(q, k, v, q_lengths=None, k_lengths=None, scale=None):
+    """softmax(scale q k^T) v for q [batch, queries, heads, width], k and v [batch, keys, key heads, width]; heads is a
+    multiple of key heads (query head h reads key head h // (heads // key heads)), scale defaults to width^-1/2.
+
+    q_lengths / k_lengths (int32 [batch], on the GPU): how many queries / keys of each batch element take part. What
+    lies behind them is never used (it may be NaN); rows behind q_lengths and rows without a key are zero, and so are the
+    gradients of what takes no part."""
+    _heads_in(q, "queries")
+    _heads_in(k, "keys")
+    _heads_in(v, "values")
+    _same_kind(q, k, v)
+    return AttentionFn.apply(q, k, v, q_lengths, k_lengths, scale)
+
+
+class SelfAttentionFn(Function):
+    """Norm, rotation and attention over one packed projection: the values are read where they lie and the gradients of
+    queries, keys and values are written into one packed gradient."""
+
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, pos, heads, kv_heads, axes, lengths, base, eps, scale):
+        q, k, v = qkv.split((heads, kv_heads, kv_heads), 2)
+        rg = _rotary_geom(q, k, pos, axes, base, eps)
+        ag = _attention_geom(q, k, v, lengths, lengths, scale)
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        yq, yk, o = new(q), new(k), new(q)
+        with _on(qkv):
+            _raw_rotary_fwd(rg, q, k, wq, wk, pos, yq, yk)
+            lse = _raw_attention_fwd(ag, yq, yk, v, lengths, lengths, o, any(ctx.needs_input_grad))
+        ctx.rg, ctx.ag, ctx.label, ctx.split = rg, ag, grads.ticket(), (heads, kv_heads, kv_heads)
+        _mark_leaves(ctx, qkv, wq, wk)
+        ctx.save_for_backward(qkv, wq, wk, pos, yq, yk, o, lse, lengths)
+        return o
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, go):
+        qkv, wq, wk, pos, yq, yk, o, lse, lengths = ctx.saved_tensors
+        lab, need = ctx.label, ctx.needs_input_grad
+        q, k, v = qkv.split(ctx.split, 2)
+        gqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        gq, gk, gv = gqkv.split(ctx.split, 2)
+        gyq, gyk = torch.empty_like(yq), torch.empty_like(yk)
+        params = not inputs_only.active
+        with _on(qkv):
+            _raw_attention_bwd(ctx.ag, yq, yk, v, o, lse, _heads_grad(go), lengths, lengths, gyq, gyk, gv)
+            gwq, gwk = _raw_rotary_bwd(ctx.rg, q, k, wq, wk, pos, gyq, gyk, gq, gk, (params and need[1], params and need[2]))
+        return (gqkv if need[0] else None, grads.route(wq, lab + (0,), gwq) if wq is not None else None,
+                grads.route(wk, lab + (1,), gwk) if wk is not None else None) + (None,) * 8
+
+
+def self_attention(qkv, heads, kv_heads=None, q_weight=None, k_weight=None, positions=None, axes=(), lengths=None, base=10000.0,
+                   eps=1e-6, scale=None):
+    """`qk_norm_rotary` and `attention` of the tokens of each batch element among themselves. qkv [batch, tokens,
+    heads + 2 * kv_heads, width]: queries, keys and values as one projection leaves them. lengths (int32 [batch]): tokens
+    of each batch element. Returns [batch, tokens, heads, width]."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    _heads_in(qkv, "packed queries, keys and values")
+    if heads < 1 or kv_heads < 1 or qkv.shape[2] != heads + 2 * kv_heads:
+        raise _hip.HipError("packed tensor has %d heads, expected %d + 2 * %d" % (qkv.shape[2], heads, kv_heads))
+    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _channel_param(w, qkv.shape[3], qkv, what)
+    return SelfAttentionFn.apply(qkv, q_weight, k_weight, positions, heads, kv_heads, tuple(axes), lengths, float(base), float(eps),
+                                 scale)
+
+
+class GatedLinearFn(Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, act):
+        lib = _hip.load()
+        xm, wm = to_nhwc(x), _weight_mem(w)
+        m, c, f = xm.shape[0], xm.shape[1], wm.shape[0] // 2
+        with _on(x):
+            if wm.dtype != xm.dtype:        # f32 master of a bf16 layer
+                wm = plane_cache.bf16_copy(wm).view(wm.shape)
+            h = torch.empty((m, f), dtype=xm.dtype, device=xm.device)
+            training = any(ctx.needs_input_grad)
+            again = xm.dtype == BF16 and bool(lib.vg_gated_linear_recomputes_h(m, c, f))
+            z = torch.empty((m, 2 * f), dtype=F32, device=xm.device) if training and not again else None
+            call(_A("vg_gated_linear_fwd", xm), m, c, f, _p(xm), _p(wm), _ptr(bias), _p(h), _ptr(z), act, _stream())
+        ctx.act, ctx.label = act, grads.ticket()
+        _mark_leaves(ctx, x, w, bias)
+        # (wm: what the forward product read; a bf16 copy made here is the one the backward products read)
+        ctx.save_for_backward(xm, wm, bias, z)
+        ctx.params = (w, bias, x)
+        return h
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, gh):
+        lib = _hip.load()
+        xm, wm, bias, z = ctx.saved_tensors
+        w, bias_in, _ = ctx.params
+        lab, need, act = ctx.label, ctx.needs_input_grad, ctx.act
+        m, c, f = xm.shape[0], xm.shape[1], wm.shape[0] // 2
+        gh = _cast_raw(gh if gh.is_contiguous() else gh.contiguous(), xm.dtype)
+        params = not inputs_only.active
+        gx = gw = gb = None
+        with _on(xm):
+            gz = torch.empty((m, 2 * f), dtype=xm.dtype, device=xm.device)
+            want_gb = params and bias is not None and need[2]
+            rows = lib.vg_gated_linear_partial_rows(m, int(z is None))
+            part = torch.empty((rows, 2 * f), dtype=F32, device=xm.device) if want_gb else None
+            if z is None:
+                call("vg_gated_linear_rebwd_h", m, c, f, _p(xm), _p(wm), _ptr(bias), _p(gh), _p(gz), _ptr(part), act, _stream())
+            else:
+                call(_A("vg_gated_linear_bwd", xm), m, f, _ptr(z), _p(gh), _p(gz), _ptr(part), act, _stream())
+            if want_gb:
+                gb = torch.empty(2 * f, dtype=F32, device=xm.device)
+                if rows:
+                    scratch, keep = _scratch(lib.vg_colsum_workspace_bytes(rows, 2 * f), xm.device)
+                    call("vg_colsum", _ptr(part), _ptr(gb), rows, 2 * f, *scratch, _stream())
+                else:
+                    call("vg_fill", _ptr(gb), c_float(0.0), c_size_t(2 * f), _stream())
+            if _wants_input_grad(ctx, xm):
+                gx = torch.empty((m, c), dtype=xm.dtype, device=xm.device)
+                scratch, keep = _scratch(lib.vg_gated_linear_gx_workspace_bytes(m, c, f), xm.device)
+                call(_A("vg_gated_linear_gx", xm), m, c, f, _p(gz), _p(wm), _p(gx), *scratch, _stream())
+            if params and need[1]:
+                gw = torch.empty((2 * f, c), dtype=w.dtype, device=xm.device)
+                scratch, keep = _scratch(lib.vg_gated_linear_gw_workspace_bytes(m, c, f), xm.device)
+                if xm.dtype == BF16:
+                    call("vg_gated_linear_gw_h", m, c, f, _p(gz), _p(xm), _p(gw), int(gw.dtype == F32), *scratch, _stream())
+                else:
+                    call("vg_gated_linear_gw", m, c, f, _p(gz), _p(xm), _p(gw), *scratch, _stream())
+        return gx, grads.route(w, lab, gw), grads.route(bias_in, lab, gb) if bias_in is not None else None, None
+
+
+def gated_linear(x, w, bias=None, act="silu"):
+    """act(x Wg^T + bg) * (x Wu^T + bu): the first half of a gated feed-forward block. x [rows, features], w
+    [2 * out, features] with the gate's rows first, bias [2 * out] (float32) or None; act "silu", "gelu" (exact), "relu" or
+    "sigmoid". With bfloat16 x, w may be bfloat16 or a float32 master (rounded to bfloat16 for the products; its gradient
+    is float32)."""
+    _token_tensor(x, "input", 2)
+    _token_tensor(w, "weight", 2)
+    if w.shape[0] < 2 or w.shape[0] % 2 or w.shape[1] != x.shape[1] or not x.shape[1]:
+        raise _hip.HipError("gated linear layer: input %s and weight %s do not belong together" % (tuple(x.shape), tuple(w.shape)))
+    if w.device != x.device or (w.dtype != x.dtype and w.dtype != F32):
+        raise _hip.HipError("gated linear layer: %s weight on %s with %s input on %s" % (w.dtype, w.device, x.dtype, x.device))
+    _channel_param(bias, w.shape[0], x, "bias")
+    if act not in _hip.GATES:
+        raise _hip.HipError("gate activation %r: expected one of %s" % (act, sorted(_hip.GATES)))
+    return GatedLinearFn.apply(x, w, bias, _hip.GATES[act])

@@ -459,6 +459,95 @@ int vg_act_fwd_h(const void* x, void* y, size_t n, int act, float slope, void* s
 int vg_act_bwd_h(const void* gy, const void* ref, void* gx, size_t n, int act, float slope, void* stream);
 int vg_act_dbwd_ref_h(const void* gg, const void* gy, const void* ref, void* d_ref, size_t n, int act, void* stream);
 
+/* ---- token operators --------------------------------------------------------------------------------------------------
+ * The layers of a generator or critic that works on tokens (the pixels of a feature map, the patches of a clip); the
+ * reference takes such layers from torch inside the user's module (vegans/utils/networks.py:36-47). Queries, keys and
+ * values are [B][T][H][D] with any strides between heads, tokens and batch elements (in elements; the D elements of a
+ * head are contiguous, every head starts on a 16-byte border), so they may be slices of one packed projection. `_h`: bf16
+ * tensors, everything per channel and every saved statistic f32. */
+typedef struct vg_heads_layout {
+  int64_t sb, st, sh;
+} vg_heads_layout;
+
+/* Norm of every query and key head and its rotation by positions on up to four axes, one pass:
+ *   n = x w / sqrt(mean(x^2) + eps)  (w null: n = x);  section a of a head (the first width[0] elements, then width[1], ...):
+ *   pair (2i, 2i+1) turns by pos[b][t][a] * base^(-2i / width[a]); elements behind the sections are not turned.
+ * pos: int32, or int64 where pos_wide, [B][T][axes], batch stride pos_sb elements (0: one grid for the whole batch).
+ * Forward: inputs at layouts q, k, outputs at oq, ok. Backward: inputs at q, k, output gradients at gq, gk, input
+ * gradients written at oq, ok; gwq, gwk [D] nullable. Hk may be 0. D is a multiple of 8 up to 256. */
+typedef struct vg_rotary_geom {
+  int32_t B, T, Hq, Hk, D;
+  int32_t axes, width[4];
+  int32_t pos_wide;
+  float eps;
+  double base;
+  int64_t pos_sb;
+  vg_heads_layout q, k, oq, ok, gq, gk;
+} vg_rotary_geom;
+size_t vg_qk_norm_rotary_workspace_bytes(const vg_rotary_geom* g);   /* backward with weight gradients */
+int vg_qk_norm_rotary_fwd(const vg_rotary_geom* g, const float* q, const float* k, const float* wq, const float* wk, const void* pos,
+                          float* yq, float* yk, void* stream);
+int vg_qk_norm_rotary_fwd_h(const vg_rotary_geom* g, const void* q, const void* k, const float* wq, const float* wk, const void* pos,
+                            void* yq, void* yk, void* stream);
+int vg_qk_norm_rotary_bwd(const vg_rotary_geom* g, const float* q, const float* k, const float* wq, const float* wk, const void* pos,
+                          const float* gyq, const float* gyk, float* gq, float* gk, float* gwq, float* gwk, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int vg_qk_norm_rotary_bwd_h(const vg_rotary_geom* g, const void* q, const void* k, const float* wq, const float* wk, const void* pos,
+                            const void* gyq, const void* gyk, void* gq, void* gk, float* gwq, float* gwk, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Attention o = softmax(scale q k^T) v; query head h reads key head h / (Hq / Hk). q_len, k_len: int32 [B] on the device,
+ * nullable (all): queries and keys at or past them take no part and may hold anything; rows without a key, and rows past
+ * q_len, are zero, as are the gradients of everything that takes no part. Lengths outside 0..T are clamped. lse [B][Hk]
+ * [Tq * Hq / Hk] f32 (log2 of the row sums; nullable in the forward pass) is what the backward pass needs besides o.
+ * Backward: gq, and gk with gv, may be null (not wanted).
+ * D is a multiple of 8 up to 128. */
+typedef struct vg_attention_geom {
+  int32_t B, Tq, Tk, Hq, Hk, D;
+  float scale;
+  vg_heads_layout q, k, v, o, go, gq, gk, gv;
+} vg_attention_geom;
+size_t vg_attention_workspace_bytes(const vg_attention_geom* g, int backward);
+int vg_attention_fwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const int32_t* q_len, const int32_t* k_len,
+                     float* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int vg_attention_fwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len,
+                       void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int vg_attention_bwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const float* o, const float* lse,
+                     const float* go, const int32_t* q_len, const int32_t* k_len, float* gq, float* gk, float* gv, void* workspace,
+                     size_t workspace_bytes, void* stream);
+int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                       const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Gated linear layer h[M][F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M][C], w [2F][C] (gate rows first), bias [2F] nullable.
+ *   vg_gated_linear_fwd       z [M][2F] f32 (pre-activations, for the backward pass) nullable
+ *   vg_gated_linear_bwd       gz [M][2F] = gradient of the pre-activations from z and gh
+ *   vg_gated_linear_rebwd_h   the same from x and w (what vg_gated_linear_recomputes_h prefers to a stored z)
+ *   vg_gated_linear_gx / _gw  gx = gz w, gw = gz^T x (_h: f32 where gw_f32, else bf16); scratch: *_workspace_bytes
+ * gb_part [vg_gated_linear_partial_rows(M, recompute)][2F] f32, nullable: its column sums are the bias gradient. */
+#define VG_GATE_SIGMOID 0
+#define VG_GATE_RELU 1
+#define VG_GATE_GELU 2
+#define VG_GATE_SILU 3
+int vg_gated_linear_fwd(int M, int C, int F, const float* x, const float* w, const float* bias, float* h, float* z, int act, void* stream);
+int vg_gated_linear_fwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, void* h, float* z, int act, void* stream);
+int vg_gated_linear_bwd(int M, int F, const float* z, const float* gh, float* gz, float* gb_part, int act, void* stream);
+int vg_gated_linear_bwd_h(int M, int F, const float* z, const void* gh, void* gz, float* gb_part, int act, void* stream);
+int vg_gated_linear_partial_rows(int M, int recompute);
+int vg_gated_linear_recomputes_h(int M, int C, int F);
+int vg_gated_linear_rebwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const void* gh, void* gz, float* gb_part,
+                            int act, void* stream);
+size_t vg_gated_linear_gx_workspace_bytes(int M, int C, int F);
+size_t vg_gated_linear_gw_workspace_bytes(int M, int C, int F);
+int vg_gated_linear_gx(int M, int C, int F, const float* gz, const float* w, float* gx, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int vg_gated_linear_gw(int M, int C, int F, const float* gz, const float* x, float* gw, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int vg_gated_linear_gx_h(int M, int C, int F, const void* gz, const void* w, void* gx, void* workspace, size_t workspace_bytes,
+                         void* stream);
+int vg_gated_linear_gw_h(int M, int C, int F, const void* gz, const void* x, void* gw, int gw_f32, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

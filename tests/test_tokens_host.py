@@ -1,0 +1,117 @@
+"""Token operators on the host: argument checks of the C entry points (nothing is launched) and of the Python operators
+without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _layouts(g, heads, d):
+    from vegans import _hip
+    for name, _ in g._fields_:
+        if isinstance(getattr(g, name), _hip.HeadsLayout):
+            setattr(g, name, _hip.HeadsLayout(heads * d * 4, heads * d, d))
+    return g
+
+
+def _rotary(**kw):
+    from vegans import _hip
+    g = _hip.RotaryGeom(**{**dict(B=2, T=4, Hq=2, Hk=1, D=16, axes=1, eps=1e-6, base=1e4), **kw})
+    g.width[0] = 8
+    return _layouts(g, 3, 16)
+
+
+def _attention(**kw):
+    from vegans import _hip
+    return _layouts(_hip.AttentionGeom(**{**dict(B=2, Tq=4, Tk=4, Hq=2, Hk=1, D=16, scale=0.25), **kw}), 3, 16)
+
+
+DUMMY = ctypes.c_void_p(256)        # never dereferenced
+
+
+def _text(lib):
+    return lib.vg_last_error().decode()
+
+
+def test_rotary_arguments_are_checked_before_any_launch():
+    from vegans import _hip
+    lib = _hip.load()
+
+    def fwd(g, q=DUMMY, pos=DUMMY):
+        return lib.vg_qk_norm_rotary_fwd(ctypes.byref(g), q, DUMMY, DUMMY, DUMMY, pos, DUMMY, DUMMY, None)
+
+    for g, word in ((_rotary(D=12), "head width"), (_rotary(D=264), "head width"), (_rotary(axes=5), "axes"), (_rotary(Hq=0), "bad sizes"),
+                    (_rotary(T=-1), "bad sizes"), (_rotary(base=0.0), "base")):
+        assert fwd(g) == -1 and word in _text(lib), _text(lib)
+        assert lib.vg_qk_norm_rotary_workspace_bytes(ctypes.byref(g)) == 0
+    g = _rotary()
+    g.width[0] = 18
+    assert fwd(g) == -1 and "more than the head width" in _text(lib)
+    g.width[0] = 3
+    assert fwd(g) == -1 and "not even" in _text(lib)
+    assert fwd(_rotary(), q=None) == -1 and "null" in _text(lib)
+    assert fwd(_rotary(), pos=None) == -1 and "null positions" in _text(lib)
+    assert fwd(_rotary(), q=ctypes.c_void_p(264)) == -1 and "16-byte" in _text(lib)
+    g = _rotary()
+    g.q.sh = 18
+    assert fwd(g) == -1 and "16-byte" in _text(lib)
+    assert lib.vg_qk_norm_rotary_fwd(None, DUMMY, DUMMY, DUMMY, DUMMY, DUMMY, DUMMY, DUMMY, None) == -1
+    need = lib.vg_qk_norm_rotary_workspace_bytes(ctypes.byref(_rotary()))
+    assert need > 0
+    rc = lib.vg_qk_norm_rotary_bwd(ctypes.byref(_rotary()), *[DUMMY] * 11, DUMMY, 8, None)
+    assert rc == -3 and "too small" in _text(lib)
+    rc = lib.vg_qk_norm_rotary_bwd(ctypes.byref(_rotary()), DUMMY, DUMMY, None, DUMMY, *[DUMMY] * 7, DUMMY, need, None)
+    assert rc == -1 and "not there" in _text(lib)
+    assert fwd(_rotary(T=0), q=None) == 0       # nothing to do
+
+
+def test_attention_arguments_are_checked_before_any_launch():
+    from vegans import _hip
+    lib = _hip.load()
+
+    def fwd(g, q=DUMMY, ws=None, size=0):
+        return lib.vg_attention_fwd(ctypes.byref(g), q, DUMMY, DUMMY, None, None, DUMMY, None, ws, size, None)
+
+    for g, word in ((_attention(D=12), "head width"), (_attention(D=136), "head width"), (_attention(Hq=3, Hk=2), "multiple"),
+                    (_attention(Tk=-1), "bad sizes"), (_attention(Hk=0), "bad sizes"), (_attention(scale=float("inf")), "finite"),
+                    (_attention(Tq=1 << 29, Hq=4), "too many"), (_attention(Tk=1 << 30), "too many"),
+                    (_attention(B=1 << 20, Tq=1 << 14), "too many")):
+        assert fwd(g) == -1 and word in _text(lib), _text(lib)
+        assert lib.vg_attention_workspace_bytes(ctypes.byref(g), 0) == 0
+    assert fwd(_attention(), q=None) == -1 and "null" in _text(lib)
+    assert fwd(_attention(), q=ctypes.c_void_p(8)) == -1 and "16-byte" in _text(lib)
+    # one query over many keys: the keys are split, and the partial results need space
+    g = _attention(B=1, Tq=1, Tk=1 << 14)
+    need = lib.vg_attention_workspace_bytes(ctypes.byref(g), 0)
+    assert need > 0
+    assert fwd(g, ws=DUMMY, size=need - 1) == -3 and "are needed" in _text(lib)
+    assert fwd(g, ws=ctypes.c_void_p(264), size=need) == -1 and "aligned" in _text(lib)
+    assert fwd(_attention(B=0), q=None) == 0
+    rc = lib.vg_attention_bwd(ctypes.byref(_attention()), *[DUMMY] * 8, DUMMY, DUMMY, None, DUMMY, 1 << 20, None)
+    assert rc == -1 and "null" in _text(lib)                 # keys' gradient without values'
+    rc = lib.vg_attention_bwd(ctypes.byref(_attention()), *[DUMMY] * 8, DUMMY, DUMMY, DUMMY, None, 0, None)
+    assert rc == -3
+
+
+def test_gated_arguments_are_checked_before_any_launch():
+    from vegans import _hip
+    lib = _hip.load()
+    assert lib.vg_gated_linear_fwd(4, 8, 8, None, DUMMY, None, DUMMY, None, 3, None) == -1 and "null" in _text(lib)
+    assert lib.vg_gated_linear_fwd(4, 8, 8, DUMMY, DUMMY, None, DUMMY, None, 4, None) == -1 and "activation" in _text(lib)
+    assert lib.vg_gated_linear_fwd(4, 0, 8, DUMMY, DUMMY, None, DUMMY, None, 3, None) == -1 and "bad sizes" in _text(lib)
+    assert lib.vg_gated_linear_fwd(1 << 30, 8, 8, DUMMY, DUMMY, None, DUMMY, None, 3, None) == -1 and "too many" in _text(lib)
+    assert lib.vg_gated_linear_fwd(0, 8, 8, None, None, None, None, None, 3, None) == 0
+    need = lib.vg_gated_linear_gw_workspace_bytes(4096, 64, 32)
+    assert need > 0 and need % (64 * 64 * 4) == 0
+    assert lib.vg_gated_linear_gw(4096, 64, 32, DUMMY, DUMMY, DUMMY, DUMMY, need - 1, None) == -3
+    assert lib.vg_gated_linear_gx(4096, 64, 32, None, DUMMY, DUMMY, None, 0, None) == -1
+
+
+def test_operators_refuse_cpu_tensors():
+    from vegans import _hip
+    from vegans.engine import ops
+    q = torch.zeros(1, 4, 2, 16)
+    for call in (lambda: ops.qk_norm_rotary(q, q), lambda: ops.attention(q, q, q), lambda: ops.self_attention(torch.zeros(1, 4, 6, 16), 2),
+                 lambda: ops.gated_linear(torch.zeros(4, 8), torch.zeros(6, 8))):
+        with pytest.raises(_hip.HipError, match="GPU"):
+            call()

@@ -70,6 +70,10 @@ struct RowFrag;
 template <int DP>
 struct RowFrag<__bf16, DP> {
   bf16x8 f[DP / 16];
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) f[s] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, f[s]) ^ 0x80008000u);
+  }
   __device__ __forceinline__ void load(const __bf16* row, int D, int h, bool ok) {
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
@@ -82,6 +86,10 @@ struct RowFrag<__bf16, DP> {
 template <int DP>
 struct RowFrag<float, DP> {
   f32x4 f[DP / 8];
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (int s = 0; s < DP / 8; ++s) f[s] = -f[s];
+  }
   __device__ __forceinline__ void load(const float* row, int D, int h, bool ok) {
 #pragma unroll
     for (int s = 0; s < DP / 8; ++s) {
@@ -154,17 +162,35 @@ __device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int
 }
 
 // Stages ROWS rows of up to DP elements in registers on their way to an LDS tile; what is out of range becomes zero.
+// A thread's byte offsets from the tile's first row are the same in every tile, so a tile costs one scalar addition to
+// the base and the range-checked loads themselves (vector instructions do not overlap the matrix instructions of a
+// SIMD: the address arithmetic of pointers, five instructions a vector, took a fifth of the forward kernel).
+constexpr int kOutside = 0x7fffffff, kRange = 0x7ffffff0;
 template <class T, int DP, int ROWS>
 struct Stage {
   static constexpr int V = TokNum<T>::V, VPR = DP / V, N = ROWS * VPR / (64 * kWaves);
   static_assert(ROWS * VPR % (64 * kWaves) == 0, "whole vectors per thread");
   u32x4 r[N];
+  int off[N];
   template <class At>
-  __device__ __forceinline__ void load(int D, int rows, At at) {     // at(row) -> pointer to its first element
+  __device__ __forceinline__ void place(int D, At at) {     // at(row) -> its byte offset from the tile's first row
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = threadIdx.x + i * 64 * kWaves, row = id / VPR, d = (id % VPR) * V;
-      r[i] = row < rows && d < D ? *reinterpret_cast<const u32x4*>(at(row) + d) : u32x4{0, 0, 0, 0};
+      off[i] = d < D ? at(row) + d * (int)sizeof(T) : kOutside;
+    }
+  }
+  __device__ __forceinline__ void load(const T* base, int rows) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, kRange, 0x00020000);
+    if (rows >= ROWS) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off[i], 0, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = (threadIdx.x + i * 64 * kWaves) / VPR;
+        r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, row < rows ? off[i] : kOutside, 0, 0));
+      }
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
@@ -195,7 +221,7 @@ __device__ __forceinline__ void store_cols(T* row, const f32x16& a, int j, int h
 // Grid: (row tile, split, problem), the row tiles of a problem on one XCD. SPLIT: every split leaves its unnormalised
 // rows, maximum and sum for the joining kernel.
 template <class T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(256) attn_fwd_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(const AttnParams p) {
   constexpr int KT = tile_len<T, DP>(), LD = Tile<T, DP>::LD;
   __shared__ __attribute__((aligned(16))) T smem[2][2][KT * LD];
   const vg_attention_geom& g = p.g;
@@ -210,12 +236,16 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const AttnParams p) {
 
   RowFrag<T, DP> qf;
   qf.load(row_at<T>(p.q, g.q, p, b, hk, r < rows ? r : 0), g.D, h, r < rows);
+  if (p.cs < 0.f) qf.negate();             // the largest score is then the largest product
+  const float cs = fabsf(p.cs);
   const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
   const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
   Stage<T, DP, KT> sk, sv;
+  sk.place(g.D, [&](int row) { return row * (int)(g.k.st * sizeof(T)); });
+  sv.place(g.D, [&](int row) { return row * (int)(g.v.st * sizeof(T)); });
   auto fetch = [&](int j) {
-    sk.load(g.D, kend - j, [&](int row) { return kb + (int64_t)(j + row) * g.k.st; });
-    sv.load(g.D, kend - j, [&](int row) { return vb + (int64_t)(j + row) * g.v.st; });
+    sk.load(kb + j * g.k.st, kend - j);
+    sv.load(vb + j * g.v.st, kend - j);
   };
   f32x16 o[DP / 32];
 #pragma unroll
@@ -232,33 +262,39 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const AttnParams p) {
     const bool more = j + KT < kend;
     if (more) fetch(j + KT);
     f32x16 s[KT / 32];
-    float top = m;
 #pragma unroll
-    for (int kk = 0; kk < KT / 32; ++kk) {
-      s[kk] = mul_rows<DP>(smem[buf][0], qf, 32 * kk, c, h);
+    for (int kk = 0; kk < KT / 32; ++kk) s[kk] = mul_rows<DP>(smem[buf][0], qf, 32 * kk, c, h);
+    if (j + KT > kend) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kk][i] *= p.cs;
-        if (j + KT > kend && j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) s[kk][i] = -INFINITY;
-        top = fmaxf(top, s[kk][i]);
-      }
+      for (int kk = 0; kk < KT / 32; ++kk)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) s[kk][i] = -INFINITY;
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float alpha = __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    float sum = 0.f;
+    float top = s[0][0];
+#pragma unroll
+    for (int kk = 0; kk < KT / 32; ++kk)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kk][i]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * cs;
+    // the rows' scale changes only when a maximum grows, after the first tiles seldom
+    if (__any(top > m)) {
+      top = fmaxf(top, m);
+      const float alpha = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+    }
 #pragma unroll
     for (int kk = 0; kk < KT / 32; ++kk)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[kk][i] = __builtin_amdgcn_exp2f(s[kk][i] - m);
-        sum += s[kk][i];
+        s[kk][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk][i], cs, -m));
+        l += s[kk][i];
       }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
 #pragma unroll
     for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP>(smem[buf][1], s[kk], 32 * kk, lane, o);
     if (more) {
@@ -347,7 +383,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, flo
 
 // Queries' gradient: the forward kernel's walk with p rebuilt from lse.
 template <class T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(256) attn_gq_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(const AttnParams p) {
   constexpr int KT = tile_len<T, DP>(), LD = Tile<T, DP>::LD;
   __shared__ __attribute__((aligned(16))) T smem[2][2][KT * LD];
   const vg_attention_geom& g = p.g;
@@ -368,9 +404,11 @@ __global__ void __launch_bounds__(256) attn_gq_kernel(const AttnParams p) {
   const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
   const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
   Stage<T, DP, KT> sk, sv;
+  sk.place(g.D, [&](int row) { return row * (int)(g.k.st * sizeof(T)); });
+  sv.place(g.D, [&](int row) { return row * (int)(g.v.st * sizeof(T)); });
   auto fetch = [&](int j) {
-    sk.load(g.D, kend - j, [&](int row) { return kb + (int64_t)(j + row) * g.k.st; });
-    sv.load(g.D, kend - j, [&](int row) { return vb + (int64_t)(j + row) * g.v.st; });
+    sk.load(kb + j * g.k.st, kend - j);
+    sv.load(vb + j * g.v.st, kend - j);
   };
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -441,9 +479,24 @@ __global__ void __launch_bounds__(256, 1) attn_gkv_kernel(const AttnParams p) {
   vf.load((const T*)p.v + b * g.v.sb + hk * g.v.sh + (int64_t)(key < kl ? key : 0) * g.v.st, g.D, h, key < kl);
   Stage<T, DP, RT> sq, sg;
   float st_l = INFINITY, st_d = 0.f;
+  auto place = [&](int j) {        // rows of a tile are whole queries where G divides RT: the same offsets in every tile
+    const int t0 = row_query(p, j);
+    auto at = [&](int row, const vg_heads_layout& l) {
+      const int r = j + row, t = row_query(p, r);
+      return (int)(((t - t0) * l.st + (r - t * p.G) * l.sh) * (int64_t)sizeof(T));
+    };
+    sq.place(g.D, [&](int row) { return at(row, g.q); });
+    sg.place(g.D, [&](int row) { return at(row, g.go); });
+  };
+  place(rbeg);
+  const T* qb = (const T*)p.q + b * g.q.sb + (int64_t)hk * p.G * g.q.sh;
+  const T* gb = (const T*)p.go + b * g.go.sb + (int64_t)hk * p.G * g.go.sh;
+  const bool whole = RT % p.G == 0;
   auto fetch = [&](int j) {
-    sq.load(g.D, rend - j, [&](int row) { return row_at<T>(p.q, g.q, p, b, hk, j + row); });
-    sg.load(g.D, rend - j, [&](int row) { return row_at<T>(p.go, g.go, p, b, hk, j + row); });
+    if (!whole) place(j);
+    const int t0 = row_query(p, j);
+    sq.load(qb + t0 * g.q.st, rend - j);
+    sg.load(gb + t0 * g.go.st, rend - j);
     if (threadIdx.x < RT) {
       const bool ok = j + (int)threadIdx.x < rend;
       st_l = ok ? p.lse_in[(size_t)prob * p.R + j + threadIdx.x] : INFINITY;
@@ -551,7 +604,22 @@ int check_geom(const vg_attention_geom* g) {
   VG_REQUIRE(((R + kTileRows - 1) / kTileRows + 1) * g->B * (long long)g->Hk < (1ll << 31) / 64 &&
                  (((long long)g->Tk + kTileRows - 1) / kTileRows + 1) * g->B * (long long)g->Hk < (1ll << 31) / 64,
              "attention: too many blocks");
-  VG_REQUIRE(isfinite(g->scale), "attention: scale is not finite");
+  VG_REQUIRE(isfinite(g->scale) && g->scale != 0.f, "attention: scale is zero or not finite");
+  return VG_OK;
+}
+
+// byte offsets inside a tile of 64 rows are 31-bit
+template <class T>
+bool strides_ok(const vg_heads_layout& l, int tokens, int heads) {
+  const int64_t most = kRange / 2 / (int64_t)sizeof(T);
+  return (tokens <= 1 || (l.st >= 0 && l.st < most / 66)) && (heads <= 1 || (l.sh >= 0 && l.sh < most / heads));
+}
+template <class T>
+int check_strides(const vg_attention_geom* g, bool backward) {
+  const int G = g->Hq / g->Hk;
+  VG_REQUIRE(strides_ok<T>(g->q, g->Tq, G) && (!backward || strides_ok<T>(g->go, g->Tq, G)) && strides_ok<T>(g->k, g->Tk, 1) &&
+                 strides_ok<T>(g->v, g->Tk, 1),
+             "attention: a stride between tokens or heads is too large");
   return VG_OK;
 }
 
@@ -659,6 +727,8 @@ int attention_fwd(const vg_attention_geom* g, const void* q, const void* k, cons
   VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->Tq, g->Hq) && tok_layout_ok<T>(g->o, o, g->B, g->Tq, g->Hq) &&
                  tok_layout_ok<T>(g->k, k, g->B, g->Tk, g->Hk) && tok_layout_ok<T>(g->v, v, g->B, g->Tk, g->Hk),
              "attention: a head does not start on a 16-byte border");
+  const int sc = check_strides<T>(g, false);
+  if (sc) return sc;
   const size_t need = fwd_bytes(g, pl);
   if (need && (!ws || ws_bytes < need)) return vg_fail(VG_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu are needed", ws_bytes, need);
   VG_REQUIRE(!need || vg_aligned16(ws), "attention: workspace is not 16-byte aligned");
@@ -695,6 +765,8 @@ int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, cons
                  tok_layout_ok<T>(g->k, k, g->B, g->Tk, g->Hk) && tok_layout_ok<T>(g->v, v, g->B, g->Tk, g->Hk) &&
                  tok_layout_ok<T>(g->gk, gk, g->B, g->Tk, g->Hk) && tok_layout_ok<T>(g->gv, gv, g->B, g->Tk, g->Hk),
              "attention backward: a head does not start on a 16-byte border");
+  const int sc = check_strides<T>(g, true);
+  if (sc) return sc;
   const size_t need = bwd_bytes(g, pl);
   if (need && (!ws || ws_bytes < need))
     return vg_fail(VG_ERR_WORKSPACE, "attention backward: workspace of %zu bytes, %zu are needed", ws_bytes, need);

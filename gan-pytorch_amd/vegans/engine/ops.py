@@ -2046,8 +2046,8 @@ def _attention_geom(q, k, v, q_lengths, k_lengths, scale):
                               not n.is_contiguous()):
             raise _hip.HipError("%s must be a contiguous int32 tensor [%d] on the device of the queries" % (what, b))
     scale = d ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise _hip.HipError("scale must be finite, got %s" % scale)
+    if not math.isfinite(scale) or ctypes.c_float(scale).value == 0.0:
+        raise _hip.HipError("scale must be finite and not zero, got %s" % scale)
     return _hip.AttentionGeom(B=b, Tq=tq, Tk=k.shape[1], Hq=hq, Hk=k.shape[2], D=d, scale=scale)
 
 

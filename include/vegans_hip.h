@@ -501,7 +501,7 @@ int vg_qk_norm_rotary_bwd_h(const vg_rotary_geom* g, const void* q, const void* 
  * q_len, are zero, as are the gradients of everything that takes no part. Lengths outside 0..T are clamped. lse [B][Hk]
  * [Tq * Hq / Hk] f32 (log2 of the row sums; nullable in the forward pass) is what the backward pass needs besides o.
  * Backward: gq, and gk with gv, may be null (not wanted).
- * D is a multiple of 8 up to 128. */
+ * D is a multiple of 8 up to 128; scale is finite and not zero. */
 typedef struct vg_attention_geom {
   int32_t B, Tq, Tk, Hq, Hk, D;
   float scale;

@@ -217,6 +217,20 @@ def test_attention_strides_and_orders(gpu, dtype):
                 2 * u * 1.01 * want[n].abs().sum(0, keepdim=True), n)
 
 
+@pytest.mark.parametrize("scale", [-0.3, 1.7])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_attention_scales(gpu, dtype, scale):
+    """A negative scale turns the order of the scores; ragged keys keep out under both."""
+    case = (2, 40, 100, 4, 2, 32, True)
+    q, k, v, ql, kl, go = _attention_case(case, dtype)
+    want = oracle.attention(q.double(), k.double(), v.double(), ql, kl, scale, go.double())
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    o = _ops().attention(*leaves, ql.cuda(), kl.cuda(), scale=scale)
+    got = dict(zip(("o", "gq", "gk", "gv"), (o,) + torch.autograd.grad(o, leaves, go.cuda())))
+    for n in got:
+        _within(got[n], want[n], _attention_allowed(want, dtype, case, n), n)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_attention_extreme_scores(gpu, dtype):
     """Scores far from zero on both sides, rows with one dominant key, equal scores."""
@@ -534,6 +548,7 @@ def test_refusals(gpu):
         lambda: ops.attention(q, k, k, None, torch.zeros(3, dtype=torch.int32, device="cuda")),
         lambda: ops.attention(q, k, k, None, torch.zeros(2, dtype=torch.int32)),
         lambda: ops.attention(q, k, k, scale=math.inf),
+        lambda: ops.attention(q, k, k, scale=0.0),
         lambda: ops.attention(q[0], k[0], k[0]),
         lambda: ops.self_attention(z(2, 4, 5, 16), 2),
         lambda: ops.self_attention(z(2, 4, 4, 16), 2, 0),

@@ -57,11 +57,19 @@ __device__ __forceinline__ int clamped(const int* len, int b, int most) {
 }
 
 // ---- fragments ------------------------------------------------------------------------------------------------------
-// LD: elements of an LDS row. 16 bytes of padding spread the rows of a fragment over the banks.
-template <class T, int DP>
+// An LDS tile of rows of DP elements. A fragment of rows is read 16 bytes a lane, rows 0..15 side by side: padded by 16
+// bytes, they start on different banks. The transposing load (TR tiles, bf16) reads 64 bytes of four rows side by
+// side: its rows are 16 banks apart (mod 64), and to keep the first kind of read apart as well the four 16-byte pieces of
+// every 64 bytes change places by bits 2-3 of the row. (Padded by 16 bytes alone, half the LDS cycles of these
+// kernels were bank conflicts of the transposing loads, ten cycles each instead of four.) f32 columns are read 4 bytes
+// a lane, side by side.
+template <class T, int DP, bool TR>
 struct Tile {
   static constexpr int V = TokNum<T>::V;
-  static constexpr int LD = DP + V;
+  static constexpr bool SWAP = TR && sizeof(T) == 2;
+  static constexpr int LD = SWAP ? (DP == 32 ? 32 : DP + 32) : DP + V;
+  // element index of a 16-byte piece that starts at column d
+  static __device__ __forceinline__ int at(int row, int d) { return row * LD + (SWAP ? d ^ (((row >> 2) & 3) * 8) : d); }
 };
 
 // Registers of a 32-row operand whose contraction index is d: bf16 holds 8 d of each 16 (8 h ..), f32 4 of each 8.
@@ -107,19 +115,19 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // C[row of the LDS tile][column] += sum_d tile[row0 + row][d] * frag(column)[d]
-template <int DP>
+template <int DP, bool TR>
 __device__ __forceinline__ f32x16 mul_rows(const __bf16* tile, const RowFrag<__bf16, DP>& b, int row0, int c, int h) {
   f32x16 acc = zero16();
-  const __bf16* a = tile + (row0 + c) * Tile<__bf16, DP>::LD + 8 * h;
+  const __bf16 *even = tile + Tile<__bf16, DP, TR>::at(row0 + c, 8 * h), *odd = tile + Tile<__bf16, DP, TR>::at(row0 + c, 16 + 8 * h);
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s)
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(a + 16 * s), b.f[s], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>((s % 2 ? odd : even) + s / 2 * 32), b.f[s], acc, 0, 0, 0);
   return acc;
 }
-template <int DP>
+template <int DP, bool TR>
 __device__ __forceinline__ f32x16 mul_rows(const float* tile, const RowFrag<float, DP>& b, int row0, int c, int h) {
   f32x16 acc = zero16();
-  const float* a = tile + (row0 + c) * Tile<float, DP>::LD + 4 * h;
+  const float* a = tile + Tile<float, DP, TR>::at(row0 + c, 4 * h);
 #pragma unroll
   for (int s = 0; s < DP / 8; ++s) {
     const f32x4 x = *reinterpret_cast<const f32x4*>(a + 8 * s);
@@ -128,30 +136,43 @@ __device__ __forceinline__ f32x16 mul_rows(const float* tile, const RowFrag<floa
   }
   return acc;
 }
+// the same with both operands in LDS (rows of a plain tile as columns)
+template <int DP, bool TR>
+__device__ __forceinline__ f32x16 mul_tiles(const __bf16* tile, const __bf16* cols, int row0, int col0, int c, int h) {
+  f32x16 acc = zero16();
+  const __bf16 *even = tile + Tile<__bf16, DP, TR>::at(row0 + c, 8 * h), *odd = tile + Tile<__bf16, DP, TR>::at(row0 + c, 16 + 8 * h);
+  const __bf16* b = cols + Tile<__bf16, DP, false>::at(col0 + c, 8 * h);
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>((s % 2 ? odd : even) + s / 2 * 32),
+                                                  *reinterpret_cast<const bf16x8*>(b + 16 * s), acc, 0, 0, 0);
+  return acc;
+}
 
-// acc[j] (rows d = 32 j + row) += sum over the 32 tile rows k0.. of tile[k][d] * w[k][column], w as a product left it
+// acc[j] (rows d = 32 j + row) += sum over the 32 rows k0.. of a TR tile of tile[k][d] * w[k][column], w as a product left it
 template <int DP>
 __device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
-  constexpr int LD = Tile<__bf16, DP>::LD;
+  using L = Tile<__bf16, DP, true>;
   const int h = lane >> 5, q = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  // rows k0 + 16 s + 4 h + q and 8 further: bits 2-3 of the row are h and 2 + h
+  const __bf16 *a = tile + (k0 + 4 * h + q) * L::LD + (col ^ (8 * h)), *b = tile + (k0 + 8 + 4 * h + q) * L::LD + (col ^ (8 * (2 + h)));
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const u32x4 pk = {tok_pack2(w[8 * s], w[8 * s + 1]), tok_pack2(w[8 * s + 2], w[8 * s + 3]), tok_pack2(w[8 * s + 4], w[8 * s + 5]),
                       tok_pack2(w[8 * s + 6], w[8 * s + 7])};
-    const bf16x8 b = __builtin_bit_cast(bf16x8, pk);
-    const __bf16* a = tile + (k0 + 16 * s + 4 * h + q) * LD + col;
+    const bf16x8 x = __builtin_bit_cast(bf16x8, pk);
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) {
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 32 * j));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 32 * j + 8 * LD));
-      const s16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), b, acc[j], 0, 0, 0);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 16 * s * L::LD + 32 * j));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b + 16 * s * L::LD + 32 * j));
+      const s16x8 y = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, y), x, acc[j], 0, 0, 0);
     }
   }
 }
 template <int DP>
 __device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
-  constexpr int LD = Tile<float, DP>::LD;
+  constexpr int LD = Tile<float, DP, true>::LD;
   const int h = lane >> 5, c = lane & 31;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -166,7 +187,7 @@ __device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int
 // the base and the range-checked loads themselves (vector instructions do not overlap the matrix instructions of a
 // SIMD: the address arithmetic of pointers, five instructions a vector, took a fifth of the forward kernel).
 constexpr int kOutside = 0x7fffffff, kRange = 0x7ffffff0;
-template <class T, int DP, int ROWS>
+template <class T, int DP, int ROWS, bool TR>
 struct Stage {
   static constexpr int V = TokNum<T>::V, VPR = DP / V, N = ROWS * VPR / (64 * kWaves);
   static_assert(ROWS * VPR % (64 * kWaves) == 0, "whole vectors per thread");
@@ -197,7 +218,7 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = threadIdx.x + i * 64 * kWaves, row = id / VPR, d = (id % VPR) * V;
-      *reinterpret_cast<u32x4*>(tile + row * Tile<T, DP>::LD + d) = r[i];
+      *reinterpret_cast<u32x4*>(tile + Tile<T, DP, TR>::at(row, d)) = r[i];
     }
   }
 };
@@ -222,8 +243,9 @@ __device__ __forceinline__ void store_cols(T* row, const f32x16& a, int j, int h
 // rows, maximum and sum for the joining kernel.
 template <class T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(const AttnParams p) {
-  constexpr int KT = tile_len<T, DP>(), LD = Tile<T, DP>::LD;
-  __shared__ __attribute__((aligned(16))) T smem[2][2][KT * LD];
+  constexpr int KT = tile_len<T, DP>();
+  __shared__ __attribute__((aligned(16))) T ktile[2][KT * Tile<T, DP, false>::LD];
+  __shared__ __attribute__((aligned(16))) T vtile[2][KT * Tile<T, DP, true>::LD];
   const vg_attention_geom& g = p.g;
   const int id = tok_xcd_order(blockIdx.x, gridDim.x);
   const int rt = id % p.row_tiles, sp = (id / p.row_tiles) % p.splits, prob = id / (p.row_tiles * p.splits);
@@ -240,7 +262,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
   const float cs = fabsf(p.cs);
   const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
   const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
-  Stage<T, DP, KT> sk, sv;
+  Stage<T, DP, KT, false> sk;
+  Stage<T, DP, KT, true> sv;
   sk.place(g.D, [&](int row) { return row * (int)(g.k.st * sizeof(T)); });
   sv.place(g.D, [&](int row) { return row * (int)(g.v.st * sizeof(T)); });
   auto fetch = [&](int j) {
@@ -254,8 +277,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
   int buf = 0;
   if (kbeg < kend) {
     fetch(kbeg);
-    sk.store(smem[0][0]);
-    sv.store(smem[0][1]);
+    sk.store(ktile[0]);
+    sv.store(vtile[0]);
   }
   __syncthreads();
   for (int j = kbeg; j < kend; j += KT) {
@@ -263,7 +286,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
     if (more) fetch(j + KT);
     f32x16 s[KT / 32];
 #pragma unroll
-    for (int kk = 0; kk < KT / 32; ++kk) s[kk] = mul_rows<DP>(smem[buf][0], qf, 32 * kk, c, h);
+    for (int kk = 0; kk < KT / 32; ++kk) s[kk] = mul_rows<DP, false>(ktile[buf], qf, 32 * kk, c, h);
     if (j + KT > kend) {
 #pragma unroll
       for (int kk = 0; kk < KT / 32; ++kk)
@@ -296,10 +319,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
         l += s[kk][i];
       }
 #pragma unroll
-    for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP>(smem[buf][1], s[kk], 32 * kk, lane, o);
+    for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP>(vtile[buf], s[kk], 32 * kk, lane, o);
     if (more) {
-      sk.store(smem[buf ^ 1][0]);
-      sv.store(smem[buf ^ 1][1]);
+      sk.store(ktile[buf ^ 1]);
+      sv.store(vtile[buf ^ 1]);
     }
     __syncthreads();
     buf ^= 1;
@@ -384,8 +407,9 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, flo
 // Queries' gradient: the forward kernel's walk with p rebuilt from lse.
 template <class T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(const AttnParams p) {
-  constexpr int KT = tile_len<T, DP>(), LD = Tile<T, DP>::LD;
-  __shared__ __attribute__((aligned(16))) T smem[2][2][KT * LD];
+  constexpr int KT = tile_len<T, DP>();
+  __shared__ __attribute__((aligned(16))) T ktile[2][KT * Tile<T, DP, true>::LD];
+  __shared__ __attribute__((aligned(16))) T vtile[2][KT * Tile<T, DP, false>::LD];
   const vg_attention_geom& g = p.g;
   const int id = tok_xcd_order(blockIdx.x, gridDim.x);
   const int rt = id % p.row_tiles, sp = (id / p.row_tiles) % p.splits, prob = id / (p.row_tiles * p.splits);
@@ -403,7 +427,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
   const float delta = r < rows ? p.delta[(size_t)prob * p.R + r] : 0.f;
   const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
   const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
-  Stage<T, DP, KT> sk, sv;
+  Stage<T, DP, KT, true> sk;
+  Stage<T, DP, KT, false> sv;
   sk.place(g.D, [&](int row) { return row * (int)(g.k.st * sizeof(T)); });
   sv.place(g.D, [&](int row) { return row * (int)(g.v.st * sizeof(T)); });
   auto fetch = [&](int j) {
@@ -416,8 +441,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
   int buf = 0;
   if (kbeg < kend) {
     fetch(kbeg);
-    sk.store(smem[0][0]);
-    sv.store(smem[0][1]);
+    sk.store(ktile[0]);
+    sv.store(vtile[0]);
   }
   __syncthreads();
   for (int j = kbeg; j < kend; j += KT) {
@@ -425,19 +450,19 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
     if (more) fetch(j + KT);
 #pragma unroll
     for (int kk = 0; kk < KT / 32; ++kk) {
-      const f32x16 s = mul_rows<DP>(smem[buf][0], qf, 32 * kk, c, h);
-      f32x16 dp = mul_rows<DP>(smem[buf][1], gf, 32 * kk, c, h);
+      const f32x16 s = mul_rows<DP, true>(ktile[buf], qf, 32 * kk, c, h);
+      f32x16 dp = mul_rows<DP, false>(vtile[buf], gf, 32 * kk, c, h);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.cs, -lse));
         if (j + KT > kend && j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) w = 0.f;
         dp[i] = w * (dp[i] - delta);
       }
-      mul_cols<DP>(smem[buf][0], dp, 32 * kk, lane, acc);
+      mul_cols<DP>(ktile[buf], dp, 32 * kk, lane, acc);
     }
     if (more) {
-      sk.store(smem[buf ^ 1][0]);
-      sv.store(smem[buf ^ 1][1]);
+      sk.store(ktile[buf ^ 1]);
+      sv.store(vtile[buf ^ 1]);
     }
     __syncthreads();
     buf ^= 1;
@@ -454,15 +479,20 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
   }
 }
 
-// Gradients of keys and values: a block owns kTileRows keys (32 a wave, in registers) and walks the problem's rows.
+// Gradients of keys and values: a block owns kTileRows keys (32 a wave, in registers) and walks the problem's rows. bf16
+// heads of 128: the values of the block's keys stay in LDS instead and the rows come 32 at a time, which brings the kernel
+// under 256 registers, i.e. to two waves a SIMD (video case 3138 us with all in registers, 2350 so).
 template <class T, int DP>
 constexpr int row_len() {
-  return sizeof(T) == 2 ? 64 : 32;
+  return sizeof(T) == 2 && DP < 128 ? 64 : 32;
 }
 template <class T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(256, 1) attn_gkv_kernel(const AttnParams p) {
-  constexpr int RT = row_len<T, DP>(), LD = Tile<T, DP>::LD;
-  __shared__ __attribute__((aligned(16))) T smem[2][2][RT * LD];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(const AttnParams p) {
+  constexpr int RT = row_len<T, DP>();
+  constexpr bool kValuesInLds = sizeof(T) == 2 && DP == 128;
+  using Plain = Tile<T, DP, false>;
+  __shared__ __attribute__((aligned(16))) T smem[2][2][RT * Tile<T, DP, true>::LD];
+  __shared__ __attribute__((aligned(16))) T vtile[kValuesInLds ? kTileRows * Plain::LD : 1];
   __shared__ __attribute__((aligned(16))) float stat[2][2][RT];
   const vg_attention_geom& g = p.g;
   const int id = tok_xcd_order(blockIdx.x, gridDim.x);
@@ -476,8 +506,17 @@ __global__ void __launch_bounds__(256, 1) attn_gkv_kernel(const AttnParams p) {
 
   RowFrag<T, DP> kf, vf;
   kf.load((const T*)p.k + b * g.k.sb + hk * g.k.sh + (int64_t)(key < kl ? key : 0) * g.k.st, g.D, h, key < kl);
-  vf.load((const T*)p.v + b * g.v.sb + hk * g.v.sh + (int64_t)(key < kl ? key : 0) * g.v.st, g.D, h, key < kl);
-  Stage<T, DP, RT> sq, sg;
+  if constexpr (kValuesInLds) {
+    constexpr int V = TokNum<T>::V;
+    for (int id = threadIdx.x; id < kTileRows * DP / V; id += 64 * kWaves) {
+      const int row = id / (DP / V), d = id % (DP / V) * V, j = kt * kTileRows + row;
+      const T* src = (const T*)p.v + b * g.v.sb + hk * g.v.sh + (int64_t)j * g.v.st + d;
+      *reinterpret_cast<u32x4*>(vtile + Plain::at(row, d)) = j < kl && d < g.D ? *reinterpret_cast<const u32x4*>(src) : u32x4{0, 0, 0, 0};
+    }
+  } else {
+    vf.load((const T*)p.v + b * g.v.sb + hk * g.v.sh + (int64_t)(key < kl ? key : 0) * g.v.st, g.D, h, key < kl);
+  }
+  Stage<T, DP, RT, true> sq, sg;
   float st_l = INFINITY, st_d = 0.f;
   auto place = [&](int j) {        // rows of a tile are whole queries where G divides RT: the same offsets in every tile
     const int t0 = row_query(p, j);
@@ -525,8 +564,11 @@ __global__ void __launch_bounds__(256, 1) attn_gkv_kernel(const AttnParams p) {
     if (more) fetch(j + RT);
 #pragma unroll
     for (int rr = 0; rr < RT / 32; ++rr) {
-      f32x16 w = mul_rows<DP>(smem[buf][0], kf, 32 * rr, c, h);
-      f32x16 dp = mul_rows<DP>(smem[buf][1], vf, 32 * rr, c, h);
+      f32x16 w = mul_rows<DP, true>(smem[buf][0], kf, 32 * rr, c, h), dp;
+      if constexpr (kValuesInLds)
+        dp = mul_tiles<DP, true>(smem[buf][1], vtile, 32 * rr, 32 * wid, c, h);
+      else
+        dp = mul_rows<DP, true>(smem[buf][1], vf, 32 * rr, c, h);
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[buf][0][32 * rr + 8 * i4 + 4 * h]);
@@ -539,6 +581,7 @@ __global__ void __launch_bounds__(256, 1) attn_gkv_kernel(const AttnParams p) {
         }
       }
       mul_cols<DP>(smem[buf][1], w, 32 * rr, lane, gv);
+      __builtin_amdgcn_sched_barrier(0);     // (reads hoisted across this line spill)
       mul_cols<DP>(smem[buf][0], dp, 32 * rr, lane, gk);
     }
     if (more) put(buf ^ 1);

@@ -114,10 +114,9 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
-// C[row of the LDS tile][column] += sum_d tile[row0 + row][d] * frag(column)[d]
+// C[row of the LDS tile][column] = acc + sum_d tile[row0 + row][d] * frag(column)[d]
 template <int DP, bool TR>
-__device__ __forceinline__ f32x16 mul_rows(const __bf16* tile, const RowFrag<__bf16, DP>& b, int row0, int c, int h) {
-  f32x16 acc = zero16();
+__device__ __forceinline__ f32x16 mul_rows(const __bf16* tile, const RowFrag<__bf16, DP>& b, int row0, int c, int h, f32x16 acc = zero16()) {
   const __bf16 *even = tile + Tile<__bf16, DP, TR>::at(row0 + c, 8 * h), *odd = tile + Tile<__bf16, DP, TR>::at(row0 + c, 16 + 8 * h);
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s)
@@ -125,8 +124,7 @@ __device__ __forceinline__ f32x16 mul_rows(const __bf16* tile, const RowFrag<__b
   return acc;
 }
 template <int DP, bool TR>
-__device__ __forceinline__ f32x16 mul_rows(const float* tile, const RowFrag<float, DP>& b, int row0, int c, int h) {
-  f32x16 acc = zero16();
+__device__ __forceinline__ f32x16 mul_rows(const float* tile, const RowFrag<float, DP>& b, int row0, int c, int h, f32x16 acc = zero16()) {
   const float* a = tile + Tile<float, DP, TR>::at(row0 + c, 4 * h);
 #pragma unroll
   for (int s = 0; s < DP / 8; ++s) {
@@ -138,8 +136,7 @@ __device__ __forceinline__ f32x16 mul_rows(const float* tile, const RowFrag<floa
 }
 // the same with both operands in LDS (rows of a plain tile as columns)
 template <int DP, bool TR>
-__device__ __forceinline__ f32x16 mul_tiles(const __bf16* tile, const __bf16* cols, int row0, int col0, int c, int h) {
-  f32x16 acc = zero16();
+__device__ __forceinline__ f32x16 mul_tiles(const __bf16* tile, const __bf16* cols, int row0, int col0, int c, int h, f32x16 acc) {
   const __bf16 *even = tile + Tile<__bf16, DP, TR>::at(row0 + c, 8 * h), *odd = tile + Tile<__bf16, DP, TR>::at(row0 + c, 16 + 8 * h);
   const __bf16* b = cols + Tile<__bf16, DP, false>::at(col0 + c, 8 * h);
 #pragma unroll
@@ -300,8 +297,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kk][i]);
     top = fmaxf(top, __shfl_xor(top, 32, 64)) * cs;
-    // the rows' scale changes only when a maximum grows, after the first tiles seldom
-    if (__any(top > m)) {
+    // the rows' scale follows a maximum that grows by more than 2^8 only: that seldom happens after the first tile, and up to
+    // 2^8 the f32 sums and the relative roundings of the probabilities lose nothing
+    if (__any(top > m + 8.f)) {
       top = fmaxf(top, m);
       const float alpha = __builtin_amdgcn_exp2f(m - top);
       m = top;
@@ -404,10 +402,11 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, flo
   if (threadIdx.x % 8 == 0 && row < (long long)g.B * g.Hk * p.R) delta[row] = sum;
 }
 
-// Queries' gradient: the forward kernel's walk with p rebuilt from lse.
+// Queries' gradient: the forward kernel's walk with p rebuilt from lse. Heads of 128 take their keys 32 at a time (fewer
+// staging registers: at 64 the kernel spills, video case 1993 us).
 template <class T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(const AttnParams p) {
-  constexpr int KT = tile_len<T, DP>();
+  constexpr int KT = DP >= 128 ? 32 : tile_len<T, DP>();
   __shared__ __attribute__((aligned(16))) T ktile[2][KT * Tile<T, DP, true>::LD];
   __shared__ __attribute__((aligned(16))) T vtile[2][KT * Tile<T, DP, false>::LD];
   const vg_attention_geom& g = p.g;
@@ -424,7 +423,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
   qf.load(row_at<T>(p.q, g.q, p, b, hk, r < rows ? r : 0), g.D, h, r < rows);
   gf.load(row_at<T>(p.go, g.go, p, b, hk, r < rows ? r : 0), g.D, h, r < rows);
   const float lse = r < rows ? p.lse_in[(size_t)prob * p.R + r] : INFINITY;
-  const float delta = r < rows ? p.delta[(size_t)prob * p.R + r] : 0.f;
+  f32x16 less;               // -delta: what the product go v^T starts from
+  {
+    const float delta = r < rows ? p.delta[(size_t)prob * p.R + r] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) less[i] = -delta;
+  }
   const T* kb = (const T*)p.k + b * g.k.sb + hk * g.k.sh;
   const T* vb = (const T*)p.v + b * g.v.sb + hk * g.v.sh;
   Stage<T, DP, KT, true> sk;
@@ -450,14 +454,17 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
     if (more) fetch(j + KT);
 #pragma unroll
     for (int kk = 0; kk < KT / 32; ++kk) {
-      const f32x16 s = mul_rows<DP, true>(ktile[buf], qf, 32 * kk, c, h);
-      f32x16 dp = mul_rows<DP, false>(vtile[buf], gf, 32 * kk, c, h);
+      f32x16 s = mul_rows<DP, true>(ktile[buf], qf, 32 * kk, c, h);
+      f32x16 dp = mul_rows<DP, false>(vtile[buf], gf, 32 * kk, c, h, less);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.cs, -lse));
-        if (j + KT > kend && j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) w = 0.f;
-        dp[i] = w * (dp[i] - delta);
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.cs, -lse));
+      if (j + KT > kend) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (j + 32 * kk + 8 * (i / 4) + 4 * h + i % 4 >= kend) s[i] = 0.f;
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] *= s[i];
       mul_cols<DP>(ktile[buf], dp, 32 * kk, lane, acc);
     }
     if (more) {
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(c
     sg.store(smem[buf][1]);
     if (threadIdx.x < RT) {
       stat[buf][0][threadIdx.x] = st_l;
-      stat[buf][1][threadIdx.x] = st_d;
+      stat[buf][1][threadIdx.x] = -st_d;
     }
   };
   f32x16 gk[DP / 32], gv[DP / 32];
@@ -565,21 +572,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(c
 #pragma unroll
     for (int rr = 0; rr < RT / 32; ++rr) {
       f32x16 w = mul_rows<DP, true>(smem[buf][0], kf, 32 * rr, c, h), dp;
-      if constexpr (kValuesInLds)
-        dp = mul_tiles<DP, true>(smem[buf][1], vtile, 32 * rr, 32 * wid, c, h);
-      else
-        dp = mul_rows<DP, true>(smem[buf][1], vf, 32 * rr, c, h);
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
+      for (int i4 = 0; i4 < 4; ++i4) {      // go v^T starts from -delta
         const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[buf][0][32 * rr + 8 * i4 + 4 * h]);
-        const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][1][32 * rr + 8 * i4 + 4 * h]);
+        const f32x4 less = *reinterpret_cast<const f32x4*>(&stat[buf][1][32 * rr + 8 * i4 + 4 * h]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = 4 * i4 + e;
-          w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[i], p.cs, -lse[e]));
-          dp[i] = w[i] * (dp[i] - delta[e]);
+          w[4 * i4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[4 * i4 + e], p.cs, -lse[e]));
+          dp[4 * i4 + e] = less[e];
         }
       }
+      if constexpr (kValuesInLds)
+        dp = mul_tiles<DP, true>(smem[buf][1], vtile, 32 * rr, 32 * wid, c, h, dp);
+      else
+        dp = mul_rows<DP, true>(smem[buf][1], vf, 32 * rr, c, h, dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] *= w[i];
       mul_cols<DP>(smem[buf][1], w, 32 * rr, lane, gv);
       __builtin_amdgcn_sched_barrier(0);     // (reads hoisted across this line spill)
       mul_cols<DP>(smem[buf][0], dp, 32 * rr, lane, gk);

@@ -3,9 +3,10 @@
 //
 //   gg = gh u act'(g)     gu = gh act(g)     gx = [gg gu] [Wg; Wu]     gW = [gg gu]^T x     gb = column sums of [gg gu]
 //
-// The weights lie as one [2F][C] matrix (gate rows first). A block's weight tile takes 32 gate rows, the matching 32
-// value rows, the next 32 gate rows, ...: gate and value of one output element end in the same lane's accumulators and
-// the epilogue is private to the lane. Bound by the matrix cores (4 M C F flops forward, twice that backward).
+// The weights lie as one [2F][C] matrix (gate rows first). They are the rows of the product and x its columns; a block's
+// weight tile takes 32 gate rows, the matching 32 value rows, the next 32 gate rows, ...: gate and value of one output
+// element end in the same lane's accumulators, sixteen neighbouring elements of one row of h a lane, so the epilogue is
+// private to the lane and moves 16 bytes at a time. Bound by the matrix cores (4 M C F flops forward, twice that backward).
 //
 // What the backward pass needs of g and u is either written by the forward pass in f32 (z) or, with bf16 operands and
 // few input features, computed again: a product of C terms per element against 8 bytes written and read. z is never
@@ -25,21 +26,39 @@ struct GatedParams {
   int M, C, F, act, row_tiles, col_tiles;
 };
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
-
-__device__ __forceinline__ float gate(float g, int act) {
-  switch (act) {
-    case VG_GATE_SIGMOID: return sigmoid(g);
-    case VG_GATE_RELU: return g > 0.f ? g : (g != g ? g : 0.f);
-    case VG_GATE_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-    default: return g * sigmoid(g);
+// The gates. f32 takes the library's exponential and error function. bf16 results keep 8 bits: the hardware's exponential
+// and reciprocal (one unit in the last place of f32) and, for the normal distribution's tail, formula 7.1.26 of
+// Abramowitz and Stegun, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by at most 1.5e-7 - the library's
+// error function took longer than the products of a tile.
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float g) {
+  if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+  return 1.f / (1.f + expf(-g));
+}
+// distribution and density of the standard normal
+template <bool FAST>
+__device__ __forceinline__ void normal(float g, float& cdf, float& pdf) {
+  if constexpr (FAST) {
+    const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);      // exp(-g^2 / 2)
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(g), 1.f));
+    float q = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+    q = __builtin_fmaf(t, q, 1.421413741f);
+    q = __builtin_fmaf(t, q, -0.284496736f);
+    q = __builtin_fmaf(t, q, 0.254829592f);
+    const float tail = 0.5f * t * q * e;
+    cdf = g < 0.f ? tail : 1.f - tail;
+    pdf = 0.3989422804014327f * e;
+  } else {
+    cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    pdf = 0.3989422804014327f * expf(-0.5f * g * g);
   }
 }
-// act(g) and act'(g)
+// act(g) and act'(g) (the caller's compiler drops what it does not use)
+template <bool FAST>
 __device__ __forceinline__ void gate_both(float g, int act, float& a, float& d) {
   switch (act) {
     case VG_GATE_SIGMOID: {
-      a = sigmoid(g);
+      a = sigmoid<FAST>(g);
       d = a * (1.f - a);
       break;
     }
@@ -49,13 +68,14 @@ __device__ __forceinline__ void gate_both(float g, int act, float& a, float& d) 
       break;
     }
     case VG_GATE_GELU: {
-      const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-      a = g * cdf;
-      d = __builtin_fmaf(g * 0.3989422804014327f, expf(-0.5f * g * g), cdf);
+      float pdf;
+      normal<FAST>(g, d, pdf);
+      a = g * d;
+      d = __builtin_fmaf(g, pdf, d);
       break;
     }
     default: {
-      const float s = sigmoid(g);
+      const float s = sigmoid<FAST>(g);
       a = g * s;
       d = __builtin_fmaf(a, 1.f - s, s);
     }
@@ -65,73 +85,218 @@ __device__ __forceinline__ void gate_both(float g, int act, float& a, float& d) 
 template <class T>
 __device__ __forceinline__ float load1(const T* p) { return (float)*p; }
 
-// BWD: the epilogue turns gh into [gg gu] instead of writing h
-template <class T, int BM, int BN, int WM, int WN, bool ALIGNED, bool BWD>
-__global__ void __launch_bounds__(64 * WM * WN, 1) gated_kernel(const GatedParams p) {
-  using G = TokGemm<T, false, false, BM, BN, WM, WN, ALIGNED>;
+// Sixteen neighbouring elements, n of them inside the row; any alignment of an element.
+template <class T>
+__device__ __forceinline__ void load16(const T* p, int n, float (&v)[16]) {
+  constexpr int V = TokNum<T>::V;
+  if (n >= 16) {
+#pragma unroll
+    for (int i = 0; i < 16 / V; ++i) {
+      u32x4 raw;
+      __builtin_memcpy(&raw, p + i * V, 16);
+      float f[V];
+      tok_widen(raw, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i * V + e] = f[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store16(T* p, int n, const float (&v)[16]) {
+  constexpr int V = TokNum<T>::V;
+  if (n >= 16) {
+#pragma unroll
+    for (int i = 0; i < 16 / V; ++i) {
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = v[i * V + e];
+      const u32x4 raw = tok_narrow(f);
+      __builtin_memcpy(p + i * V, &raw, 16);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (e < n) p[e] = (T)v[e];
+  }
+}
+
+// Tile order: runs of kGroup row tiles walk the column tiles together, so that the tiles in flight on an XCD share rows of
+// x and of the weights in its L2 (32 tiles at once: 8 + 4 operand tiles instead of 1 + 32).
+constexpr int kGroup = 8;
+__device__ __forceinline__ void tile_of(int id, int row_tiles, int col_tiles, int& mt, int& nt) {
+  const int run = kGroup * col_tiles, first = id / run * kGroup, rest = id % run, wide = min(kGroup, row_tiles - first);
+  mt = first + rest % wide;
+  nt = rest / wide;
+}
+
+// BWD: the epilogue turns gh into [gg gu] instead of writing h. WM waves along the weights' rows, WN along the rows of x.
+template <class T, int BF, int BM, int WM, int WN, bool BWD>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gated_kernel(const GatedParams p) {
+  using G = TokGemm<T, false, false, BF, BM, WM, WN>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
-  T* smem = reinterpret_cast<T*>(smem_raw);
-  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
-  const int mt = id / p.col_tiles, nt = id - mt * p.col_tiles;
-  const int m0 = mt * BM, n0 = nt * BN;
+  int mt, nt;
+  tile_of(tok_xcd_order(blockIdx.x, gridDim.x), p.row_tiles, p.col_tiles, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BF;
   f32x16 acc[G::TM][G::TN];
-  const TokOperand<T> A = {(const T*)p.x, p.C, p.M, 0}, B = {(const T*)p.w, p.C, 2 * p.F, p.F};
-  G::run(A, B, m0, n0, 0, p.C, smem, acc);
+  const TokOperand<T> A = {(const T*)p.w, p.C, 2 * p.F, p.F}, B = {(const T*)p.x, p.C, p.M, 0};
+  G::run(A, B, n0, m0, 0, p.C, reinterpret_cast<T*>(smem_raw), acc);
 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
   const int wm = wid / WN, wn = wid % WN;
-  float sums[G::TN];
+  constexpr int LDR = 68;                                       // a lane column of partial sums, padded
+  float* red = reinterpret_cast<float*>(smem_raw);              // [wave][32][LDR], then [WN][BF] sums behind it
+  float* total = red + WM * WN * 32 * LDR;
+  static_assert((WM * WN * 32 * LDR + WN * BF) * 4 <= G::LDS_BYTES, "the sums fit the tiles' space");
 #pragma unroll
-  for (int j = 0; j < G::TN; j += 2) {
-    const int f = n0 / 2 + wn * G::TN * 16 + j * 16 + c;
-    const bool in = f < p.F;
-    const float bg = in && p.bias ? p.bias[f] : 0.f, bu = in && p.bias ? p.bias[p.F + f] : 0.f;
-    float sg = 0.f, su = 0.f;
+  for (int i = 0; i < G::TM; i += 2) {
+    const int f = n0 / 2 + (wm * G::TM + i) * 16 + 16 * h, left = p.F - f;
+    float bg[16], bu[16], sg[16], su[16];
 #pragma unroll
-    for (int i = 0; i < G::TM; ++i) {
+    for (int e = 0; e < 16; ++e) sg[e] = su[e] = bg[e] = bu[e] = 0.f;
+    if (p.bias) {
+      load16(p.bias + f, left, bg);
+      load16(p.bias + p.F + f, left, bu);
+    }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int m = m0 + (wm * G::TM + i) * 32 + 8 * (e / 4) + 4 * h + e % 4;
-        if (!in || m >= p.M) continue;
-        const float g = acc[i][j][e] + bg, u = acc[i][j + 1][e] + bu;
-        if constexpr (!BWD) {
-          ((T*)p.h)[(size_t)m * p.F + f] = (T)(gate(g, p.act) * u);
-          if (p.z) {
-            p.z[(size_t)m * 2 * p.F + f] = g;
-            p.z[(size_t)m * 2 * p.F + p.F + f] = u;
-          }
-        } else {
+    for (int j = 0; j < G::TN; ++j) {
+      const int m = m0 + (wn * G::TN + j) * 32 + c;
+      if (m < p.M && left > 0) {
+        float g[16], u[16], gg[16], gu[16];
+        [[maybe_unused]] float x[16];
+        const size_t at = (size_t)m * p.F + f, at2 = (size_t)m * 2 * p.F + f;
+        if constexpr (BWD) load16((const T*)p.gh + at, left, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          g[e] = acc[i][j][e] + bg[e];
+          u[e] = acc[i + 1][j][e] + bu[e];
           float a, d;
-          gate_both(g, p.act, a, d);
-          const float gh = load1((const T*)p.gh + (size_t)m * p.F + f);
-          const float gg = gh * u * d, gu = gh * a;
-          sg += gg;
-          su += gu;
-          ((T*)p.gz)[(size_t)m * 2 * p.F + f] = (T)gg;
-          ((T*)p.gz)[(size_t)m * 2 * p.F + p.F + f] = (T)gu;
+          gate_both<sizeof(T) == 2>(g[e], p.act, a, d);
+          if constexpr (BWD) {
+            gg[e] = x[e] * u[e] * d;
+            gu[e] = x[e] * a;
+            sg[e] += gg[e];
+            su[e] += gu[e];
+          } else {
+            gg[e] = a * u[e];
+          }
+        }
+        if constexpr (BWD) {
+          store16((T*)p.gz + at2, left, gg);
+          store16((T*)p.gz + at2 + p.F, left, gu);
+        } else {
+          store16((T*)p.h + at, left, gg);
+          if (p.z) {
+            store16(p.z + at2, left, g);
+            store16(p.z + at2 + p.F, left, u);
+          }
         }
       }
     }
-    sums[j] = sg;
-    sums[j + 1] = su;
+    if constexpr (BWD) {
+      if (p.gb_part) {       // column sums: the wave's 32 rows of x in a fixed order (its own space: no barrier needed)
+        float* mine = red + wid * 32 * LDR;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          *reinterpret_cast<f32x4*>(mine + c * LDR + 32 * h + e) = f32x4{sg[e], sg[e + 1], sg[e + 2], sg[e + 3]};
+          *reinterpret_cast<f32x4*>(mine + c * LDR + 32 * h + 16 + e) = f32x4{su[e], su[e + 1], su[e + 2], su[e + 3]};
+        }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float v = 0.f;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) v += mine[r * LDR + lane];
+        total[wn * BF + (wm * G::TM + i) * 32 + lane] = v;      // lane = 32 h + 16 (value) + element
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
   }
   if constexpr (BWD) {
     if (!p.gb_part) return;
-    // column sums of the block's rows: lane halves, then the row waves, in a fixed order
-    float* red = reinterpret_cast<float*>(smem_raw);
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < G::TN; ++j) {
-      const float v = sums[j] + __shfl_xor(sums[j], 32, 64);
-      if (h == 0) red[wm * BN + (wn * G::TN + j) * 32 + c] = v;
-    }
-    __syncthreads();
-    for (int n = threadIdx.x; n < BN; n += G::NT) {
+    for (int n = threadIdx.x; n < BF; n += G::NT) {             // n = 64 block + 32 h + 16 (value) + element
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < WM; ++w) v += red[w * BN + n];
-      const int f = n0 / 2 + (n >> 6) * 32 + (n & 31);
-      if (f < p.F) p.gb_part[(size_t)mt * 2 * p.F + ((n >> 5) & 1) * p.F + f] = v;
+      for (int w = 0; w < WN; ++w) v += total[w * BF + n];
+      const int f = n0 / 2 + (n >> 6) * 32 + ((n >> 5) & 1) * 16 + (n & 15);
+      if (f < p.F) p.gb_part[(size_t)mt * 2 * p.F + ((n >> 4) & 1) * p.F + f] = v;
+    }
+  }
+}
+
+// Few rows of x (up to 64): all there is to read is the weights, once. A block takes 16 output columns, i.e. 16 gate and 16
+// value rows as the 32 rows of a product tile whose columns are the rows of x, and its waves split the features. Weights
+// and x go from memory into the operand registers: a lane reads 128 bytes of one row (the order of k inside a product does
+// not matter, so its half of a block of k is contiguous), eight 16-byte loads in flight. The partial products of the waves
+// meet in LDS. Tiles of rows 0..15 and 16..31 put gate and value of an element in one lane: registers i and i + 8.
+constexpr int kFewRows = 64, kFewWaves = 8;
+template <class T, int NB>
+__global__ void __launch_bounds__(64 * kFewWaves) gated_few_kernel(const GatedParams p) {
+  constexpr int V = TokNum<T>::V, HALF = 8 * V, KB = 2 * HALF;     // features a lane half, a wave takes at once
+  using Frag = std::conditional_t<sizeof(T) == 2, bf16x8, f32x4>;
+  __shared__ float red[kFewWaves][NB][16][64];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+  const int f0 = blockIdx.x * 16;
+  const int fr = min(f0 + (c & 15), p.F - 1);                      // clamped: what it gives is not stored
+  const T* w = (const T*)p.w + (size_t)(fr + (c >> 4) * p.F) * p.C + h * HALF;
+  const T* x[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) x[n] = (const T*)p.x + (size_t)min(n * 32 + c, p.M - 1) * p.C + h * HALF;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+  using S = TokStage<T, false, 128, sizeof(T) == 2 ? 64 : 32, 256>;      // (its loads)
+  for (int k = wid * KB; k < p.C; k += kFewWaves * KB) {
+    u32x4 a[8], b[NB][8];
+    if (k + KB <= p.C) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = S::whole(reinterpret_cast<const char*>(w + k + i * V));
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[n][i] = S::whole(reinterpret_cast<const char*>(x[n] + k + i * V));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int left = p.C - k - h * HALF - i * V;
+        a[i] = left >= V ? S::whole(reinterpret_cast<const char*>(w + k + i * V)) : S::part(reinterpret_cast<const char*>(w + k + i * V), left);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          b[n][i] = left >= V ? S::whole(reinterpret_cast<const char*>(x[n] + k + i * V))
+                              : S::part(reinterpret_cast<const char*>(x[n] + k + i * V), left);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[n] = tok_mma(__builtin_bit_cast(Frag, a[i]), __builtin_bit_cast(Frag, b[n][i]), acc[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) red[wid][n][e][lane] = acc[n][e];
+  __syncthreads();
+  for (int id = threadIdx.x; id < NB * 8 * 64; id += 64 * kFewWaves) {
+    const int l = id & 63, i = (id >> 6) & 7, n = id >> 9;
+    const int f = f0 + 8 * (i / 4) + 4 * (l >> 5) + i % 4, m = n * 32 + (l & 31);
+    if (f >= p.F || m >= p.M) continue;
+    float g = p.bias ? p.bias[f] : 0.f, u = p.bias ? p.bias[p.F + f] : 0.f;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) {
+      g += red[v][n][i][l];
+      u += red[v][n][i + 8][l];
+    }
+    float a, d;
+    gate_both<sizeof(T) == 2>(g, p.act, a, d);
+    ((T*)p.h)[(size_t)m * p.F + f] = (T)(a * u);
+    if (p.z) {
+      p.z[(size_t)m * 2 * p.F + f] = g;
+      p.z[(size_t)m * 2 * p.F + p.F + f] = u;
     }
   }
 }
@@ -175,7 +340,7 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float a, d;
-        gate_both(g[e], p.act, a, d);
+        gate_both<sizeof(T) == 2>(g[e], p.act, a, d);
         gg[e] = x[e] * u[e] * d;
         gu[e] = x[e] * a;
         sg[e] += gg[e];
@@ -215,9 +380,9 @@ struct ProductParams {
   void* out;            // [M][N], or splits slabs of it (f32)
   int out_f32, col_tiles, tiles, splits, chunk;
 };
-template <class T, bool ARC, int BM, int BN, int WM, int WN, bool ALIGNED>
-__global__ void __launch_bounds__(64 * WM * WN, 1) product_kernel(const ProductParams p) {
-  using G = TokGemm<T, ARC, true, BM, BN, WM, WN, ALIGNED>;
+template <class T, bool ARC, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) product_kernel(const ProductParams p) {
+  using G = TokGemm<T, ARC, true, BM, BN, WM, WN>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
   const int id = tok_xcd_order(blockIdx.x, gridDim.x);
   const int sp = id / p.tiles, t = id - sp * p.tiles;
@@ -258,7 +423,6 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* slabs, int s
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
-constexpr int kBM = 128, kBN = 128;
 
 template <class K>
 int allow_lds(K kernel, int bytes) {
@@ -273,30 +437,52 @@ int check_sizes(int M, int C, int F, int act) {
   VG_REQUIRE(M >= 0 && C >= 1 && F >= 1, "gated: bad sizes rows=%d in=%d out=%d", M, C, F);
   VG_REQUIRE(act >= VG_GATE_SIGMOID && act <= VG_GATE_SILU, "gated: unknown activation %d", act);
   // tile counts and row indices of 31 bits (element offsets are 64-bit)
-  VG_REQUIRE(M < (1 << 30) && C < (1 << 30) && F < (1 << 29) &&
-                 ((long long)M / kBM + 1) * ((long long)F * 2 / kBN + 1) < (1ll << 31) && ((long long)M / kBM + 1) * ((long long)C / kBN + 1) < (1ll << 31) / 64 &&
-                 ((long long)F * 2 / kBM + 1) * ((long long)C / kBN + 1) < (1ll << 31) / 64,
+  // ... and byte offsets inside a tile of 32
+  VG_REQUIRE(M < (1 << 30) && C < (1 << 21) && F < (1 << 20) &&
+                 ((long long)M / 128 + 1) * ((long long)F * 2 / 128 + 1) < (1ll << 31) && ((long long)M / 128 + 1) * ((long long)C / 128 + 1) < (1ll << 31) / 64 &&
+                 ((long long)F * 2 / 128 + 1) * ((long long)C / 128 + 1) < (1ll << 31) / 64,
              "gated: too many tiles (rows=%d in=%d out=%d)", M, C, F);
   return VG_OK;
 }
 
-template <class T, bool BWD>
-int launch_gated(GatedParams& p, hipStream_t st) {
-  p.row_tiles = ceil_div(p.M, kBM);
-  p.col_tiles = ceil_div(2ll * p.F, kBN);      // 64 output columns a tile
-  const bool aligned = vg_aligned16(p.x) && vg_aligned16(p.w) && p.C % TokNum<T>::V == 0;
-  const int grid = p.row_tiles * p.col_tiles;
-  auto go = [&](auto kernel, int lds) {
-    const int rc = allow_lds(kernel, lds);
-    if (rc) return rc;
-    kernel<<<grid, 256, lds, st>>>(p);
-    return (int)VG_OK;
-  };
-  const int rc = aligned ? go(gated_kernel<T, kBM, kBN, 2, 2, true, BWD>, TokGemm<T, false, false, kBM, kBN, 2, 2, true>::LDS_BYTES)
-                         : go(gated_kernel<T, kBM, kBN, 2, 2, false, BWD>, TokGemm<T, false, false, kBM, kBN, 2, 2, false>::LDS_BYTES);
+// Products are cut into 256 x 256 tiles (bf16: eight waves of 128 x 64, one block a CU) or 128 x 128 (two blocks a CU). The
+// large tile reads its operands half as often from the caches and takes 0.65 of the time of four small ones (16384 x 1024
+// x 8192: 284 us against 416); the small one wins where too few large ones are there for 256 compute units. f32 products
+// are bound by the matrix cores with either and take the small one, by eight waves of 64 x 32 (132 us against 139 with four
+// of 64 x 64, 4096 x 512 x 2816).
+constexpr double kLarge = 4 * 0.65;
+template <class T>
+bool large_tiles(long long M, long long N) {
+  const long long large = (long long)ceil_div(M, 256) * ceil_div(N, 256), small = (long long)ceil_div(M, 128) * ceil_div(N, 128);
+  return sizeof(T) == 2 && ceil_div(large, 256) * kLarge < ceil_div(small, 256);
+}
+template <class T, int BMN, int WM, int WN, bool BWD>
+int launch_gated_tiles(GatedParams& p, hipStream_t st) {
+  p.row_tiles = ceil_div(p.M, BMN);
+  p.col_tiles = ceil_div(2ll * p.F, BMN);      // BMN / 2 output columns a tile
+  using G = TokGemm<T, false, false, BMN, BMN, WM, WN>;
+  auto kernel = gated_kernel<T, BMN, BMN, WM, WN, BWD>;
+  const int rc = allow_lds(kernel, G::LDS_BYTES);
   if (rc) return rc;
+  kernel<<<p.row_tiles * p.col_tiles, G::NT, G::LDS_BYTES, st>>>(p);
   VG_CHECK_LAUNCH("gated");
   return VG_OK;
+}
+template <class T, bool BWD>
+int launch_gated(GatedParams& p, hipStream_t st) {
+  if constexpr (!BWD) {
+    if (p.M <= kFewRows) {
+      if (p.M <= 32)
+        gated_few_kernel<T, 1><<<ceil_div(p.F, 16), 64 * kFewWaves, 0, st>>>(p);
+      else
+        gated_few_kernel<T, 2><<<ceil_div(p.F, 16), 64 * kFewWaves, 0, st>>>(p);
+      VG_CHECK_LAUNCH("gated");
+      return VG_OK;
+    }
+  }
+  if constexpr (sizeof(T) == 2)
+    if (large_tiles<T>(p.M, 2ll * p.F)) return launch_gated_tiles<T, 256, 2, 4, BWD>(p, st);
+  return launch_gated_tiles<T, 128, 2, sizeof(T) == 4 ? 4 : 2, BWD>(p, st);
 }
 
 template <class T>
@@ -342,23 +528,53 @@ int gated_bwd_z(int M, int F, const float* z, const void* gh, void* gz, float* g
   return VG_OK;
 }
 
-// A product with fewer tiles than compute units is split along k towards one block for each, no split under 4 k-steps.
-int product_splits(int M, int N, int K) {
-  const long long tiles = (long long)ceil_div(M, kBM) * ceil_div(N, kBN);
-  if (tiles >= 192) return 1;
-  long long s = 256 / tiles, most = K / 256;
-  if (s > most) s = most;
-  return s < 1 ? 1 : (int)s;
+struct ProductPlan {
+  int tile, splits, chunk;
+};
+// A product with few tiles is split along k, each split into a slab of its own (f32), summed in order. With n blocks on
+// the busiest compute unit the time goes as n (K / splits + 128): 128 k for a block's start, its stores and its share of
+// the slab sum. No split under 256 k.
+template <class T>
+ProductPlan product_plan(int M, int N, int K) {
+  ProductPlan best = {128, 1, K};
+  double least = 1e30;
+  for (int tile = 128; tile <= (sizeof(T) == 2 ? 256 : 128); tile *= 2) {
+    const long long tiles = (long long)ceil_div(M, tile) * ceil_div(N, tile);
+    if (tile == 256 && (M < 256 || N < 256)) break;
+    for (int s = 1; s <= 64 && (s == 1 || K / s >= 256); ++s) {
+      const long long n = (tiles * s + 255) / 256;
+      const double t = (double)n * ((double)K / s + 128) * (tile == 256 ? kLarge : 1);
+      if (t < least * (s > 1 ? 0.97 : 1.0)) {
+        least = t;
+        best = {tile, s, K};
+      }
+    }
+  }
+  best.chunk = ((K + best.splits - 1) / best.splits + 63) & ~63;
+  return best;
 }
+template <class T>
 size_t product_bytes(int M, int N, int K) {
-  const int s = product_splits(M, N, K);
+  const int s = product_plan<T>(M, N, K).splits;
   return s == 1 ? 0 : (size_t)s * M * N * 4;
 }
 
+template <class T, bool ARC, int BMN, int WM, int WN>
+int launch_product(ProductParams& p, hipStream_t st) {
+  using G = TokGemm<T, ARC, true, BMN, BMN, WM, WN>;
+  p.col_tiles = ceil_div(p.N, BMN);
+  p.tiles = ceil_div(p.M, BMN) * p.col_tiles;
+  auto kernel = product_kernel<T, ARC, BMN, BMN, WM, WN>;
+  const int rc = allow_lds(kernel, G::LDS_BYTES);
+  if (rc) return rc;
+  kernel<<<p.tiles * p.splits, G::NT, G::LDS_BYTES, st>>>(p);
+  return VG_OK;
+}
 template <class T, bool ARC>
 int product(const void* a, int64_t lda, const void* b, int64_t ldb, int M, int N, int K, void* out, int out_f32, void* ws, size_t ws_bytes,
             hipStream_t st) {
-  const size_t need = product_bytes(M, N, K);
+  const ProductPlan plan = product_plan<T>(M, N, K);
+  const size_t need = product_bytes<T>(M, N, K);
   if (need && (!ws || ws_bytes < need)) return vg_fail(VG_ERR_WORKSPACE, "gated backward: workspace of %zu bytes, %zu are needed", ws_bytes, need);
   ProductParams p = {};
   p.a = a;
@@ -368,22 +584,15 @@ int product(const void* a, int64_t lda, const void* b, int64_t ldb, int M, int N
   p.M = M;
   p.N = N;
   p.K = K;
-  p.splits = product_splits(M, N, K);
-  p.chunk = ((K + p.splits - 1) / p.splits + 63) & ~63;
+  p.splits = plan.splits;
+  p.chunk = plan.chunk;
   p.out = p.splits > 1 ? ws : out;
   p.out_f32 = p.splits > 1 ? 1 : out_f32;
-  p.col_tiles = ceil_div(N, kBN);
-  p.tiles = ceil_div(M, kBM) * p.col_tiles;
-  const bool aligned = vg_aligned16(a) && vg_aligned16(b) && lda % TokNum<T>::V == 0 && ldb % TokNum<T>::V == 0;
-  const int grid = p.tiles * p.splits;
-  auto go = [&](auto kernel, int lds) {
-    const int rc = allow_lds(kernel, lds);
-    if (rc) return rc;
-    kernel<<<grid, 256, lds, st>>>(p);
-    return (int)VG_OK;
-  };
-  const int rc = aligned ? go(product_kernel<T, ARC, kBM, kBN, 2, 2, true>, TokGemm<T, ARC, true, kBM, kBN, 2, 2, true>::LDS_BYTES)
-                         : go(product_kernel<T, ARC, kBM, kBN, 2, 2, false>, TokGemm<T, ARC, true, kBM, kBN, 2, 2, false>::LDS_BYTES);
+  int rc;
+  if constexpr (sizeof(T) == 2)
+    rc = plan.tile == 256 ? launch_product<T, ARC, 256, 2, 4>(p, st) : launch_product<T, ARC, 128, 2, 2>(p, st);
+  else
+    rc = launch_product<T, ARC, 128, 2, 4>(p, st);
   if (rc) return rc;
   if (p.splits > 1) {
     const size_t n = (size_t)M * N;
@@ -427,8 +636,10 @@ int vg_gated_linear_bwd(int M, int F, const float* z, const float* gh, float* gz
 int vg_gated_linear_bwd_h(int M, int F, const float* z, const void* gh, void* gz, float* gb_part, int act, void* stream) {
   return gated_bwd_z<__bf16>(M, F, z, gh, gz, gb_part, act, stream);
 }
-int vg_gated_linear_partial_rows(int M, int recompute) { return M < 1 ? 0 : ceil_div(M, recompute ? kBM : kRowsBlock); }
-int vg_gated_linear_recomputes_h(int M, int C, int F) { return C <= 1024; }
+int vg_gated_linear_partial_rows(int M, int F, int recompute) {
+  return M < 1 ? 0 : ceil_div(M, !recompute ? kRowsBlock : large_tiles<__bf16>(M, 2ll * F) ? 256 : 128);
+}
+int vg_gated_linear_recomputes_h(int M, int C, int F) { return M > kFewRows && C <= 768; }
 int vg_gated_linear_rebwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const void* gh, void* gz, float* gb_part,
                             int act, void* stream) {
   const int rc = check_sizes(M, C, F, act);
@@ -448,10 +659,16 @@ int vg_gated_linear_rebwd_h(int M, int C, int F, const void* x, const void* w, c
   return launch_gated<__bf16, true>(p, (hipStream_t)stream);
 }
 size_t vg_gated_linear_gx_workspace_bytes(int M, int C, int F) {
-  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes(M, C, 2 * F);
+  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<float>(M, C, 2 * F);
+}
+size_t vg_gated_linear_gx_workspace_bytes_h(int M, int C, int F) {
+  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<__bf16>(M, C, 2 * F);
 }
 size_t vg_gated_linear_gw_workspace_bytes(int M, int C, int F) {
-  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes(2 * F, C, M);
+  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<float>(2 * F, C, M);
+}
+size_t vg_gated_linear_gw_workspace_bytes_h(int M, int C, int F) {
+  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<__bf16>(2 * F, C, M);
 }
 int vg_gated_linear_gx(int M, int C, int F, const float* gz, const float* w, float* gx, void* workspace, size_t workspace_bytes,
                        void* stream) {

@@ -5,8 +5,10 @@
 // Tiles go global -> registers -> LDS in 16-byte vectors, two LDS buffers, one barrier per k-step, the next k-step's
 // loads in flight under the products. KC tiles are kept [row][k] with 16 bytes of padding (a lane's 8 k are one
 // ds_read_b128); RC tiles are kept [k][row] as loaded and read with the transposing LDS load, which hands a lane 4
-// consecutive k of its row (f32: 4-byte loads). Operands whose rows do not start on 16-byte borders are loaded element by element
-// (ALIGNED = false): same tiles, same results.
+// consecutive k of its row (f32: 4-byte loads). A thread's offsets from the tile's first element are the same in every
+// k-step; only the uniform base moves. Row indices past the operand are clamped to its last row (what they produce is
+// not stored); k past the end becomes zero, in the last k-step only. The vector loads need no alignment beyond an
+// element's, so odd leading dimensions take the same path.
 #pragma once
 #include "token_common.h"
 
@@ -15,10 +17,14 @@ struct TokOperand {
   const T* p;
   int64_t ld;
   int rows;     // valid row indices
-  int split;    // KC with two interleaved halves (gate and value weights): rows of the second half start here; 0: plain
+  int split;    // KC, two interleaved halves (gate and value weights): rows of the second half start here; 0: plain
 };
 
-template <class T, bool RC, int ROWS, int BK, int NT, bool ALIGNED>
+// Order of the 32 rows of a block of an interleaved operand: a product leaves lane half h the rows 8 (i / 4) + 4 h + i % 4 of
+// its column; with this order those are the operand's rows 16 h + i, sixteen in a row that leave as one piece.
+__device__ __forceinline__ int tok_split_row(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
+
+template <class T, bool RC, int ROWS, int BK, int NT>
 struct TokStage {
   static constexpr int V = TokNum<T>::V;
   static constexpr int LD = RC ? ROWS + 32 : BK + V;                   // elements of an LDS row
@@ -27,42 +33,77 @@ struct TokStage {
   static constexpr int N = ROWS * BK / V / NT;
   static_assert(ROWS * BK / V % NT == 0, "whole vectors per thread");
   u32x4 r[N];
+  unsigned off[N];      // bytes from the base
+  const char* base;     // first row of the operand (KC) or first row of the tile (RC), at the current k
+  unsigned ragged;      // RC: vectors of this thread that are not 16 bytes inside the operand's rows, one bit each
+  bool edge;            // ... of any thread of the block
 
-  static __device__ __forceinline__ u32x4 vec(const T* p, int left) {   // `left` elements of the vector are inside
-    if constexpr (ALIGNED) {
-      return left > 0 ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
-    } else {
-      u32x4 out = {0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (sizeof(T) == 4) {
-          if (e < left) out[e] = *reinterpret_cast<const unsigned*>(p + e);
-        } else {
-          if (e < left) out[e / 2] |= (unsigned)*reinterpret_cast<const unsigned short*>(p + e) << (16 * (e % 2));
-        }
-      }
-      return out;
-    }
+  static __device__ __forceinline__ u32x4 whole(const char* p) {
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
   }
-  // rows row0.. of the operand, k from k0, nothing at or past kend
-  __device__ __forceinline__ void load(const TokOperand<T>& a, int row0, int k0, int kend) {
+  static __device__ __forceinline__ u32x4 part(const char* p, int left) {   // the first `left` elements, then zeros
+    u32x4 out = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if constexpr (sizeof(T) == 4) {
+        if (e < left) out[e] = *reinterpret_cast<const unsigned*>(p + 4 * e);
+      } else {
+        if (e < left) out[e / 2] |= (unsigned)*reinterpret_cast<const unsigned short*>(p + 2 * e) << (16 * (e % 2));
+      }
+    }
+    return out;
+  }
+  // rows row0.. of the operand, from k
+  __device__ __forceinline__ void place(const TokOperand<T>& a, int row0, int k) {
+    ragged = 0;
+    base = reinterpret_cast<const char*>(a.p + (RC ? k * a.ld + row0 : k + (a.split ? 0 : row0 * a.ld)));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = threadIdx.x + i * NT, lr = id / VPR, lv = (id % VPR) * V;
       if constexpr (RC) {
-        const int k = k0 + lr, row = row0 + lv;
-        r[i] = vec(a.p + k * a.ld + row, k < kend ? a.rows - row : 0);
+        const int left = a.rows - row0 - lv;
+        if (left < V && (left > 0 || a.rows - row0 < V)) ragged |= 1u << i;
+        off[i] = (unsigned)(((int64_t)lr * a.ld + (left > 0 ? lv : 0)) * (int)sizeof(T));
       } else {
-        int row = row0 + lr;
-        bool ok = row < a.rows;
-        if (a.split) {       // 32 rows of the first half, the matching 32 of the second, ...
-          const int f = (row >> 6) * 32 + (row & 31);
-          ok = f < a.split;
-          row = f + ((row >> 5) & 1) * a.split;
+        int row = lr;
+        if (a.split) {       // 32 rows of the first half, the matching 32 of the second, ... (tok_split_row)
+          const int v = row0 + lr, f = (v >> 6) * 32 + tok_split_row(v & 31);
+          row = (f < a.split ? f : a.split - 1) + ((v >> 5) & 1) * a.split;
+        } else if (row0 + row >= a.rows) {
+          row = a.rows - 1 - row0;
         }
-        r[i] = vec(a.p + row * a.ld + k0 + lv, ok ? kend - k0 - lv : 0);
+        off[i] = (unsigned)(((int64_t)row * a.ld + lv) * (int)sizeof(T));
       }
     }
+    edge = RC && row0 + ROWS > a.rows && a.rows % V != 0;
+  }
+  // the k-step at the base, all of it inside the operand; then on to the next
+  __device__ __forceinline__ void load_inside(const TokOperand<T>& a) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = whole(base + off[i]);
+    base += (RC ? BK * a.ld : BK) * (int64_t)sizeof(T);
+  }
+  // the k-step that starts at k, whatever lies outside
+  __device__ __forceinline__ void load(const TokOperand<T>& a, int row0, int k, int kend) {
+    if (k + BK <= kend && !edge) {
+      load_inside(a);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = threadIdx.x + i * NT, lr = id / VPR, lv = (id % VPR) * V;
+      int left;
+      if constexpr (RC) {
+        left = k + lr < kend ? a.rows - row0 - lv : 0;
+        if (k + lr < kend && left <= 0 && !(ragged >> i & 1)) left = V;      // (clamped: its values are not used)
+      } else {
+        left = kend - k - lv;
+      }
+      r[i] = left >= V ? whole(base + off[i]) : part(base + off[i], left);
+    }
+    base += (RC ? BK * a.ld : BK) * (int64_t)sizeof(T);
   }
   __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
@@ -104,18 +145,18 @@ __device__ __forceinline__ f32x16 tok_mma(f32x4 a, f32x4 b, f32x16 c) {
   return c;
 }
 
-template <class T, bool ARC, bool BRC, int BM, int BN, int WM, int WN, bool ALIGNED>
+template <class T, bool ARC, bool BRC, int BM, int BN, int WM, int WN>
 struct TokGemm {
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int BK = sizeof(T) == 2 ? 64 : 32;
   static constexpr int TM = BM / (32 * WM), TN = BN / (32 * WN);
   static constexpr int KS = sizeof(T) == 2 ? 16 : 8;        // k of one fragment
-  using SA = TokStage<T, ARC, BM, BK, NT, ALIGNED>;
-  using SB = TokStage<T, BRC, BN, BK, NT, ALIGNED>;
+  using SA = TokStage<T, ARC, BM, BK, NT>;
+  using SB = TokStage<T, BRC, BN, BK, NT>;
   static constexpr int BUF = SA::ELEMS + SB::ELEMS;
   static constexpr int LDS_BYTES = 2 * BUF * (int)sizeof(T);
 
-  // acc over k in [kbeg, kend); smem holds LDS_BYTES. All threads of the block call it.
+  // acc over k in [kbeg, kend); smem holds LDS_BYTES. All threads of the block call it; both operands have rows.
   static __device__ __forceinline__ void run(const TokOperand<T>& A, const TokOperand<T>& B, int m0, int n0, int kbeg, int kend, T* smem,
                                              f32x16 (&acc)[TM][TN]) {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -128,40 +169,67 @@ struct TokGemm {
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     SA sa;
     SB sb;
+    sa.place(A, m0, kbeg);
+    sb.place(B, n0, kbeg);
+    using FA = decltype(SA::frag(smem, 0, 0, 0));
+    constexpr int S = BK / KS;
     int buf = 0;
+    // One k-step on buffer `buf`. The registers hold the next one: it goes to the other buffer under the products, and
+    // the one behind it is requested then, a whole k-step before its own turn.
+    auto step = [&](auto inside, int k) {
+      const T* ta = smem + buf * BUF;
+      const T* tb = ta + SA::ELEMS;
+      FA fa[2][TM], fb[2][TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[0][i] = SA::frag(ta, mw + 32 * i, 0, lane);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[0][j] = SB::frag(tb, nw + 32 * j, 0, lane);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s + 1 < S) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) fa[(s + 1) & 1][i] = SA::frag(ta, mw + 32 * i, s + 1, lane);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) fb[(s + 1) & 1][j] = SB::frag(tb, nw + 32 * j, s + 1, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = tok_mma(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+        if (s == 0) {
+          T* next = smem + (buf ^ 1) * BUF;
+          if constexpr (decltype(inside)::value) {
+            sa.store(next);
+            sb.store(next + SA::ELEMS);
+            sa.load_inside(A);
+            sb.load_inside(B);
+          } else if (k + BK < kend) {
+            sa.store(next);
+            sb.store(next + SA::ELEMS);
+            if (k + 2 * BK < kend) {
+              sa.load(A, m0, k + 2 * BK, kend);
+              sb.load(B, n0, k + 2 * BK, kend);
+            }
+          }
+        }
+      }
+      __syncthreads();
+      buf ^= 1;
+    };
     if (kbeg < kend) {
       sa.load(A, m0, kbeg, kend);
       sb.load(B, n0, kbeg, kend);
       sa.store(smem);
       sb.store(smem + SA::ELEMS);
+      if (kbeg + BK < kend) {
+        sa.load(A, m0, kbeg + BK, kend);
+        sb.load(B, n0, kbeg + BK, kend);
+      }
     }
     __syncthreads();
-    for (int k = kbeg; k < kend; k += BK) {
-      const bool more = k + BK < kend;
-      if (more) {
-        sa.load(A, m0, k + BK, kend);
-        sb.load(B, n0, k + BK, kend);
-      }
-      const T* ta = smem + buf * BUF;
-      const T* tb = ta + SA::ELEMS;
-#pragma unroll
-      for (int s = 0; s < BK / KS; ++s) {
-        decltype(SA::frag(ta, 0, 0, 0)) fa[TM], fb[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) fa[i] = SA::frag(ta, mw + 32 * i, s, lane);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) fb[j] = SB::frag(tb, nw + 32 * j, s, lane);
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = tok_mma(fa[i], fb[j], acc[i][j]);
-      }
-      if (more) {
-        sa.store(smem + (buf ^ 1) * BUF);
-        sb.store(smem + (buf ^ 1) * BUF + SA::ELEMS);
-      }
-      __syncthreads();
-      buf ^= 1;
-    }
+    int k = kbeg;
+    if (!sa.edge && !sb.edge)
+      for (; k + 3 * BK <= kend; k += BK) step(std::true_type{}, k);
+    for (; k < kend; k += BK) step(std::false_type{}, k);
   }
 };

@@ -195,11 +195,13 @@ SIGNATURES = {
     "vg_gated_linear_fwd_h": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
     "vg_gated_linear_bwd": (c_int, [c_int] * 2 + [_P] * 4 + [c_int, _P]),
     "vg_gated_linear_bwd_h": (c_int, [c_int] * 2 + [_P] * 4 + [c_int, _P]),
-    "vg_gated_linear_partial_rows": (c_int, [c_int, c_int]),
+    "vg_gated_linear_partial_rows": (c_int, [c_int] * 3),
     "vg_gated_linear_recomputes_h": (c_int, [c_int] * 3),
     "vg_gated_linear_rebwd_h": (c_int, [c_int] * 3 + [_P] * 6 + [c_int, _P]),
     "vg_gated_linear_gx_workspace_bytes": (c_size_t, [c_int] * 3),
     "vg_gated_linear_gw_workspace_bytes": (c_size_t, [c_int] * 3),
+    "vg_gated_linear_gx_workspace_bytes_h": (c_size_t, [c_int] * 3),
+    "vg_gated_linear_gw_workspace_bytes_h": (c_size_t, [c_int] * 3),
     "vg_gated_linear_gx": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
     "vg_gated_linear_gx_h": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
     "vg_gated_linear_gw": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),

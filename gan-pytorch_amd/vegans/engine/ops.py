@@ -2199,7 +2199,7 @@ class GatedLinearFn(Function):
         with _on(xm):
             gz = torch.empty((m, 2 * f), dtype=xm.dtype, device=xm.device)
             want_gb = params and bias is not None and need[2]
-            rows = lib.vg_gated_linear_partial_rows(m, int(z is None))
+            rows = lib.vg_gated_linear_partial_rows(m, f, int(z is None))
             part = torch.empty((rows, 2 * f), dtype=F32, device=xm.device) if want_gb else None
             if z is None:
                 call("vg_gated_linear_rebwd_h", m, c, f, _p(xm), _p(wm), _ptr(bias), _p(gh), _p(gz), _ptr(part), act, _stream())
@@ -2214,11 +2214,11 @@ class GatedLinearFn(Function):
                     call("vg_fill", _ptr(gb), c_float(0.0), c_size_t(2 * f), _stream())
             if _wants_input_grad(ctx, xm):
                 gx = torch.empty((m, c), dtype=xm.dtype, device=xm.device)
-                scratch, keep = _scratch(lib.vg_gated_linear_gx_workspace_bytes(m, c, f), xm.device)
+                scratch, keep = _scratch(getattr(lib, _A("vg_gated_linear_gx_workspace_bytes", xm))(m, c, f), xm.device)
                 call(_A("vg_gated_linear_gx", xm), m, c, f, _p(gz), _p(wm), _p(gx), *scratch, _stream())
             if params and need[1]:
                 gw = torch.empty((2 * f, c), dtype=w.dtype, device=xm.device)
-                scratch, keep = _scratch(lib.vg_gated_linear_gw_workspace_bytes(m, c, f), xm.device)
+                scratch, keep = _scratch(getattr(lib, _A("vg_gated_linear_gw_workspace_bytes", xm))(m, c, f), xm.device)
                 if xm.dtype == BF16:
                     call("vg_gated_linear_gw_h", m, c, f, _p(gz), _p(xm), _p(gw), int(gw.dtype == F32), *scratch, _stream())
                 else:

@@ -524,7 +524,7 @@ int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k,
  *   vg_gated_linear_bwd       gz [M][2F] = gradient of the pre-activations from z and gh
  *   vg_gated_linear_rebwd_h   the same from x and w (what vg_gated_linear_recomputes_h prefers to a stored z)
  *   vg_gated_linear_gx / _gw  gx = gz w, gw = gz^T x (_h: f32 where gw_f32, else bf16); scratch: *_workspace_bytes
- * gb_part [vg_gated_linear_partial_rows(M, recompute)][2F] f32, nullable: its column sums are the bias gradient. */
+ * gb_part [vg_gated_linear_partial_rows(M, F, recompute)][2F] f32, nullable: its column sums are the bias gradient. */
 #define VG_GATE_SIGMOID 0
 #define VG_GATE_RELU 1
 #define VG_GATE_GELU 2
@@ -533,12 +533,14 @@ int vg_gated_linear_fwd(int M, int C, int F, const float* x, const float* w, con
 int vg_gated_linear_fwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, void* h, float* z, int act, void* stream);
 int vg_gated_linear_bwd(int M, int F, const float* z, const float* gh, float* gz, float* gb_part, int act, void* stream);
 int vg_gated_linear_bwd_h(int M, int F, const float* z, const void* gh, void* gz, float* gb_part, int act, void* stream);
-int vg_gated_linear_partial_rows(int M, int recompute);
+int vg_gated_linear_partial_rows(int M, int F, int recompute);
 int vg_gated_linear_recomputes_h(int M, int C, int F);
 int vg_gated_linear_rebwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const void* gh, void* gz, float* gb_part,
                             int act, void* stream);
 size_t vg_gated_linear_gx_workspace_bytes(int M, int C, int F);
 size_t vg_gated_linear_gw_workspace_bytes(int M, int C, int F);
+size_t vg_gated_linear_gx_workspace_bytes_h(int M, int C, int F);
+size_t vg_gated_linear_gw_workspace_bytes_h(int M, int C, int F);
 int vg_gated_linear_gx(int M, int C, int F, const float* gz, const float* w, float* gx, void* workspace, size_t workspace_bytes,
                        void* stream);
 int vg_gated_linear_gw(int M, int C, int F, const float* gz, const float* x, float* gw, void* workspace, size_t workspace_bytes,

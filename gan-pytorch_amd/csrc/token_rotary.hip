@@ -7,9 +7,12 @@
 //
 // Bound by HBM: one read and one write per element forward, two reads and one write backward. A thread holds one
 // 16-byte vector of a head, a power of two of neighbouring lanes the head, and a wave one token (or several, where its
-// heads do not fill it) whose heads it walks: the angles depend on the token and the lane's place in the head only, so
-// the sine and cosine are worked out once per token and thread, not per head. The angle is formed in 64 bits, in
-// turns, and reduced to half a turn before it becomes an f32, so far positions keep their accuracy.
+// heads do not fill it) whose heads it walks, queries, then keys: the angles depend on the token and the lane's place in
+// the head only, so the sine and cosine are worked out once per token and thread, not per head, under the loads of the
+// heads. The angle is formed in 64 bits, in turns, and reduced to half a turn before it becomes an f32, so far positions
+// keep their accuracy.
+#include <math.h>
+
 #include "token_common.h"
 
 namespace {
@@ -23,15 +26,20 @@ struct RotaryParams {
   float* part;            // backward: [blocks][2][D] partial sums of the weight gradients
   int lph, hps;           // lanes of a head, head slots of a wave's token group
   int wave_tokens;        // tokens a wave works on at once
+  double decay[4];        // log2 of the ratio of neighbouring elements' frequencies on an axis
 };
 
 constexpr int kUnroll = 4;          // head steps whose loads are in flight together
-constexpr int kBwdBlocks = 512;     // rows of partial weight-gradient sums at most
+// Blocks of four waves: as many as run at once (registers: four waves a SIMD forward, three backward), so that a wave's
+// start (frequencies in 64 bits) is spread over as many tokens as can be. Measured on 4 x 8192 tokens, 20 heads of 128, bf16
+// (336 MB forward, 503 MB backward): forward 1024 blocks 81 us (4.1 TB/s), 2048 86, 512 108; backward 768 blocks 128 us
+// (3.9 TB/s), 512 at two waves a SIMD 141.
+constexpr int kBlocks = 1024;
+constexpr int kBwdBlocks = 768;     // rows of partial weight-gradient sums at most
 
 template <int V>
-__device__ __forceinline__ void angles(const RotaryParams& p, long long token, int t, int b, const double (&freq)[V / 2],
-                                       const int (&axis)[V / 2], float (&c)[V / 2], float (&s)[V / 2]) {
-  const long long at = (long long)b * p.g.pos_sb + (long long)t * p.g.axes;
+__device__ __forceinline__ void angles(const RotaryParams& p, long long at, const double (&freq)[V / 2], const int (&axis)[V / 2],
+                                       float (&c)[V / 2], float (&s)[V / 2]) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
     c[i] = 1.f;
@@ -44,8 +52,23 @@ __device__ __forceinline__ void angles(const RotaryParams& p, long long token, i
   }
 }
 
+// sum over the `lanes` (a power of two) neighbouring lanes of a head, in every one of them
+template <int CTRL>
+__device__ __forceinline__ float plus_lane(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float head_sum(float v, int lanes) {
+  if (lanes >= 2) v = plus_lane<0xB1>(v);      // lane ^ 1
+  if (lanes >= 4) v = plus_lane<0x4E>(v);      // lane ^ 2
+  if (lanes >= 8) v = plus_lane<0x141>(v);     // mirrored in 8: the other four's sum
+  if (lanes >= 16) v = plus_lane<0x140>(v);    // mirrored in 16
+  if (lanes >= 32) v += __shfl_xor(v, 16, 64);
+  if (lanes >= 64) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+
 template <class T, bool BWD>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryParams p) {
   constexpr int V = TokNum<T>::V;
   const vg_rotary_geom& g = p.g;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -61,18 +84,19 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
     axis[i] = -1;
-    freq[i] = 0.0;
     int d = d0 + 2 * i;
+    double e = 0.0;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       if (a < g.axes && axis[i] < 0) {
         if (d < g.width[a]) {
           axis[i] = a;
-          freq[i] = exp2(-(double)d / (double)g.width[a] * log2(g.base)) * 0.15915494309189533577;
+          e = (double)d * p.decay[a];
         }
         d -= g.width[a];
       }
     }
+    freq[i] = g.axes ? exp2(e) * 0.15915494309189533577 : 0.0;
     if (!in) axis[i] = -1;
   }
   float wq[V], wk[V], sq[V], sk[V];                    // weights, and (backward) sums of their gradients
@@ -84,33 +108,39 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   }
   const float inv_d = 1.f / (float)g.D;
   const long long tokens = (long long)g.B * g.T;
-  const long long step = (long long)gridDim.x * 4 * p.wave_tokens;
-  for (long long base = ((long long)blockIdx.x * 4 + wid) * p.wave_tokens; base < tokens; base += step) {
+  const long long stride = (long long)gridDim.x * 4 * p.wave_tokens;
+  const int q_steps = (g.Hq + p.hps - 1) / p.hps, steps = q_steps + (g.Hk + p.hps - 1) / p.hps;
+  for (long long base = ((long long)blockIdx.x * 4 + wid) * p.wave_tokens; base < tokens; base += stride) {
     const long long token = base + sub;
     const bool tok = token < tokens;
     const int b = tok ? (int)(token / g.T) : 0, t = tok ? (int)(token - (long long)b * g.T) : 0;
     float c[V / 2], s[V / 2];
-    angles<V>(p, token, t, b, freq, axis, c, s);
-    // one side (queries, keys) after the other; kUnroll head steps of loads at a time
-    auto side = [&](const T* x, const vg_heads_layout& lx, const T* gy, const vg_heads_layout& lg, T* out, const vg_heads_layout& lo,
-                    int heads, const float (&w)[V], bool normed, float (&sum)[V]) {
-      const T* xb = x + b * lx.sb + t * lx.st + d0;
-      const T* gb = BWD ? gy + b * lg.sb + t * lg.st + d0 : nullptr;
-      T* ob = out + b * lo.sb + t * lo.st + d0;
-      for (int h0 = 0; h0 < heads; h0 += p.hps * kUnroll) {
-        u32x4 rx[kUnroll], rg[kUnroll];
+    for (int s0 = 0; s0 < steps; s0 += kUnroll) {
+      u32x4 rx[kUnroll], rg[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int h = h0 + u * p.hps + slot;
-          const bool ok = tok && in && h < heads;
-          rx[u] = ok && (!BWD || normed) ? *reinterpret_cast<const u32x4*>(xb + h * lx.sh) : u32x4{0, 0, 0, 0};
-          if constexpr (BWD) rg[u] = ok ? *reinterpret_cast<const u32x4*>(gb + h * lg.sh) : u32x4{0, 0, 0, 0};
+      for (int u = 0; u < kUnroll; ++u) {
+        const bool isq = s0 + u < q_steps;                       // uniform
+        const int h = (s0 + u - (isq ? 0 : q_steps)) * p.hps + slot;
+        const bool ok = tok && in && s0 + u < steps && h < (isq ? g.Hq : g.Hk);
+        const vg_heads_layout& lx = isq ? g.q : g.k;
+        const T* x = (const T*)(isq ? p.q : p.k) + b * lx.sb + t * lx.st + h * lx.sh + d0;
+        rx[u] = ok && (!BWD || (isq ? p.wq : p.wk)) ? *reinterpret_cast<const u32x4*>(x) : u32x4{0, 0, 0, 0};
+        if constexpr (BWD) {
+          const vg_heads_layout& lg = isq ? g.gq : g.gk;
+          const T* gy = (const T*)(isq ? p.gq : p.gk) + b * lg.sb + t * lg.st + h * lg.sh + d0;
+          rg[u] = ok ? *reinterpret_cast<const u32x4*>(gy) : u32x4{0, 0, 0, 0};
         }
+      }
+      if (s0 == 0) angles<V>(p, (long long)b * g.pos_sb + (long long)t * g.axes, freq, axis, c, s);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (h0 + u * p.hps >= heads) break;          // uniform over the wave
-          const int h = h0 + u * p.hps + slot;
-          const bool ok = tok && in && h < heads;
+      for (int u = 0; u < kUnroll; ++u) {
+        if (s0 + u >= steps) break;          // uniform
+        const bool isq = s0 + u < q_steps;
+        const int h = (s0 + u - (isq ? 0 : q_steps)) * p.hps + slot;
+        const bool ok = tok && in && h < (isq ? g.Hq : g.Hk);
+        const vg_heads_layout& lo = isq ? g.oq : g.ok;
+        T* out = (T*)(isq ? p.oq : p.ok) + b * lo.sb + t * lo.st + h * lo.sh + d0;
+        auto one = [&](const float (&w)[V], bool normed, float (&sum)[V]) {
           float xv[V], y[V];
           tok_widen(rx[u], xv);
           float r = 1.f;
@@ -118,8 +148,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) ss = __builtin_fmaf(xv[e], xv[e], ss);
-            for (int o = p.lph >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            r = 1.f / sqrtf(__builtin_fmaf(ss, inv_d, g.eps));
+            r = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum(ss, p.lph), inv_d, g.eps));
           }
           if constexpr (!BWD) {
 #pragma unroll
@@ -133,9 +162,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
             tok_widen(rg[u], gv);
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
-              const float g0 = gv[2 * i] * c[i] + gv[2 * i + 1] * s[i], g1 = gv[2 * i + 1] * c[i] - gv[2 * i] * s[i];
-              y[2 * i] = g0;
-              y[2 * i + 1] = g1;
+              y[2 * i] = gv[2 * i] * c[i] + gv[2 * i + 1] * s[i];
+              y[2 * i + 1] = gv[2 * i + 1] * c[i] - gv[2 * i] * s[i];
             }
             if (normed) {
 #pragma unroll
@@ -146,18 +174,19 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
                 xv[e] = xh;
                 y[e] = wg;
               }
-              for (int o = p.lph >> 1; o > 0; o >>= 1) inner += __shfl_xor(inner, o, 64);
-              inner *= inv_d;
+              inner = head_sum(inner, p.lph) * inv_d;
 #pragma unroll
               for (int e = 0; e < V; ++e) y[e] = r * __builtin_fmaf(-xv[e], inner, y[e]);
             }
           }
-          if (ok) *reinterpret_cast<u32x4*>(ob + h * lo.sh) = tok_narrow(y);
-        }
+          if (ok) *reinterpret_cast<u32x4*>(out) = tok_narrow(y);
+        };
+        if (isq)
+          one(wq, p.wq != nullptr, sq);
+        else
+          one(wk, p.wk != nullptr, sk);
       }
-    };
-    side((const T*)p.q, g.q, (const T*)p.gq, g.gq, (T*)p.oq, g.oq, g.Hq, wq, p.wq != nullptr, sq);
-    if (g.Hk) side((const T*)p.k, g.k, (const T*)p.gk, g.gk, (T*)p.ok, g.ok, g.Hk, wk, p.wk != nullptr, sk);
+    }
   }
   if constexpr (BWD) {
     if (!p.part) return;
@@ -179,19 +208,22 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   }
 }
 
-// gw[which][d] = sum over blocks of part[block][which][d]: 32 columns and 8 row lanes per workgroup
-__global__ void __launch_bounds__(256) rotary_weight_kernel(const float* part, int rows, int D, float* gwq, float* gwk) {
-  __shared__ float red[8][32];
+// gw[which][d] = sum over blocks of part[block][which][d]: 32 columns and 32 row lanes per workgroup, every lane's rows
+// requested before the first is added
+__global__ void __launch_bounds__(1024) rotary_weight_kernel(const float* part, int rows, int D, float* gwq, float* gwk) {
+  __shared__ float red[32][33];
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int i = blockIdx.x * 32 + col;
-  float v = 0.f;
-  if (i < 2 * D)
-    for (int r = row; r < rows; r += 8) v += part[(size_t)r * 2 * D + i];
+  float got[kBwdBlocks / 32], v = 0.f;
+#pragma unroll
+  for (int r = 0; r < kBwdBlocks / 32; ++r) got[r] = i < 2 * D && row + 32 * r < rows ? part[(size_t)(row + 32 * r) * 2 * D + i] : 0.f;
+#pragma unroll
+  for (int r = 0; r < kBwdBlocks / 32; ++r) v += got[r];
   red[row][col] = v;
   __syncthreads();
   if (row == 0 && i < 2 * D) {
 #pragma unroll
-    for (int r = 1; r < 8; ++r) v += red[r][col];
+    for (int r = 1; r < 32; ++r) v += red[r][col];
     float* out = i < D ? gwq : gwk;
     if (out) out[i < D ? i : i - D] = v;
   }
@@ -223,6 +255,7 @@ void plan(RotaryParams& p, int V) {
   const int heads = p.g.Hq > p.g.Hk ? p.g.Hq : p.g.Hk;
   p.hps = pow2(heads) < 64 / p.lph ? pow2(heads) : 64 / p.lph;
   p.wave_tokens = 64 / (p.lph * p.hps);
+  for (int a = 0; a < p.g.axes; ++a) p.decay[a] = -log2(p.g.base) / p.g.width[a];
 }
 
 long long wave_groups(const RotaryParams& p) { return ((long long)p.g.B * p.g.T + p.wave_tokens - 1) / p.wave_tokens; }
@@ -237,10 +270,10 @@ int rotary_fwd(const vg_rotary_geom* g, const void* q, const void* k, const floa
   VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->T, g->Hq) && tok_layout_ok<T>(g->oq, yq, g->B, g->T, g->Hq) &&
                  (g->Hk == 0 || (tok_layout_ok<T>(g->k, k, g->B, g->T, g->Hk) && tok_layout_ok<T>(g->ok, yk, g->B, g->T, g->Hk))),
              "rotary: a head does not start on a 16-byte border");
-  RotaryParams p = {*g, q, k, nullptr, nullptr, yq, yk, wq, wk, pos, nullptr, 0, 0, 0};
+  RotaryParams p = {*g, q, k, nullptr, nullptr, yq, yk, wq, wk, pos};
   plan(p, TokNum<T>::V);
   long long blocks = (wave_groups(p) + 3) / 4;
-  if (blocks > 4096) blocks = 4096;
+  if (blocks > kBlocks) blocks = kBlocks;
   rotary_kernel<T, false><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(p);
   VG_CHECK_LAUNCH("rotary");
   return VG_OK;
@@ -260,7 +293,7 @@ int rotary_bwd(const vg_rotary_geom* g, const void* q, const void* k, const floa
   VG_REQUIRE((!gwq || wq) && (!gwk || wk), "rotary: gradient of a weight that is not there");
   const bool sums = gwq || gwk;
   hipStream_t st = (hipStream_t)stream;
-  RotaryParams p = {*g, q, k, gyq, gyk, gq, gk, wq, wk, pos, nullptr, 0, 0, 0};
+  RotaryParams p = {*g, q, k, gyq, gyk, gq, gk, wq, wk, pos};
   plan(p, TokNum<T>::V);
   int blocks = 0;
   if ((long long)g->B * g->T != 0) {
@@ -280,7 +313,7 @@ int rotary_bwd(const vg_rotary_geom* g, const void* q, const void* k, const floa
     VG_CHECK_LAUNCH("rotary backward");
   }
   if (sums) {      // (no tokens: zeros)
-    rotary_weight_kernel<<<(2 * g->D + 31) / 32, 256, 0, st>>>(p.part, blocks, g->D, gwq, gwk);
+    rotary_weight_kernel<<<(2 * g->D + 31) / 32, 1024, 0, st>>>(p.part, blocks, g->D, gwq, gwk);
     VG_CHECK_LAUNCH("rotary weight gradient");
   }
   return VG_OK;

@@ -503,31 +503,6 @@ int gated_fwd(int M, int C, int F, const void* x, const void* w, const float* bi
   return launch_gated<T, false>(p, (hipStream_t)stream);
 }
 
-template <class T>
-int gated_bwd_z(int M, int F, const float* z, const void* gh, void* gz, float* gb_part, int act, void* stream) {
-  const int rc = check_sizes(M, 1, F, act);
-  if (rc || M == 0) return rc;
-  VG_REQUIRE(z && gh && gz, "gated backward: null tensor");
-  VG_REQUIRE(ceil_div(F, 64) <= 65535, "gated backward: %d columns are too many", F);
-  GatedParams p = {};
-  p.z = const_cast<float*>(z);
-  p.gh = gh;
-  p.gz = gz;
-  p.gb_part = gb_part;
-  p.M = M;
-  p.F = F;
-  p.act = act;
-  hipStream_t st = (hipStream_t)stream;
-  const bool wide = F % 4 == 0 && vg_aligned16(z) && vg_aligned16(gh) && vg_aligned16(gz);
-  const dim3 grid(ceil_div(M, kRowsBlock), ceil_div(F, wide ? 256 : 64));
-  if (wide)
-    gated_bwd_kernel<T, 4><<<grid, 256, 0, st>>>(p);
-  else
-    gated_bwd_kernel<T, 1><<<grid, 256, 0, st>>>(p);
-  VG_CHECK_LAUNCH("gated backward");
-  return VG_OK;
-}
-
 struct ProductPlan {
   int tile, splits, chunk;
 };
@@ -605,19 +580,84 @@ int product(const void* a, int64_t lda, const void* b, int64_t ldb, int M, int N
   return VG_OK;
 }
 
+// What the backward pass of these sizes runs on: pre-activations kept by the forward pass in f32 (8 bytes written and read
+// an element), or, with bf16 operands, computed again. 16384 x C x 4096, forward and backward: C = 256 623 us again, 742
+// kept; 512 829 and 884; 1024 1249 and 1198. (Up to 64 rows the forward kernel has no backward twin.)
 template <class T>
-int gated_gx(int M, int C, int F, const void* gz, const void* w, void* gx, void* ws, size_t ws_bytes, void* stream) {
-  const int rc = check_sizes(M, C, F, VG_GATE_SILU);
-  if (rc || M == 0) return rc;
-  VG_REQUIRE(gz && w && gx, "gated backward: null tensor");
-  return product<T, false>(gz, 2 * (int64_t)F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, ws, ws_bytes, (hipStream_t)stream);
+bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 768; }
+
+// Scratch of the backward pass, one piece after the other: [gg gu], partial column sums and their reduction's scratch,
+// slabs of the two products (one after the other on one stream: they share the space).
+struct BwdSpace {
+  size_t gz, part, colsum, slabs, total;
+  int rows;          // of partial column sums
+};
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+template <class T>
+BwdSpace bwd_space(int M, int C, int F) {
+  BwdSpace s;
+  s.rows = ceil_div(M, keeps_z<T>(M, C) ? kRowsBlock : large_tiles<T>(M, 2ll * F) ? 256 : 128);
+  s.gz = 0;
+  s.part = align256((size_t)M * 2 * F * sizeof(T));
+  s.colsum = s.part + align256((size_t)s.rows * 2 * F * 4);
+  s.slabs = s.colsum + align256(vg_colsum_workspace_bytes(s.rows, 2 * F));
+  const size_t a = product_bytes<T>(M, C, 2 * F), b = product_bytes<T>(2 * F, C, M);
+  s.total = s.slabs + (a > b ? a : b);
+  return s;
 }
+
 template <class T>
-int gated_gw(int M, int C, int F, const void* gz, const void* x, void* gw, int gw_f32, void* ws, size_t ws_bytes, void* stream) {
-  const int rc = check_sizes(M, C, F, VG_GATE_SILU);
+int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bias, const float* z, const void* gh, void* gx, void* gw,
+              int gw_f32, float* gb, int act, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_sizes(M, C, F, act);
   if (rc) return rc;
-  VG_REQUIRE(gw && (M == 0 || (gz && x)), "gated backward: null tensor");
-  return product<T, true>(gz, 2 * (int64_t)F, x, C, 2 * F, C, M, gw, gw_f32, ws, ws_bytes, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (M == 0) {        // sums over no rows
+    if (gw) rc = product<T, true>(gh, 2 * (int64_t)F, x, C, 2 * F, C, 0, gw, gw_f32, nullptr, 0, st);
+    if (!rc && gb) rc = vg_fill(gb, 0.f, 2 * (size_t)F, stream);
+    return rc;
+  }
+  VG_REQUIRE(x && w && gh, "gated backward: null tensor");
+  VG_REQUIRE(!keeps_z<T>(M, C) || z, "gated backward: these sizes need the pre-activations of the forward pass");
+  VG_REQUIRE(ceil_div(F, 64) <= 65535, "gated backward: %d columns are too many", F);
+  const BwdSpace s = bwd_space<T>(M, C, F);
+  if (!ws || ws_bytes < s.total) return vg_fail(VG_ERR_WORKSPACE, "gated backward: workspace of %zu bytes, %zu are needed", ws_bytes, s.total);
+  VG_REQUIRE(vg_aligned16(ws), "gated backward: workspace is not 16-byte aligned");
+  char* at = (char*)ws;
+  GatedParams p = {};
+  p.x = x;
+  p.w = w;
+  p.bias = bias;
+  p.gh = gh;
+  p.gz = at + s.gz;
+  p.gb_part = gb ? (float*)(at + s.part) : nullptr;
+  p.M = M;
+  p.C = C;
+  p.F = F;
+  p.act = act;
+  if (keeps_z<T>(M, C)) {
+    p.z = const_cast<float*>(z);
+    const bool wide = F % 4 == 0 && vg_aligned16(z) && vg_aligned16(gh);
+    const dim3 grid(ceil_div(M, kRowsBlock), ceil_div(F, wide ? 256 : 64));
+    if (wide)
+      gated_bwd_kernel<T, 4><<<grid, 256, 0, st>>>(p);
+    else
+      gated_bwd_kernel<T, 1><<<grid, 256, 0, st>>>(p);
+    VG_CHECK_LAUNCH("gated backward");
+  } else if constexpr (sizeof(T) == 2) {
+    rc = launch_gated<T, true>(p, st);
+    if (rc) return rc;
+  }
+  if (gb) {
+    rc = vg_colsum((const float*)(at + s.part), gb, s.rows, 2 * F, at + s.colsum, s.slabs - s.colsum, stream);
+    if (rc) return rc;
+  }
+  if (gx) {
+    rc = product<T, false>(p.gz, 2 * (int64_t)F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, at + s.slabs, s.total - s.slabs, st);
+    if (rc) return rc;
+  }
+  if (gw) rc = product<T, true>(p.gz, 2 * (int64_t)F, x, C, 2 * F, C, M, gw, gw_f32, at + s.slabs, s.total - s.slabs, st);
+  return rc;
 }
 
 }  // namespace
@@ -630,61 +670,19 @@ int vg_gated_linear_fwd(int M, int C, int F, const float* x, const float* w, con
 int vg_gated_linear_fwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, void* h, float* z, int act, void* stream) {
   return gated_fwd<__bf16>(M, C, F, x, w, bias, h, z, act, stream);
 }
-int vg_gated_linear_bwd(int M, int F, const float* z, const float* gh, float* gz, float* gb_part, int act, void* stream) {
-  return gated_bwd_z<float>(M, F, z, gh, gz, gb_part, act, stream);
+int vg_gated_linear_keeps_z(int M, int C, int F, int half) { return half ? keeps_z<__bf16>(M, C) : keeps_z<float>(M, C); }
+size_t vg_gated_linear_bwd_workspace_bytes(int M, int C, int F, int half) {
+  if (check_sizes(M, C, F, VG_GATE_SILU) || M == 0) return 0;
+  return half ? bwd_space<__bf16>(M, C, F).total : bwd_space<float>(M, C, F).total;
 }
-int vg_gated_linear_bwd_h(int M, int F, const float* z, const void* gh, void* gz, float* gb_part, int act, void* stream) {
-  return gated_bwd_z<__bf16>(M, F, z, gh, gz, gb_part, act, stream);
+int vg_gated_linear_bwd(int M, int C, int F, const float* x, const float* w, const float* bias, const float* z, const float* gh, float* gx,
+                        float* gw, int gw_f32, float* gb, int act, void* workspace, size_t workspace_bytes, void* stream) {
+  VG_REQUIRE(gw_f32 || !gw, "gated backward: f32 tensors have an f32 weight gradient");
+  return gated_bwd<float>(M, C, F, x, w, bias, z, gh, gx, gw, 1, gb, act, workspace, workspace_bytes, stream);
 }
-int vg_gated_linear_partial_rows(int M, int F, int recompute) {
-  return M < 1 ? 0 : ceil_div(M, !recompute ? kRowsBlock : large_tiles<__bf16>(M, 2ll * F) ? 256 : 128);
-}
-int vg_gated_linear_recomputes_h(int M, int C, int F) { return M > kFewRows && C <= 768; }
-int vg_gated_linear_rebwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const void* gh, void* gz, float* gb_part,
-                            int act, void* stream) {
-  const int rc = check_sizes(M, C, F, act);
-  if (rc || M == 0) return rc;
-  VG_REQUIRE(x && w && gh && gz, "gated backward: null tensor");
-  GatedParams p = {};
-  p.x = x;
-  p.w = w;
-  p.bias = bias;
-  p.gh = gh;
-  p.gz = gz;
-  p.gb_part = gb_part;
-  p.M = M;
-  p.C = C;
-  p.F = F;
-  p.act = act;
-  return launch_gated<__bf16, true>(p, (hipStream_t)stream);
-}
-size_t vg_gated_linear_gx_workspace_bytes(int M, int C, int F) {
-  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<float>(M, C, 2 * F);
-}
-size_t vg_gated_linear_gx_workspace_bytes_h(int M, int C, int F) {
-  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<__bf16>(M, C, 2 * F);
-}
-size_t vg_gated_linear_gw_workspace_bytes(int M, int C, int F) {
-  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<float>(2 * F, C, M);
-}
-size_t vg_gated_linear_gw_workspace_bytes_h(int M, int C, int F) {
-  return check_sizes(M, C, F, VG_GATE_SILU) || M == 0 ? 0 : product_bytes<__bf16>(2 * F, C, M);
-}
-int vg_gated_linear_gx(int M, int C, int F, const float* gz, const float* w, float* gx, void* workspace, size_t workspace_bytes,
-                       void* stream) {
-  return gated_gx<float>(M, C, F, gz, w, gx, workspace, workspace_bytes, stream);
-}
-int vg_gated_linear_gx_h(int M, int C, int F, const void* gz, const void* w, void* gx, void* workspace, size_t workspace_bytes,
-                         void* stream) {
-  return gated_gx<__bf16>(M, C, F, gz, w, gx, workspace, workspace_bytes, stream);
-}
-int vg_gated_linear_gw(int M, int C, int F, const float* gz, const float* x, float* gw, void* workspace, size_t workspace_bytes,
-                       void* stream) {
-  return gated_gw<float>(M, C, F, gz, x, gw, 1, workspace, workspace_bytes, stream);
-}
-int vg_gated_linear_gw_h(int M, int C, int F, const void* gz, const void* x, void* gw, int gw_f32, void* workspace, size_t workspace_bytes,
-                         void* stream) {
-  return gated_gw<__bf16>(M, C, F, gz, x, gw, gw_f32, workspace, workspace_bytes, stream);
+int vg_gated_linear_bwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const float* z, const void* gh, void* gx,
+                          void* gw, int gw_f32, float* gb, int act, void* workspace, size_t workspace_bytes, void* stream) {
+  return gated_bwd<__bf16>(M, C, F, x, w, bias, z, gh, gx, gw, gw_f32, gb, act, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -193,19 +193,10 @@ SIGNATURES = {
     "vg_attention_bwd_h": (c_int, [_AG] + [_P] * 12 + [c_size_t, _P]),
     "vg_gated_linear_fwd": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
     "vg_gated_linear_fwd_h": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
-    "vg_gated_linear_bwd": (c_int, [c_int] * 2 + [_P] * 4 + [c_int, _P]),
-    "vg_gated_linear_bwd_h": (c_int, [c_int] * 2 + [_P] * 4 + [c_int, _P]),
-    "vg_gated_linear_partial_rows": (c_int, [c_int] * 3),
-    "vg_gated_linear_recomputes_h": (c_int, [c_int] * 3),
-    "vg_gated_linear_rebwd_h": (c_int, [c_int] * 3 + [_P] * 6 + [c_int, _P]),
-    "vg_gated_linear_gx_workspace_bytes": (c_size_t, [c_int] * 3),
-    "vg_gated_linear_gw_workspace_bytes": (c_size_t, [c_int] * 3),
-    "vg_gated_linear_gx_workspace_bytes_h": (c_size_t, [c_int] * 3),
-    "vg_gated_linear_gw_workspace_bytes_h": (c_size_t, [c_int] * 3),
-    "vg_gated_linear_gx": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
-    "vg_gated_linear_gx_h": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
-    "vg_gated_linear_gw": (c_int, [c_int] * 3 + [_P] * 4 + [c_size_t, _P]),
-    "vg_gated_linear_gw_h": (c_int, [c_int] * 3 + [_P] * 3 + [c_int, _P, c_size_t, _P]),
+    "vg_gated_linear_keeps_z": (c_int, [c_int] * 4),
+    "vg_gated_linear_bwd_workspace_bytes": (c_size_t, [c_int] * 4),
+    "vg_gated_linear_bwd": (c_int, [c_int] * 3 + [_P] * 7 + [c_int, _P, c_int, _P, c_size_t, _P]),
+    "vg_gated_linear_bwd_h": (c_int, [c_int] * 3 + [_P] * 7 + [c_int, _P, c_int, _P, c_size_t, _P]),
 }
 
 _lib = None

@@ -1828,8 +1828,10 @@ def flatten(x):
 # token operators: per-head norm with rotation, attention, gated linear layer
 # ----------------------------------------------------------------------------------------------------------------
 # Their scratch is allocated per call (the caching allocator keeps it to the calling stream, a capture keeps it in its
-# graph's pool), so calls on any streams and graphs replayed side by side share none. Their gradients cannot be
-# differentiated again: the backward pass of a gradient penalty through a critic that contains one raises.
+# graph's pool), so calls on any streams and graphs replayed side by side share none. What depends on shapes, strides and
+# types only - the checks, the geometry handed to the library, scratch sizes - is worked out once per such combination
+# (`_token_plan`); a call then allocates, passes pointers and launches. Their gradients cannot be differentiated again: the
+# backward pass of a gradient penalty through a critic that contains one raises.
 class _FirstOrderFn(Function):
     """A gradient as computed, tied to the tensors it depends on: differentiating it raises (left untied it would
     silently count as a constant)."""
@@ -1844,32 +1846,89 @@ class _FirstOrderFn(Function):
                             "are not implemented: a critic under a gradient penalty cannot contain them")
 
 
+# A gradient that autograd itself accumulates into a leaf goes through that leaf's accumulation node, which belongs to
+# the stream it was made on and lives as long as any graph over the leaf. A backward pass captured into a HIP graph
+# while an eager graph of the same leaf is alive would pull that eager stream into the capture, which ends the
+# process. The nodes are therefore marked when an operator first meets them (`_recorded`), and such a backward pass raises
+# instead. (Inside a training iteration the gradient ledger takes the parameters' gradients and no such node runs.)
+def _recorded(out):
+    """`out` (a tensor, or several of one operator) after its operator was recorded: marks the accumulation nodes of leaves."""
+    for node, _ in (out if torch.is_tensor(out) else out[0]).grad_fn.next_functions:
+        if type(node) is _AccumulateGrad:
+            node.metadata.setdefault("vg_captured", torch.cuda.is_current_stream_capturing())
+    return out
+
+
+def _accumulate_grad_type():
+    leaf = torch.zeros(1, requires_grad=True)
+    with torch.enable_grad():
+        return type(leaf.view_as(leaf).grad_fn.next_functions[0][0])
+
+
+_AccumulateGrad = _accumulate_grad_type()
+
+
 def _first_order(backward):
-    """Backward passes of the token operators: checked against captures (_check_capture), run without recording, results
-    tied to their sources where a graph is being built (create_graph=True)."""
+    """Backward passes of the token operators: refused where a capture would meet an eager graph, run without recording,
+    results tied to their sources where a graph is being built (create_graph=True)."""
 
     @functools.wraps(backward)
     def run(ctx, *gouts):
-        _check_capture(ctx)
+        if torch.cuda.is_current_stream_capturing():
+            for node, _ in ctx.next_functions:
+                if type(node) is _AccumulateGrad and not grads.accepts(node.variable) and not node.metadata.get("vg_captured", True):
+                    raise _hip.HipError("backward pass captured while an eager graph of the same leaf tensor is alive: drop the "
+                                        "eager outputs (and losses) before the capture")
+        if not torch.is_grad_enabled():
+            return backward(ctx, *gouts)
         with torch.no_grad():
             found = backward(ctx, *gouts)
-        if not torch.is_grad_enabled():
-            return found
         sources = [t for t in ctx.saved_tensors + getattr(ctx, "params", ()) + gouts if torch.is_tensor(t) and t.requires_grad]
         return tuple(_FirstOrderFn.apply(g, *sources) if torch.is_tensor(g) and sources else g for g in found)
 
     return run
 
 
+_token_plans = {}
+
+
+def _token_plan(key, make):
+    """What `make()` returns, kept under `key` (a tuple of shapes, strides and types: no tensor, no address)."""
+    plan = _token_plans.get(key)
+    if plan is None:
+        if len(_token_plans) >= 4096:
+            _token_plans.clear()
+        plan = _token_plans[key] = make()
+    return plan
+
+
+def _recording(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _on(t):
     """Context in which calls for `t` are enqueued: its device, when that is not the current one."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return _here if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
-def _scratch(nbytes, device):
-    """(pointer, size) arguments and the buffer behind them, which the caller keeps until its calls are enqueued."""
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    return (ctypes.c_void_p(buf.data_ptr()) if nbytes else None, c_size_t(nbytes)), buf
+_here = contextlib.nullcontext()
+
+
+def _raw_stream(t):
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _scratch(nbytes, like):
+    """Buffer of `nbytes` for one call (None for none)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _at(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _token_tensor(t, what, dims):
@@ -1881,139 +1940,133 @@ def _token_tensor(t, what, dims):
         raise _hip.HipError("%s must be %d-d, got shape %s" % (what, dims, tuple(t.shape)))
 
 
-def _heads_ok(t):
-    """Whether the kernels can read [batch, tokens, heads, width] tensor `t` as it lies: contiguous heads that start on
-    16-byte borders. (What the strides of a dimension of size one are does not matter.)"""
-    vec = 16 // t.element_size()
-    return ((t.shape[3] == 1 or t.stride(3) == 1) and t.data_ptr() % 16 == 0 and
-            all(t.shape[i] <= 1 or t.stride(i) % vec == 0 for i in range(3)))
-
-
-def _heads_in(t, what):
-    _token_tensor(t, what, 4)
-    if t.numel() and not _heads_ok(t):
-        raise _hip.HipError("%s with strides %s: a head's elements must be contiguous and start on a 16-byte border" %
-                            (what, tuple(t.stride())))
-    return t
-
-
-def _heads_grad(g):
-    """A gradient as the kernels read it (autograd may hand back expanded or sliced ones)."""
-    return g if _heads_ok(g) else g.contiguous()
-
-
-def _layout(t):
-    return _hip.HeadsLayout(t.stride(0), t.stride(1), t.stride(2))
-
-
-def _same_kind(first, *others):
+def _same_device(first, *others):
     for t in others:
-        if t is not None and (t.dtype != first.dtype or t.device != first.device):
-            raise _hip.HipError("tensors of one call differ in type or device: %s on %s and %s on %s" %
-                                (first.dtype, first.device, t.dtype, t.device))
+        if t is not None and t.get_device() != first.get_device():
+            raise _hip.HipError("tensors of one call lie on different devices: %s and %s" % (first.device, t.device))
+
+
+def _aligned(*ts):
+    for t in ts:
+        if t.data_ptr() % 16:
+            raise _hip.HipError("a tensor of queries, keys or values does not start on a 16-byte border")
+
+
+def _heads_layout(t, what):
+    """Layout of [batch, tokens, heads, width] tensor `t`, whose heads must be contiguous and start on 16-byte borders (what
+    the stride of a dimension of size one is does not matter)."""
+    vec = 16 // t.element_size()
+    st = t.stride()
+    if t.numel() and ((t.shape[3] != 1 and st[3] != 1) or any(t.shape[i] > 1 and st[i] % vec for i in range(3))):
+        raise _hip.HipError("%s with strides %s: a head's elements must be contiguous and start on a 16-byte border" % (what, st))
+    return _hip.HeadsLayout(*st[:3])
+
+
+def _dense_layout(shape):
+    return _hip.HeadsLayout(shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
 
 
 def _channel_param(t, size, like, what):
     """f32 vector of `size` channel parameters on the device of `like` (None stays None)."""
-    if t is None:
-        return
-    if not t.is_cuda or t.device != like.device or t.dtype != F32 or tuple(t.shape) != (size,) or not t.is_contiguous():
+    if t is not None and (t.get_device() != like.get_device() or t.dtype != F32 or tuple(t.shape) != (size,) or not t.is_contiguous()):
         raise _hip.HipError("%s must be a contiguous float32 vector of %d elements on %s, got %s %s on %s" %
                             (what, size, like.device, t.dtype, tuple(t.shape), t.device))
 
 
-# A gradient that autograd itself accumulates into a leaf goes through that leaf's accumulation node, which belongs to
-# the stream it was made on and lives as long as any graph over the leaf. A backward pass captured into a HIP graph
-# while an eager graph of the same leaf is alive would pull that eager stream into the capture, which ends the
-# process. The nodes are therefore marked when an operator first sees them, and such a backward pass raises instead.
-# (Inside a training iteration the gradient ledger takes the parameters' gradients and no such node runs.)
-def _mark_leaves(ctx, *tensors):
-    ctx.leaf_nodes = []
-    for t in tensors:
-        if t is not None and t.requires_grad and t.is_leaf:
-            node = torch.autograd.graph.get_gradient_edge(t).node
-            node.metadata.setdefault("vg_captured", torch.cuda.is_current_stream_capturing())
-            ctx.leaf_nodes.append((t, node))
-
-
-def _check_capture(ctx):
-    if not ctx.leaf_nodes or not torch.cuda.is_current_stream_capturing():
-        return
-    for t, node in ctx.leaf_nodes:
-        if not grads.accepts(t) and not node.metadata.get("vg_captured", True):
-            raise _hip.HipError("backward pass captured while an eager graph of the same leaf tensor is alive: drop the "
-                                "eager outputs (and losses) before the capture")
-
-
 def _rotary_geom(q, k, pos, axes, base, eps):
-    """Checked geometry of a norm-and-rotate call: q, k [B, T, heads, D] (as they will be read)."""
+    """Checked geometry of a norm-and-rotate call over q, k [batch, tokens, heads, width]; layouts of the inputs filled in."""
     b, t, hq, d = q.shape
+    if q.dtype != k.dtype:
+        raise _hip.HipError("queries are %s and keys %s" % (q.dtype, k.dtype))
     if k.shape[0] != b or k.shape[1] != t or k.shape[3] != d:
         raise _hip.HipError("queries %s and keys %s differ in batch, tokens or head width" % (tuple(q.shape), tuple(k.shape)))
+    if hq < 1:
+        raise _hip.HipError("no query heads in %s" % (tuple(q.shape),))
     if d % 8 or not 8 <= d <= 256:
         raise _hip.HipError("head width %d is not a multiple of 8 from 8 to 256" % d)
-    axes = tuple(int(a) for a in axes)
     if len(axes) > 4 or any(a < 2 or a % 2 for a in axes) or sum(axes) > d:
         raise _hip.HipError("axes %s: at most four even widths whose sum is at most the head width %d" % (axes, d))
-    if not base > 0 or not eps >= 0:
+    if not (0 < base < math.inf) or not (0 <= eps < math.inf):
         raise _hip.HipError("base must be positive and eps not negative, got %s and %s" % (base, eps))
     g = _hip.RotaryGeom(B=b, T=t, Hq=hq, Hk=k.shape[2], D=d, axes=len(axes), eps=eps, base=base)
     for i, a in enumerate(axes):
         g.width[i] = a
     if axes:
-        if pos is None or not pos.is_cuda or pos.device != q.device or pos.dtype not in (torch.int32, torch.int64):
+        if pos is None or pos.dtype not in (torch.int32, torch.int64):
             raise _hip.HipError("positions must be an int32 or int64 tensor on the device of the queries")
         if tuple(pos.shape) not in ((t, len(axes)), (b, t, len(axes))) or not pos.is_contiguous():
             raise _hip.HipError("positions must be contiguous [tokens, axes] or [batch, tokens, axes], got %s for %d tokens, "
                                 "%d axes" % (tuple(pos.shape), t, len(axes)))
         g.pos_wide = int(pos.dtype == torch.int64)
         g.pos_sb = t * len(axes) if pos.dim() == 3 else 0
+    g.q, g.k = _heads_layout(q, "queries"), _heads_layout(k, "keys")
+    g.oq, g.ok = _dense_layout(q.shape), _dense_layout(k.shape)
     return g
 
 
-def _raw_rotary_fwd(g, q, k, wq, wk, pos, yq, yk):
-    g.q, g.k, g.oq, g.ok = _layout(q), _layout(k), _layout(yq), _layout(yk)
-    call(_A("vg_qk_norm_rotary_fwd", q), ctypes.byref(g), _p(q), _p(k), _ptr(wq), _ptr(wk),
-         ctypes.c_void_p(pos.data_ptr()) if pos is not None else None, _p(yq), _p(yk), _stream())
+class _RotaryPlan:
+    """Calls of qk_norm_rotary for one combination of shapes: outputs dense; the gradients' layouts are dense unless given."""
+
+    def __init__(self, q, k, pos, axes, base, eps, grad_layouts=None):
+        lib = _hip.load()
+        self.fwd_geom = _rotary_geom(q, k, pos, axes, base, eps)
+        g = self.bwd_geom = _hip.RotaryGeom.from_buffer_copy(self.fwd_geom)
+        g.gq, g.gk = self.fwd_geom.oq, self.fwd_geom.ok
+        if grad_layouts is not None:
+            g.oq, g.ok = grad_layouts
+        self.fwd_name, self.bwd_name = _A("vg_qk_norm_rotary_fwd", q), _A("vg_qk_norm_rotary_bwd", q)
+        self.fwd, self.bwd = getattr(lib, self.fwd_name), getattr(lib, self.bwd_name)
+        self.scratch = lib.vg_qk_norm_rotary_workspace_bytes(ctypes.byref(self.fwd_geom))
+
+    def forward(self, q, k, wq, wk, pos, yq, yk, stream):
+        """(addresses of q and k, tensors)"""
+        rc = self.fwd(self.fwd_geom, q, k, _at(wq), _at(wk), _at(pos), yq.data_ptr(), yk.data_ptr(), stream)
+        if rc:
+            _hip._check(rc, self.fwd_name)
+
+    def backward(self, q, k, wq, wk, pos, gyq, gyk, gq, gk, want, stream):
+        """(addresses of q, k, gq and gk, tensors.) Returns the gradients of the weights (None: no weight, or not wanted)."""
+        gwq = torch.empty_like(wq) if wq is not None and want[0] else None
+        gwk = torch.empty_like(wk) if wk is not None and want[1] else None
+        space = _scratch(self.scratch, gyq) if gwq is not None or gwk is not None else None
+        rc = self.bwd(self.bwd_geom, q, k, _at(wq), _at(wk), _at(pos), gyq.data_ptr(), gyk.data_ptr(), gq, gk, _at(gwq), _at(gwk),
+                      _at(space), self.scratch if space is not None else 0, stream)
+        if rc:
+            _hip._check(rc, self.bwd_name)
+        return gwq, gwk
 
 
-def _raw_rotary_bwd(g, q, k, wq, wk, pos, gyq, gyk, gq, gk, want_weights):
-    """Writes gq, gk; returns the gradients of the weights (None where there is no weight or none is wanted)."""
-    g.q, g.k, g.gq, g.gk, g.oq, g.ok = (_layout(t) for t in (q, k, gyq, gyk, gq, gk))
-    gwq, gwk = (torch.empty_like(w) if w is not None and want else None for w, want in zip((wq, wk), want_weights))
-    scratch, keep = _scratch(_hip.load().vg_qk_norm_rotary_workspace_bytes(ctypes.byref(g)) if gwq is not None or gwk is not None else 0,
-                             q.device)
-    call(_A("vg_qk_norm_rotary_bwd", q), ctypes.byref(g), _p(q), _p(k), _ptr(wq), _ptr(wk),
-         ctypes.c_void_p(pos.data_ptr()) if pos is not None else None, _p(gyq), _p(gyk), _p(gq), _p(gk), _ptr(gwq), _ptr(gwk),
-         *scratch, _stream())
-    return gwq, gwk
+def _positions_key(pos):
+    return None if pos is None else (pos.shape, pos.stride(), pos.dtype)
 
 
 class QkNormRotaryFn(Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, pos, axes, base, eps):
-        g = _rotary_geom(q, k, pos, axes, base, eps)
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        with _on(q):
-            _raw_rotary_fwd(g, q, k, wq, wk, pos, yq, yk)
-        ctx.g, ctx.label = g, grads.ticket()
-        _mark_leaves(ctx, q, k, wq, wk)
+    def forward(ctx, q, k, wq, wk, pos, plan):
+        ctx.plan, ctx.label = plan, grads.ticket()
         ctx.save_for_backward(q, k, wq, wk, pos)
-        return yq, yk
+        return _rotate(plan, q, k, wq, wk, pos)
 
     @staticmethod
     @_first_order
     def backward(ctx, gyq, gyk):
         q, k, wq, wk, pos = ctx.saved_tensors
         lab, need = ctx.label, ctx.needs_input_grad
-        gyq, gyk = _heads_grad(gyq), _heads_grad(gyk)
+        gyq, gyk = gyq.contiguous(), gyk.contiguous()
         gq, gk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
         params = not inputs_only.active
         with _on(q):
-            gwq, gwk = _raw_rotary_bwd(ctx.g, q, k, wq, wk, pos, gyq, gyk, gq, gk, (params and need[2], params and need[3]))
+            gwq, gwk = ctx.plan.backward(q.data_ptr(), k.data_ptr(), wq, wk, pos, gyq, gyk, gq.data_ptr(), gk.data_ptr(),
+                                         (params and need[2], params and need[3]), _raw_stream(q))
         return (gq if need[0] else None, gk if need[1] else None, grads.route(wq, lab + (0,), gwq) if wq is not None else None,
-                grads.route(wk, lab + (1,), gwk) if wk is not None else None, None, None, None, None)
+                grads.route(wk, lab + (1,), gwk) if wk is not None else None, None, None)
+
+
+def _rotate(plan, q, k, wq, wk, pos):
+    yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    with _on(q):
+        plan.forward(q.data_ptr(), k.data_ptr(), wq, wk, pos, yq, yk, _raw_stream(q))
+    return yq, yk
 
 
 def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, axes=(), base=10000.0, eps=1e-6):
@@ -2024,16 +2077,27 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, axes=(), 
     positions [tokens, len(axes)] or [batch, tokens, len(axes)] (int32 / int64): a token's place on every axis (row and
     column of a feature map, frame of a clip). axes: how many elements of a head belong to each axis, in order; pair
     (2i, 2i+1) of a section of width d turns by position * base^(-2i / d); elements behind the sections are not turned."""
-    _heads_in(q, "queries")
-    _heads_in(k, "keys")
-    _same_kind(q, k)
-    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _channel_param(w, q.shape[3], q, what)
-    return QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, tuple(axes), float(base), float(eps))
+    _token_tensor(q, "queries", 4)
+    _token_tensor(k, "keys", 4)
+    axes, base, eps = tuple(axes), float(base), float(eps)
+    plan = _token_plan(("rotary", q.shape, q.stride(), k.shape, k.stride(), q.dtype, k.dtype, _positions_key(positions), axes, base, eps),
+                       lambda: _RotaryPlan(q, k, positions, axes, base, eps))
+    _aligned(q, k)
+    _same_device(q, k, positions)
+    _channel_param(q_weight, q.shape[3], q, "q_weight")
+    _channel_param(k_weight, q.shape[3], q, "k_weight")
+    if not axes:
+        positions = None
+    if not _recording(q, k, q_weight, k_weight):
+        return _rotate(plan, q, k, q_weight, k_weight, positions)
+    return _recorded(QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, plan))
 
 
-def _attention_geom(q, k, v, q_lengths, k_lengths, scale):
+def _attention_geom(q, k, v, scale):
+    """Checked geometry of an attention call; layouts of the inputs filled in, all others dense."""
     b, tq, hq, d = q.shape
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise _hip.HipError("queries are %s, keys %s and values %s" % (q.dtype, k.dtype, v.dtype))
     if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
         raise _hip.HipError("queries %s, keys %s and values %s do not belong together" %
                             (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
@@ -2041,48 +2105,60 @@ def _attention_geom(q, k, v, q_lengths, k_lengths, scale):
         raise _hip.HipError("%d query heads are not a multiple of %d key heads" % (hq, k.shape[2]))
     if d % 8 or not 8 <= d <= 128:
         raise _hip.HipError("head width %d is not a multiple of 8 from 8 to 128" % d)
-    for n, what in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths")):
-        if n is not None and (not n.is_cuda or n.device != q.device or n.dtype != torch.int32 or tuple(n.shape) != (b,) or
-                              not n.is_contiguous()):
-            raise _hip.HipError("%s must be a contiguous int32 tensor [%d] on the device of the queries" % (what, b))
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or ctypes.c_float(scale).value == 0.0:
+    scale = d ** -0.5 if scale is None else scale
+    if not math.isfinite(scale) or not math.isfinite(c_float(scale).value) or c_float(scale).value == 0.0:
         raise _hip.HipError("scale must be finite and not zero, got %s" % scale)
-    return _hip.AttentionGeom(B=b, Tq=tq, Tk=k.shape[1], Hq=hq, Hk=k.shape[2], D=d, scale=scale)
+    g = _hip.AttentionGeom(B=b, Tq=tq, Tk=k.shape[1], Hq=hq, Hk=k.shape[2], D=d, scale=scale)
+    g.q, g.k, g.v = _heads_layout(q, "queries"), _heads_layout(k, "keys"), _heads_layout(v, "values")
+    g.o = g.go = g.gq = _dense_layout(q.shape)
+    g.gk = g.gv = _dense_layout(k.shape)
+    return g
 
 
-def _lengths_ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+class _AttentionPlan:
+    """Calls of attention for one combination of shapes."""
+
+    def __init__(self, q, k, v, scale, gv_layout=None):
+        lib = _hip.load()
+        g = self.geom = _attention_geom(q, k, v, scale)
+        if gv_layout is not None:
+            g.gv = gv_layout
+        self.fwd_name, self.bwd_name = _A("vg_attention_fwd", q), _A("vg_attention_bwd", q)
+        self.fwd, self.bwd = getattr(lib, self.fwd_name), getattr(lib, self.bwd_name)
+        self.fwd_scratch, self.bwd_scratch = (lib.vg_attention_workspace_bytes(ctypes.byref(g), i) for i in (0, 1))
+        self.lse_shape = (g.B, g.Hk, g.Tq * (g.Hq // g.Hk))
+
+    def forward(self, q, k, v, q_lengths, k_lengths, o, save, stream):
+        """(q, k, v: addresses.) Writes o; returns the row sums' logarithms when `save`."""
+        lse = torch.empty(self.lse_shape, dtype=F32, device=o.device) if save else None
+        space = _scratch(self.fwd_scratch, o)
+        rc = self.fwd(self.geom, q, k, v, _at(q_lengths), _at(k_lengths), o.data_ptr(), _at(lse), _at(space), self.fwd_scratch, stream)
+        if rc:
+            _hip._check(rc, self.fwd_name)
+        return lse
+
+    def backward(self, q, k, v, o, lse, go, q_lengths, k_lengths, gq, gk, gv, stream):
+        """(q, k, v, gq, gk, gv: addresses.)"""
+        space = _scratch(self.bwd_scratch, o)
+        rc = self.bwd(self.geom, q, k, v, o.data_ptr(), lse.data_ptr(), go.data_ptr(), _at(q_lengths), _at(k_lengths), gq, gk, gv,
+                      _at(space), self.bwd_scratch, stream)
+        if rc:
+            _hip._check(rc, self.bwd_name)
 
 
-def _raw_attention_fwd(g, q, k, v, q_lengths, k_lengths, o, save):
-    """Writes o; returns the row sums' logarithms when `save`."""
-    g.q, g.k, g.v, g.o = (_layout(t) for t in (q, k, v, o))
-    lse = torch.empty((g.B, g.Hk, g.Tq * (g.Hq // g.Hk)), dtype=F32, device=q.device) if save else None
-    scratch, keep = _scratch(_hip.load().vg_attention_workspace_bytes(ctypes.byref(g), 0), q.device)
-    call(_A("vg_attention_fwd", q), ctypes.byref(g), _p(q), _p(k), _p(v), _lengths_ptr(q_lengths), _lengths_ptr(k_lengths), _p(o),
-         _ptr(lse), *scratch, _stream())
-    return lse
-
-
-def _raw_attention_bwd(g, q, k, v, o, lse, go, q_lengths, k_lengths, gq, gk, gv):
-    g.q, g.k, g.v, g.o, g.go = (_layout(t) for t in (q, k, v, o, go))
-    none = _hip.HeadsLayout(0, 0, 0)
-    g.gq, g.gk, g.gv = (_layout(t) if t is not None else none for t in (gq, gk, gv))
-    scratch, keep = _scratch(_hip.load().vg_attention_workspace_bytes(ctypes.byref(g), 1), q.device)
-    call(_A("vg_attention_bwd", q), ctypes.byref(g), _p(q), _p(k), _p(v), _p(o), _ptr(lse), _p(go), _lengths_ptr(q_lengths),
-         _lengths_ptr(k_lengths), _p(gq), _p(gk), _p(gv), *scratch, _stream())
+def _check_lengths(n, q, what):
+    if n is not None and (n.get_device() != q.get_device() or n.dtype != torch.int32 or tuple(n.shape) != (q.shape[0],) or
+                          not n.is_contiguous()):
+        raise _hip.HipError("%s must be a contiguous int32 tensor [%d] on the device of the queries" % (what, q.shape[0]))
 
 
 class AttentionFn(Function):
     @staticmethod
-    def forward(ctx, q, k, v, q_lengths, k_lengths, scale):
-        g = _attention_geom(q, k, v, q_lengths, k_lengths, scale)
+    def forward(ctx, q, k, v, q_lengths, k_lengths, plan):
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         with _on(q):
-            lse = _raw_attention_fwd(g, q, k, v, q_lengths, k_lengths, o, any(ctx.needs_input_grad))
-        ctx.g = g
-        _mark_leaves(ctx, q, k, v)
+            lse = plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, True, _raw_stream(q))
+        ctx.plan = plan
         ctx.save_for_backward(q, k, v, o, lse, q_lengths, k_lengths)
         return o
 
@@ -2091,11 +2167,14 @@ class AttentionFn(Function):
     def backward(ctx, go):
         q, k, v, o, lse, q_lengths, k_lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        gq = new(q) if need[0] else None
-        gk, gv = (new(k), new(v)) if need[1] or need[2] else (None, None)
+        go = go.contiguous()
+        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need[0] else None
+        gk = gv = None
+        if need[1] or need[2]:
+            gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
         with _on(q):
-            _raw_attention_bwd(ctx.g, q, k, v, o, lse, _heads_grad(go), q_lengths, k_lengths, gq, gk, gv)
+            ctx.plan.backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), o, lse, go, q_lengths, k_lengths, _at(gq), _at(gk), _at(gv),
+                              _raw_stream(q))
         return gq, gk if need[1] else None, gv if need[2] else None, None, None, None
 
 
@@ -2106,29 +2185,57 @@ def attention(q, k, v, q_lengths=None, k_lengths=None, scale=None):
     q_lengths / k_lengths (int32 [batch], on the GPU): how many queries / keys of each batch element take part. What
     lies behind them is never used (it may be NaN); rows behind q_lengths and rows without a key are zero, and so are the
     gradients of what takes no part."""
-    _heads_in(q, "queries")
-    _heads_in(k, "keys")
-    _heads_in(v, "values")
-    _same_kind(q, k, v)
-    return AttentionFn.apply(q, k, v, q_lengths, k_lengths, scale)
+    _token_tensor(q, "queries", 4)
+    _token_tensor(k, "keys", 4)
+    _token_tensor(v, "values", 4)
+    scale = None if scale is None else float(scale)
+    plan = _token_plan(("attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, scale),
+                       lambda: _AttentionPlan(q, k, v, scale))
+    _aligned(q, k, v)
+    _same_device(q, k, v)
+    _check_lengths(q_lengths, q, "q_lengths")
+    _check_lengths(k_lengths, q, "k_lengths")
+    if not _recording(q, k, v):
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        with _on(q):
+            plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, False, _raw_stream(q))
+        return o
+    return _recorded(AttentionFn.apply(q, k, v, q_lengths, k_lengths, plan))
 
 
-class SelfAttentionFn(Function):
+class _SelfAttentionPlan:
     """Norm, rotation and attention over one packed projection: the values are read where they lie and the gradients of
     queries, keys and values are written into one packed gradient."""
 
-    @staticmethod
-    def forward(ctx, qkv, wq, wk, pos, heads, kv_heads, axes, lengths, base, eps, scale):
+    def __init__(self, qkv, heads, kv_heads, pos, axes, base, eps, scale):
         q, k, v = qkv.split((heads, kv_heads, kv_heads), 2)
-        rg = _rotary_geom(q, k, pos, axes, base, eps)
-        ag = _attention_geom(q, k, v, lengths, lengths, scale)
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        yq, yk, o = new(q), new(k), new(q)
+        b, t, _, d = qkv.shape
+        packed = _dense_layout(qkv.shape)
+        self.rotary = _RotaryPlan(q, k, pos, axes, base, eps, (packed, packed))
+        dense = lambda h: torch.empty(b, t, h, d, dtype=qkv.dtype, device="meta")  # noqa: E731  (its layout is all that is read)
+        self.attention = _AttentionPlan(dense(heads), dense(kv_heads), v, scale, packed)
+        self.heads, self.kv_heads = heads, kv_heads
+        self.q_shape, self.k_shape = tuple(q.shape), tuple(k.shape)
+        size = qkv.element_size()
+        self.k_at, self.v_at = (h * qkv.stride(2) * size for h in (heads, heads + kv_heads))             # bytes from the queries
+        self.gk_at, self.gv_at = (h * d * size for h in (heads, heads + kv_heads))
+
+    def forward(self, qkv, wq, wk, pos, lengths, save):
+        new = lambda shape: torch.empty(shape, dtype=qkv.dtype, device=qkv.device)  # noqa: E731
+        yq, yk, o = new(self.q_shape), new(self.k_shape), new(self.q_shape)
+        at = qkv.data_ptr()
         with _on(qkv):
-            _raw_rotary_fwd(rg, q, k, wq, wk, pos, yq, yk)
-            lse = _raw_attention_fwd(ag, yq, yk, v, lengths, lengths, o, any(ctx.needs_input_grad))
-        ctx.rg, ctx.ag, ctx.label, ctx.split = rg, ag, grads.ticket(), (heads, kv_heads, kv_heads)
-        _mark_leaves(ctx, qkv, wq, wk)
+            stream = _raw_stream(qkv)
+            self.rotary.forward(at, at + self.k_at, wq, wk, pos, yq, yk, stream)
+            lse = self.attention.forward(yq.data_ptr(), yk.data_ptr(), at + self.v_at, lengths, lengths, o, save, stream)
+        return yq, yk, o, lse
+
+
+class SelfAttentionFn(Function):
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, pos, lengths, plan):
+        yq, yk, o, lse = plan.forward(qkv, wq, wk, pos, lengths, True)
+        ctx.plan, ctx.label = plan, grads.ticket()
         ctx.save_for_backward(qkv, wq, wk, pos, yq, yk, o, lse, lengths)
         return o
 
@@ -2136,17 +2243,20 @@ class SelfAttentionFn(Function):
     @_first_order
     def backward(ctx, go):
         qkv, wq, wk, pos, yq, yk, o, lse, lengths = ctx.saved_tensors
-        lab, need = ctx.label, ctx.needs_input_grad
-        q, k, v = qkv.split(ctx.split, 2)
+        plan, lab, need = ctx.plan, ctx.label, ctx.needs_input_grad
+        go = go.contiguous()
         gqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        gq, gk, gv = gqkv.split(ctx.split, 2)
         gyq, gyk = torch.empty_like(yq), torch.empty_like(yk)
         params = not inputs_only.active
+        at, gat = qkv.data_ptr(), gqkv.data_ptr()
         with _on(qkv):
-            _raw_attention_bwd(ctx.ag, yq, yk, v, o, lse, _heads_grad(go), lengths, lengths, gyq, gyk, gv)
-            gwq, gwk = _raw_rotary_bwd(ctx.rg, q, k, wq, wk, pos, gyq, gyk, gq, gk, (params and need[1], params and need[2]))
+            stream = _raw_stream(qkv)
+            plan.attention.backward(yq.data_ptr(), yk.data_ptr(), at + plan.v_at, o, lse, go, lengths, lengths, gyq.data_ptr(),
+                                    gyk.data_ptr(), gat + plan.gv_at, stream)
+            gwq, gwk = plan.rotary.backward(at, at + plan.k_at, wq, wk, pos, gyq, gyk, gat, gat + plan.gk_at,
+                                            (params and need[1], params and need[2]), stream)
         return (gqkv if need[0] else None, grads.route(wq, lab + (0,), gwq) if wq is not None else None,
-                grads.route(wk, lab + (1,), gwk) if wk is not None else None) + (None,) * 8
+                grads.route(wk, lab + (1,), gwk) if wk is not None else None, None, None, None)
 
 
 def self_attention(qkv, heads, kv_heads=None, q_weight=None, k_weight=None, positions=None, axes=(), lengths=None, base=10000.0,
@@ -2154,33 +2264,64 @@ def self_attention(qkv, heads, kv_heads=None, q_weight=None, k_weight=None, posi
     """`qk_norm_rotary` and `attention` of the tokens of each batch element among themselves. qkv [batch, tokens,
     heads + 2 * kv_heads, width]: queries, keys and values as one projection leaves them. lengths (int32 [batch]): tokens
     of each batch element. Returns [batch, tokens, heads, width]."""
+    _token_tensor(qkv, "packed queries, keys and values", 4)
     kv_heads = heads if kv_heads is None else kv_heads
-    _heads_in(qkv, "packed queries, keys and values")
     if heads < 1 or kv_heads < 1 or qkv.shape[2] != heads + 2 * kv_heads:
         raise _hip.HipError("packed tensor has %d heads, expected %d + 2 * %d" % (qkv.shape[2], heads, kv_heads))
-    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _channel_param(w, qkv.shape[3], qkv, what)
-    return SelfAttentionFn.apply(qkv, q_weight, k_weight, positions, heads, kv_heads, tuple(axes), lengths, float(base), float(eps),
-                                 scale)
+    axes, base, eps = tuple(axes), float(base), float(eps)
+    scale = None if scale is None else float(scale)
+    plan = _token_plan(("self", qkv.shape, qkv.stride(), qkv.dtype, heads, kv_heads, _positions_key(positions), axes, base, eps, scale),
+                       lambda: _SelfAttentionPlan(qkv, heads, kv_heads, positions, axes, base, eps, scale))
+    _aligned(qkv)
+    _same_device(qkv, positions)
+    _check_lengths(lengths, qkv, "lengths")
+    _channel_param(q_weight, qkv.shape[3], qkv, "q_weight")
+    _channel_param(k_weight, qkv.shape[3], qkv, "k_weight")
+    if not axes:
+        positions = None
+    if not _recording(qkv, q_weight, k_weight):
+        return plan.forward(qkv, q_weight, k_weight, positions, lengths, False)[2]
+    return _recorded(SelfAttentionFn.apply(qkv, q_weight, k_weight, positions, lengths, plan))
+
+
+class _GatedPlan:
+    """Calls of gated_linear for one combination of sizes."""
+
+    def __init__(self, m, c, f, dtype):
+        lib = _hip.load()
+        half = dtype == BF16
+        self.m, self.c, self.f = m, c, f
+        self.fwd_name, self.bwd_name = ("vg_gated_linear_fwd_h", "vg_gated_linear_bwd_h") if half else ("vg_gated_linear_fwd", "vg_gated_linear_bwd")
+        self.fwd, self.bwd = getattr(lib, self.fwd_name), getattr(lib, self.bwd_name)
+        self.keeps_z = bool(lib.vg_gated_linear_keeps_z(m, c, f, int(half)))
+        self.scratch = lib.vg_gated_linear_bwd_workspace_bytes(m, c, f, int(half))
+
+    def forward(self, x, w, bias, act, save):
+        """Returns the output and, when `save` and the backward pass wants them, the pre-activations."""
+        h = torch.empty((self.m, self.f), dtype=x.dtype, device=x.device)
+        z = torch.empty((self.m, 2 * self.f), dtype=F32, device=x.device) if save and self.keeps_z else None
+        with _on(x):
+            rc = self.fwd(self.m, self.c, self.f, x.data_ptr(), w.data_ptr(), _at(bias), h.data_ptr(), _at(z), act, _raw_stream(x))
+            if rc:
+                _hip._check(rc, self.fwd_name)
+        return h, z
+
+
+def _gated_operands(x, w):
+    """x and w as the kernels read them: dense, the weight of a bf16 input in bf16."""
+    with _on(x):
+        x = x if x.is_contiguous() else _plain_contiguous(x)
+        w = w if w.is_contiguous() else _plain_contiguous(w)
+        return x, w if w.dtype == x.dtype else plane_cache.bf16_copy(w).view(w.shape)
 
 
 class GatedLinearFn(Function):
     @staticmethod
-    def forward(ctx, x, w, bias, act):
-        lib = _hip.load()
-        xm, wm = to_nhwc(x), _weight_mem(w)
-        m, c, f = xm.shape[0], xm.shape[1], wm.shape[0] // 2
-        with _on(x):
-            if wm.dtype != xm.dtype:        # f32 master of a bf16 layer
-                wm = plane_cache.bf16_copy(wm).view(wm.shape)
-            h = torch.empty((m, f), dtype=xm.dtype, device=xm.device)
-            training = any(ctx.needs_input_grad)
-            again = xm.dtype == BF16 and bool(lib.vg_gated_linear_recomputes_h(m, c, f))
-            z = torch.empty((m, 2 * f), dtype=F32, device=xm.device) if training and not again else None
-            call(_A("vg_gated_linear_fwd", xm), m, c, f, _p(xm), _p(wm), _ptr(bias), _p(h), _ptr(z), act, _stream())
-        ctx.act, ctx.label = act, grads.ticket()
-        _mark_leaves(ctx, x, w, bias)
-        # (wm: what the forward product read; a bf16 copy made here is the one the backward products read)
+    def forward(ctx, x, w, bias, act, plan):
+        xm, wm = _gated_operands(x, w)
+        h, z = plan.forward(xm, wm, bias, act, True)
+        ctx.plan, ctx.act, ctx.label = plan, act, grads.ticket()
+        # (wm: what the forward product read; a bf16 copy of a master is the one the backward products read)
         ctx.save_for_backward(xm, wm, bias, z)
         ctx.params = (w, bias, x)
         return h
@@ -2188,42 +2329,23 @@ class GatedLinearFn(Function):
     @staticmethod
     @_first_order
     def backward(ctx, gh):
-        lib = _hip.load()
         xm, wm, bias, z = ctx.saved_tensors
-        w, bias_in, _ = ctx.params
-        lab, need, act = ctx.label, ctx.needs_input_grad, ctx.act
-        m, c, f = xm.shape[0], xm.shape[1], wm.shape[0] // 2
-        gh = _cast_raw(gh if gh.is_contiguous() else gh.contiguous(), xm.dtype)
+        w, bias_in, x = ctx.params
+        plan, lab, need = ctx.plan, ctx.label, ctx.needs_input_grad
+        gh = _cast_raw(gh.contiguous(), xm.dtype)
         params = not inputs_only.active
-        gx = gw = gb = None
-        with _on(xm):
-            gz = torch.empty((m, 2 * f), dtype=xm.dtype, device=xm.device)
-            want_gb = params and bias is not None and need[2]
-            rows = lib.vg_gated_linear_partial_rows(m, f, int(z is None))
-            part = torch.empty((rows, 2 * f), dtype=F32, device=xm.device) if want_gb else None
-            if z is None:
-                call("vg_gated_linear_rebwd_h", m, c, f, _p(xm), _p(wm), _ptr(bias), _p(gh), _p(gz), _ptr(part), act, _stream())
-            else:
-                call(_A("vg_gated_linear_bwd", xm), m, f, _ptr(z), _p(gh), _p(gz), _ptr(part), act, _stream())
-            if want_gb:
-                gb = torch.empty(2 * f, dtype=F32, device=xm.device)
-                if rows:
-                    scratch, keep = _scratch(lib.vg_colsum_workspace_bytes(rows, 2 * f), xm.device)
-                    call("vg_colsum", _ptr(part), _ptr(gb), rows, 2 * f, *scratch, _stream())
-                else:
-                    call("vg_fill", _ptr(gb), c_float(0.0), c_size_t(2 * f), _stream())
-            if _wants_input_grad(ctx, xm):
-                gx = torch.empty((m, c), dtype=xm.dtype, device=xm.device)
-                scratch, keep = _scratch(getattr(lib, _A("vg_gated_linear_gx_workspace_bytes", xm))(m, c, f), xm.device)
-                call(_A("vg_gated_linear_gx", xm), m, c, f, _p(gz), _p(wm), _p(gx), *scratch, _stream())
-            if params and need[1]:
-                gw = torch.empty((2 * f, c), dtype=w.dtype, device=xm.device)
-                scratch, keep = _scratch(getattr(lib, _A("vg_gated_linear_gw_workspace_bytes", xm))(m, c, f), xm.device)
-                if xm.dtype == BF16:
-                    call("vg_gated_linear_gw_h", m, c, f, _p(gz), _p(xm), _p(gw), int(gw.dtype == F32), *scratch, _stream())
-                else:
-                    call("vg_gated_linear_gw", m, c, f, _p(gz), _p(xm), _p(gw), *scratch, _stream())
-        return gx, grads.route(w, lab, gw), grads.route(bias_in, lab, gb) if bias_in is not None else None, None
+        dev = xm.device
+        gx = torch.empty((plan.m, plan.c), dtype=xm.dtype, device=dev) if _wants_input_grad(ctx, x) else None
+        gw = torch.empty((2 * plan.f, plan.c), dtype=w.dtype, device=dev) if params and need[1] else None
+        gb = torch.empty(2 * plan.f, dtype=F32, device=dev) if params and bias is not None and need[2] else None
+        if gx is not None or gw is not None or gb is not None:
+            with _on(xm):
+                space = _scratch(plan.scratch, xm)
+                rc = plan.bwd(plan.m, plan.c, plan.f, xm.data_ptr(), wm.data_ptr(), _at(bias), _at(z), gh.data_ptr(), _at(gx), _at(gw),
+                              int(gw is not None and gw.dtype == F32), _at(gb), ctx.act, _at(space), plan.scratch, _raw_stream(xm))
+                if rc:
+                    _hip._check(rc, plan.bwd_name)
+        return (gx, grads.route(w, lab, gw), grads.route(bias_in, lab, gb) if bias_in is not None else None, None, None)
 
 
 def gated_linear(x, w, bias=None, act="silu"):
@@ -2235,9 +2357,14 @@ def gated_linear(x, w, bias=None, act="silu"):
     _token_tensor(w, "weight", 2)
     if w.shape[0] < 2 or w.shape[0] % 2 or w.shape[1] != x.shape[1] or not x.shape[1]:
         raise _hip.HipError("gated linear layer: input %s and weight %s do not belong together" % (tuple(x.shape), tuple(w.shape)))
-    if w.device != x.device or (w.dtype != x.dtype and w.dtype != F32):
+    if w.get_device() != x.get_device() or (w.dtype != x.dtype and w.dtype != F32):
         raise _hip.HipError("gated linear layer: %s weight on %s with %s input on %s" % (w.dtype, w.device, x.dtype, x.device))
     _channel_param(bias, w.shape[0], x, "bias")
-    if act not in _hip.GATES:
+    code = _hip.GATES.get(act)
+    if code is None:
         raise _hip.HipError("gate activation %r: expected one of %s" % (act, sorted(_hip.GATES)))
-    return GatedLinearFn.apply(x, w, bias, _hip.GATES[act])
+    m, c, f, dtype = x.shape[0], x.shape[1], w.shape[0] // 2, x.dtype
+    plan = _token_plan(("gated", m, c, f, dtype), lambda: _GatedPlan(m, c, f, dtype))
+    if not _recording(x, w, bias):
+        return plan.forward(*_gated_operands(x, w), bias, code, False)[0]
+    return _recorded(GatedLinearFn.apply(x, w, bias, code, plan))

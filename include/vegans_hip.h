@@ -520,35 +520,21 @@ int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k,
                        size_t workspace_bytes, void* stream);
 
 /* Gated linear layer h[M][F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M][C], w [2F][C] (gate rows first), bias [2F] nullable.
- *   vg_gated_linear_fwd       z [M][2F] f32 (pre-activations, for the backward pass) nullable
- *   vg_gated_linear_bwd       gz [M][2F] = gradient of the pre-activations from z and gh
- *   vg_gated_linear_rebwd_h   the same from x and w (what vg_gated_linear_recomputes_h prefers to a stored z)
- *   vg_gated_linear_gx / _gw  gx = gz w, gw = gz^T x (_h: f32 where gw_f32, else bf16); scratch: *_workspace_bytes
- * gb_part [vg_gated_linear_partial_rows(M, F, recompute)][2F] f32, nullable: its column sums are the bias gradient. */
+ * fwd: z [M][2F] f32 nullable: the pre-activations, which the backward pass of the sizes that vg_gated_linear_keeps_z names
+ * needs (the others compute them again). bwd: gx [M][C], gw [2F][C] (f32 where gw_f32, else bf16), gb [2F] f32, each
+ * nullable. */
 #define VG_GATE_SIGMOID 0
 #define VG_GATE_RELU 1
 #define VG_GATE_GELU 2
 #define VG_GATE_SILU 3
 int vg_gated_linear_fwd(int M, int C, int F, const float* x, const float* w, const float* bias, float* h, float* z, int act, void* stream);
 int vg_gated_linear_fwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, void* h, float* z, int act, void* stream);
-int vg_gated_linear_bwd(int M, int F, const float* z, const float* gh, float* gz, float* gb_part, int act, void* stream);
-int vg_gated_linear_bwd_h(int M, int F, const float* z, const void* gh, void* gz, float* gb_part, int act, void* stream);
-int vg_gated_linear_partial_rows(int M, int F, int recompute);
-int vg_gated_linear_recomputes_h(int M, int C, int F);
-int vg_gated_linear_rebwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const void* gh, void* gz, float* gb_part,
-                            int act, void* stream);
-size_t vg_gated_linear_gx_workspace_bytes(int M, int C, int F);
-size_t vg_gated_linear_gw_workspace_bytes(int M, int C, int F);
-size_t vg_gated_linear_gx_workspace_bytes_h(int M, int C, int F);
-size_t vg_gated_linear_gw_workspace_bytes_h(int M, int C, int F);
-int vg_gated_linear_gx(int M, int C, int F, const float* gz, const float* w, float* gx, void* workspace, size_t workspace_bytes,
-                       void* stream);
-int vg_gated_linear_gw(int M, int C, int F, const float* gz, const float* x, float* gw, void* workspace, size_t workspace_bytes,
-                       void* stream);
-int vg_gated_linear_gx_h(int M, int C, int F, const void* gz, const void* w, void* gx, void* workspace, size_t workspace_bytes,
-                         void* stream);
-int vg_gated_linear_gw_h(int M, int C, int F, const void* gz, const void* x, void* gw, int gw_f32, void* workspace, size_t workspace_bytes,
-                         void* stream);
+int vg_gated_linear_keeps_z(int M, int C, int F, int half);
+size_t vg_gated_linear_bwd_workspace_bytes(int M, int C, int F, int half);
+int vg_gated_linear_bwd(int M, int C, int F, const float* x, const float* w, const float* bias, const float* z, const float* gh, float* gx,
+                        float* gw, int gw_f32, float* gb, int act, void* workspace, size_t workspace_bytes, void* stream);
+int vg_gated_linear_bwd_h(int M, int C, int F, const void* x, const void* w, const float* bias, const float* z, const void* gh, void* gx,
+                          void* gw, int gw_f32, float* gb, int act, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

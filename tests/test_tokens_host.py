@@ -101,10 +101,16 @@ def test_gated_arguments_are_checked_before_any_launch():
     assert lib.vg_gated_linear_fwd(4, 0, 8, DUMMY, DUMMY, None, DUMMY, None, 3, None) == -1 and "bad sizes" in _text(lib)
     assert lib.vg_gated_linear_fwd(1 << 30, 8, 8, DUMMY, DUMMY, None, DUMMY, None, 3, None) == -1 and "too many" in _text(lib)
     assert lib.vg_gated_linear_fwd(0, 8, 8, None, None, None, None, None, 3, None) == 0
-    need = lib.vg_gated_linear_gw_workspace_bytes(4096, 64, 32)
-    assert need > 0 and need % (64 * 64 * 4) == 0
-    assert lib.vg_gated_linear_gw(4096, 64, 32, DUMMY, DUMMY, DUMMY, DUMMY, need - 1, None) == -3
-    assert lib.vg_gated_linear_gx(4096, 64, 32, None, DUMMY, DUMMY, None, 0, None) == -1
+    need = lib.vg_gated_linear_bwd_workspace_bytes(4096, 64, 32, 0)
+    assert need >= 4096 * 64 * 4                        # at least the pre-activations' gradient
+    assert lib.vg_gated_linear_bwd(4096, 64, 32, *[DUMMY] * 7, 1, None, 3, DUMMY, need - 1, None) == -3
+    assert lib.vg_gated_linear_bwd(4096, 64, 32, DUMMY, DUMMY, None, None, DUMMY, DUMMY, DUMMY, 1, None, 3, DUMMY, need, None) == -1
+    assert "pre-activations" in _text(lib)
+    assert lib.vg_gated_linear_bwd(4096, 64, 32, None, *[DUMMY] * 6, 1, None, 3, DUMMY, need, None) == -1 and "null" in _text(lib)
+    assert lib.vg_gated_linear_bwd(4096, 64, 32, *[DUMMY] * 7, 0, None, 3, DUMMY, need, None) == -1 and "f32" in _text(lib)
+    # f32 keeps its pre-activations; bf16 where computing them again would cost more
+    assert lib.vg_gated_linear_keeps_z(4096, 64, 32, 0) and not lib.vg_gated_linear_keeps_z(4096, 64, 32, 1)
+    assert lib.vg_gated_linear_keeps_z(4096, 2048, 32, 1) and lib.vg_gated_linear_keeps_z(8, 64, 32, 1)
 
 
 def test_operators_refuse_cpu_tensors():

@@ -31,12 +31,17 @@ struct AttnParams {
   vg_attention_geom g;
   const void *q, *k, *v, *o, *go;
   void *out, *gq, *gk, *gv;
+  __bf16* low;               // bf16: what the rounding of o left, dense (written forward, read for delta); null: not wanted
   const float *lse_in, *delta;
   float* lse;
   const int *q_len, *k_len;
-  float* part;               // split launches: f32 partial results
+  float* part;               // split walks over keys: f32 partial rows
   float* part_ml;            // forward: running maximum and sum of every row and split
-  int G, R, splits, chunk;   // chunk: keys (forward, queries' gradient) or rows (keys' gradient) of a split
+  float* part_kv;            // split walks over rows: f32 partial gradients of keys, then of values
+  int G, R;
+  int splits, chunk;         // walks over keys (forward, queries' gradient): how many, keys of each
+  int r_splits, r_chunk;     // walks over rows (keys' gradient)
+  int gkv_blocks;            // backward: blocks of the keys' gradient, ahead of those of the queries'
   unsigned g_magic;          // ceil(2^32 / G)
   int row_tiles, key_tiles;
   float cs;                  // scale * log2(e)
@@ -146,8 +151,9 @@ __device__ __forceinline__ f32x16 mul_tiles(const __bf16* tile, const __bf16* co
   return acc;
 }
 
-// acc[j] (rows d = 32 j + row) += sum over the 32 rows k0.. of a TR tile of tile[k][d] * w[k][column], w as a product left it
-template <int DP>
+// acc[j] (rows d = 32 j + row) += sum over the 32 rows k0.. of a TR tile of tile[k][d] * w[k][column], w as a product left it.
+// bf16: w (probabilities, ds) is rounded to bf16 for this; FINE: taken as two bf16 terms, i.e. to 2^-17.
+template <int DP, bool FINE>
 __device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
   using L = Tile<__bf16, DP, true>;
   const int h = lane >> 5, q = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -155,19 +161,27 @@ __device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, in
   const __bf16 *a = tile + (k0 + 4 * h + q) * L::LD + (col ^ (8 * h)), *b = tile + (k0 + 8 + 4 * h + q) * L::LD + (col ^ (8 * (2 + h)));
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const u32x4 pk = {tok_pack2(w[8 * s], w[8 * s + 1]), tok_pack2(w[8 * s + 2], w[8 * s + 3]), tok_pack2(w[8 * s + 4], w[8 * s + 5]),
-                      tok_pack2(w[8 * s + 6], w[8 * s + 7])};
-    const bf16x8 x = __builtin_bit_cast(bf16x8, pk);
+    float left[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) left[i] = w[8 * s + i];
+    const bf16x8 x = __builtin_bit_cast(bf16x8, tok_narrow(left));
+    [[maybe_unused]] bf16x8 x2;
+    if constexpr (FINE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) left[i] -= (float)x[i];
+      x2 = __builtin_bit_cast(bf16x8, tok_narrow(left));
+    }
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) {
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 16 * s * L::LD + 32 * j));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b + 16 * s * L::LD + 32 * j));
       const s16x8 y = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if constexpr (FINE) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, y), x2, acc[j], 0, 0, 0);
       acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, y), x, acc[j], 0, 0, 0);
     }
   }
 }
-template <int DP>
+template <int DP, bool>
 __device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
   constexpr int LD = Tile<float, DP, true>::LD;
   const int h = lane >> 5, c = lane & 31;
@@ -226,6 +240,18 @@ constexpr int tile_len() {
   return sizeof(T) == 2 ? 64 : DP >= 128 ? 32 : 64;
 }
 
+// What rounding four values to bf16 leaves of them, rounded itself (2^-17 of the value). delta = go o is a small difference's
+// worth in ds = p (go v^T - delta) where a row has few keys: taken from the rounded o alone it would carry more error than
+// all other roundings together.
+__device__ __forceinline__ float left_over(float x) { return x - (float)(__bf16)x; }
+__device__ __forceinline__ void store_low(__bf16* p, float a, float b, float c, float d) {
+  tok_store4(p, left_over(a), left_over(b), left_over(c), left_over(d));
+}
+__device__ __forceinline__ size_t low_at(const AttnParams& p, int b, int hk, int r) {
+  const int t = row_query(p, r), h = hk * p.G + r - t * p.G;
+  return (((size_t)b * p.g.Tq + t) * p.g.Hq + h) * p.g.D;
+}
+
 template <class T>
 __device__ __forceinline__ void store_cols(T* row, const f32x16& a, int j, int h, int D, float f) {
 #pragma unroll
@@ -238,7 +264,7 @@ __device__ __forceinline__ void store_cols(T* row, const f32x16& a, int j, int h
 // ---- forward --------------------------------------------------------------------------------------------------------
 // Grid: (row tile, split, problem), the row tiles of a problem on one XCD. SPLIT: every split leaves its unnormalised
 // rows, maximum and sum for the joining kernel.
-template <class T, int DP, bool SPLIT>
+template <class T, int DP, bool SPLIT, bool FINE>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(const AttnParams p) {
   constexpr int KT = tile_len<T, DP>();
   __shared__ __attribute__((aligned(16))) T ktile[2][KT * Tile<T, DP, false>::LD];
@@ -317,7 +343,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
         l += s[kk][i];
       }
 #pragma unroll
-    for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP>(vtile[buf], s[kk], 32 * kk, lane, o);
+    for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP, FINE>(vtile[buf], s[kk], 32 * kk, lane, o);
     if (more) {
       sk.store(ktile[buf ^ 1]);
       sv.store(vtile[buf ^ 1]);
@@ -341,36 +367,65 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
     T* out = const_cast<T*>(row_at<T>(p.out, g.o, p, b, hk, r));
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) store_cols(out, r < rows ? o[d] : zero16(), d, h, g.D, f);
+    if constexpr (sizeof(T) == 2) {
+      if (p.low && r < rows) {           // (other rows' are not read)
+        __bf16* low = p.low + low_at(p, b, hk, r);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            if (32 * d + 2 * i + 4 * h < g.D)
+              store_low(low + 32 * d + 2 * i + 4 * h, o[d][i] * f, o[d][i + 1] * f, o[d][i + 2] * f, o[d][i + 3] * f);
+      }
+    }
     // a row without keys: +inf, so that the backward pass finds p = exp(s - inf) = 0
     if (h == 0 && p.lse) p.lse[(size_t)prob * p.R + r] = f != 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
   }
 }
 
-// Joins the splits of a row: D / 4 lanes a row (rounded up to a power of two), 4 elements each.
+// Joins the splits of a row: DP / 4 lanes of 4 elements side by side, the row's splits dealt to `per_row` such groups of lanes.
 template <class T, int DP>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
-  constexpr int LPR = DP / 4;
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int per_row) {
+  constexpr int LPR = DP / 4, GROUPS = 256 / LPR;
+  __shared__ float red[GROUPS][DP + 4];
+  __shared__ float tops[GROUPS], sums[GROUPS];
   const vg_attention_geom& g = p.g;
-  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int d = (threadIdx.x % LPR) * 4;
-  if (row >= (long long)g.B * g.Hk * p.R) return;
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, share = group % per_row;
+  const long long row = (long long)blockIdx.x * (GROUPS / per_row) + group / per_row;
+  const bool in = row < (long long)g.B * g.Hk * p.R;
   const int prob = (int)(row / p.R), r = (int)(row - (long long)prob * p.R);
   const int b = prob / g.Hk, hk = prob - b * g.Hk;
   const size_t first = (size_t)prob * p.splits * p.R + r;
-  float m = -FLT_MAX;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (first + (size_t)s * p.R)]);
-  float l = 0.f;
+  float m = -FLT_MAX, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
+  for (int s = in ? share : p.splits; s < p.splits; s += per_row) {
     const size_t at = first + (size_t)s * p.R;
-    const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - m);
-    l += f * p.part_ml[2 * at + 1];
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * DP + d);
+    const float ms = p.part_ml[2 * at], ls = p.part_ml[2 * at + 1];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * DP + 4 * lane);
+    const float top = fmaxf(m, ms), a = __builtin_amdgcn_exp2f(m - top), f = __builtin_amdgcn_exp2f(ms - top);
+    m = top;
+    l = l * a + f * ls;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * a + f * x[e];
+  }
+  *reinterpret_cast<f32x4*>(&red[group][4 * lane]) = o;
+  if (lane == 0) {
+    tops[group] = m;
+    sums[group] = l;
+  }
+  __syncthreads();
+  if (share || !in) return;
+  for (int s = group + 1; s < group + per_row; ++s) {
+    const float ms = tops[s], top = fmaxf(m, ms), a = __builtin_amdgcn_exp2f(m - top), f = __builtin_amdgcn_exp2f(ms - top);
+    m = top;
+    l = l * a + f * sums[s];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * a + f * red[s][4 * lane + e];
   }
   const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int d = 4 * lane;
   if (d < g.D) tok_store4(const_cast<T*>(row_at<T>(p.out, g.o, p, b, hk, r)) + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+  if (sizeof(T) == 2 && p.low && d < g.D) store_low(p.low + low_at(p, b, hk, r) + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
   if (d == 0 && p.lse) p.lse[row] = f != 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
@@ -392,6 +447,14 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, flo
         float x[V], y[V];
         tok_widen(*reinterpret_cast<const u32x4*>(go + d), x);
         tok_widen(*reinterpret_cast<const u32x4*>(o + d), y);
+        if constexpr (sizeof(T) == 2) {
+          if (p.low) {
+            float z[V];
+            tok_widen(*reinterpret_cast<const u32x4*>(p.low + low_at(p, b, hk, r) + d), z);
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] += z[e];
+          }
+        }
 #pragma unroll
         for (int e = 0; e < V; ++e) sum = __builtin_fmaf(x[e], y[e], sum);
       }
@@ -404,13 +467,18 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, flo
 
 // Queries' gradient: the forward kernel's walk with p rebuilt from lse. Heads of 128 take their keys 32 at a time (fewer
 // staging registers: at 64 the kernel spills, video case 1993 us).
-template <class T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(const AttnParams p) {
-  constexpr int KT = DP >= 128 ? 32 : tile_len<T, DP>();
-  __shared__ __attribute__((aligned(16))) T ktile[2][KT * Tile<T, DP, true>::LD];
-  __shared__ __attribute__((aligned(16))) T vtile[2][KT * Tile<T, DP, false>::LD];
+template <class T, int DP>
+struct GqTiles {
+  static constexpr int KT = DP >= 128 ? 32 : tile_len<T, DP>();
+  T k[2][KT * Tile<T, DP, true>::LD];
+  T v[2][KT * Tile<T, DP, false>::LD];
+};
+template <class T, int DP, bool FINE>
+__device__ __forceinline__ void queries_gradient(const AttnParams& p, int id, GqTiles<T, DP>& tiles) {
+  constexpr int KT = GqTiles<T, DP>::KT;
+  auto& ktile = tiles.k;
+  auto& vtile = tiles.v;
   const vg_attention_geom& g = p.g;
-  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
   const int rt = id % p.row_tiles, sp = (id / p.row_tiles) % p.splits, prob = id / (p.row_tiles * p.splits);
   const int b = prob / g.Hk, hk = prob - b * g.Hk;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
@@ -465,7 +533,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= s[i];
-      mul_cols<DP>(ktile[buf], dp, 32 * kk, lane, acc);
+      if (kl == 1) dp = zero16();          // (the softmax of one key is constant)
+      mul_cols<DP, FINE>(ktile[buf], dp, 32 * kk, lane, acc);
     }
     if (more) {
       sk.store(ktile[buf ^ 1]);
@@ -475,7 +544,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gq_kernel(co
     buf ^= 1;
   }
   if (r >= p.R) return;
-  if constexpr (SPLIT) {
+  if (p.splits > 1) {
     float* out = p.part + (((size_t)prob * p.splits + sp) * p.R + r) * DP;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) store_cols(out, acc[d], d, h, DP, 1.f);
@@ -493,23 +562,30 @@ template <class T, int DP>
 constexpr int row_len() {
   return sizeof(T) == 2 && DP < 128 ? 64 : 32;
 }
-template <class T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(const AttnParams p) {
-  constexpr int RT = row_len<T, DP>();
-  constexpr bool kValuesInLds = sizeof(T) == 2 && DP == 128;
+template <class T, int DP>
+struct GkvTiles {
+  static constexpr int RT = row_len<T, DP>();
+  static constexpr bool kValues = sizeof(T) == 2 && DP == 128;
+  T rows[2][2][RT * Tile<T, DP, true>::LD];              // [buffer][queries, their output gradients]
+  T v[kValues ? kTileRows * Tile<T, DP, false>::LD : 8];
+  float stat[2][2][RT];                                  // [buffer][row sums' logarithms, -delta]
+};
+template <class T, int DP, bool FINE>
+__device__ __forceinline__ void keys_gradient(const AttnParams& p, int id, GkvTiles<T, DP>& tiles) {
+  constexpr int RT = GkvTiles<T, DP>::RT;
+  constexpr bool kValuesInLds = GkvTiles<T, DP>::kValues;
   using Plain = Tile<T, DP, false>;
-  __shared__ __attribute__((aligned(16))) T smem[2][2][RT * Tile<T, DP, true>::LD];
-  __shared__ __attribute__((aligned(16))) T vtile[kValuesInLds ? kTileRows * Plain::LD : 1];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][RT];
+  auto& smem = tiles.rows;
+  auto& vtile = tiles.v;
+  auto& stat = tiles.stat;
   const vg_attention_geom& g = p.g;
-  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
-  const int kt = id % p.key_tiles, sp = (id / p.key_tiles) % p.splits, prob = id / (p.key_tiles * p.splits);
+  const int kt = id % p.key_tiles, sp = (id / p.key_tiles) % p.r_splits, prob = id / (p.key_tiles * p.r_splits);
   const int b = prob / g.Hk, hk = prob - b * g.Hk;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
   const int rows = clamped(p.q_len, b, g.Tq) * p.G;
   const int kl = clamped(p.k_len, b, g.Tk);
   const int key = kt * kTileRows + wid * 32 + c;
-  const int rbeg = sp * p.chunk, rend = kt * kTileRows < kl ? min(rows, rbeg + p.chunk) : 0;
+  const int rbeg = sp * p.r_chunk, rend = kt * kTileRows < kl ? min(rows, rbeg + p.r_chunk) : 0;
 
   RowFrag<T, DP> kf, vf;
   kf.load((const T*)p.k + b * g.k.sb + hk * g.k.sh + (int64_t)(key < kl ? key : 0) * g.k.st, g.D, h, key < kl);
@@ -588,9 +664,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(c
         dp = mul_rows<DP, true>(smem[buf][1], vf, 32 * rr, c, h, dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= w[i];
-      mul_cols<DP>(smem[buf][1], w, 32 * rr, lane, gv);
+      if (kl == 1) dp = zero16();          // (the softmax of one key is constant)
+      mul_cols<DP, FINE>(smem[buf][1], w, 32 * rr, lane, gv);
       __builtin_amdgcn_sched_barrier(0);     // (reads hoisted across this line spill)
-      mul_cols<DP>(smem[buf][0], dp, 32 * rr, lane, gk);
+      mul_cols<DP, FINE>(smem[buf][0], dp, 32 * rr, lane, gk);
     }
     if (more) put(buf ^ 1);
     __syncthreads();
@@ -598,15 +675,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(c
   }
   if (key >= g.Tk) return;
   // keys that take no part went through the products as zeros: their columns are not used
-  const float live = key < kl ? 1.f : 0.f;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) {
     if (key >= kl) gk[d] = gv[d] = zero16();
-    if constexpr (SPLIT) {
-      const size_t at = (((size_t)prob * p.splits + sp) * g.Tk + key) * DP;
-      const size_t half = (size_t)g.B * g.Hk * p.splits * g.Tk * DP;
-      store_cols(p.part + at, gk[d], d, h, DP, 1.f);
-      store_cols(p.part + half + at, gv[d], d, h, DP, 1.f);
+    if (p.r_splits > 1) {
+      const size_t at = (((size_t)prob * p.r_splits + sp) * g.Tk + key) * DP;
+      const size_t half = (size_t)g.B * g.Hk * p.r_splits * g.Tk * DP;
+      store_cols(p.part_kv + at, gk[d], d, h, DP, 1.f);
+      store_cols(p.part_kv + half + at, gv[d], d, h, DP, 1.f);
     } else {
       store_cols((T*)p.gk + b * g.gk.sb + hk * g.gk.sh + (int64_t)key * g.gk.st, gk[d], d, h, g.D, g.scale);
       store_cols((T*)p.gv + b * g.gv.sb + hk * g.gv.sh + (int64_t)key * g.gv.st, gv[d], d, h, g.D, 1.f);
@@ -614,20 +690,41 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_gkv_kernel(c
   }
 }
 
-// out = factor * sum over splits of part[prob][split][n][DP]; which = 0 queries' rows, 1 keys, 2 values
+// Both in one launch, so that neither waits for the other's last blocks: those of the keys' gradient, which take longer, first.
+template <class T, int DP, bool FINE>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) attn_bwd_kernel(const AttnParams p) {
+  __shared__ __attribute__((aligned(16))) union {
+    unsigned char keys[sizeof(GkvTiles<T, DP>)];
+    unsigned char queries[sizeof(GqTiles<T, DP>)];
+  } smem;
+  const int id = blockIdx.x - p.gkv_blocks;
+  if (id < 0)
+    keys_gradient<T, DP, FINE>(p, tok_xcd_order(blockIdx.x, p.gkv_blocks), *reinterpret_cast<GkvTiles<T, DP>*>(smem.keys));
+  else
+    queries_gradient<T, DP, FINE>(p, tok_xcd_order(id, gridDim.x - p.gkv_blocks), *reinterpret_cast<GqTiles<T, DP>*>(smem.queries));
+}
+
+// The split walks' results: queries' rows (if split), keys, values (if split), each the sum over its splits in order, times
+// scale (values: 1).
 template <class T, int DP>
-__global__ void __launch_bounds__(256) attn_sum_kernel(const AttnParams p, const float* part, int which) {
+__global__ void __launch_bounds__(256) attn_sum_kernel(const AttnParams p) {
   constexpr int LPR = DP / 4;
   const vg_attention_geom& g = p.g;
-  const int n = which == 0 ? p.R : g.Tk;
-  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const long long nq = p.splits > 1 ? (long long)g.B * g.Hk * p.R : 0, nk = p.r_splits > 1 ? (long long)g.B * g.Hk * g.Tk : 0;
+  long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int d = (threadIdx.x % LPR) * 4;
-  if (row >= (long long)g.B * g.Hk * n || d >= g.D) return;
+  if (row >= nq + 2 * nk || d >= g.D) return;
+  const int which = row < nq ? 0 : row < nq + nk ? 1 : 2;
+  row -= which == 0 ? 0 : which == 1 ? nq : nq + nk;
+  const int n = which == 0 ? p.R : g.Tk, splits = which == 0 ? p.splits : p.r_splits;
+  const float* part = which == 0 ? p.part : p.part_kv + (which == 2 ? (size_t)nk * splits * DP : 0);
   const int prob = (int)(row / n), r = (int)(row - (long long)prob * n);
   const int b = prob / g.Hk, hk = prob - b * g.Hk;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(part + (((size_t)prob * p.splits + s) * n + r) * DP + d);
+  part += ((size_t)prob * splits * n + r) * DP + d;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part + (size_t)s * n * DP);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += x[e];
   }
@@ -675,11 +772,12 @@ int check_strides(const vg_attention_geom* g, bool backward) {
 }
 
 // A walk over `len` (keys, or rows) is split where the blocks alone leave compute units idle: towards 512 blocks (two
-// for each of the 256), but no split shorter than 256, below which a split's own start and its partial results cost
-// more than the walk it saves.
+// for each of the 256), but no split shorter than two tiles of 64 (f32, whose products take eight times as long: one),
+// below which a split's own start and its partial results cost more than the walk it saves.
+template <class T>
 int splits_for(long long blocks, long long len) {
   if (blocks >= 256 || blocks == 0) return 1;
-  long long s = 512 / blocks, most = len / 256;
+  long long s = 512 / blocks, most = len / (sizeof(T) == 2 ? 128 : 64);
   if (s > most) s = most;
   return s < 1 ? 1 : (int)s;
 }
@@ -687,6 +785,7 @@ int splits_for(long long blocks, long long len) {
 struct Plan {
   int G, R, row_tiles, key_tiles, probs, fwd_splits, gkv_splits;
 };
+template <class T>
 Plan plan_of(const vg_attention_geom* g) {
   Plan q;
   q.G = g->Hq / g->Hk;
@@ -694,8 +793,8 @@ Plan plan_of(const vg_attention_geom* g) {
   q.probs = g->B * g->Hk;
   q.row_tiles = ceil_div(q.R, kTileRows);
   q.key_tiles = ceil_div(g->Tk, kTileRows);
-  q.fwd_splits = splits_for((long long)q.row_tiles * q.probs, g->Tk);
-  q.gkv_splits = splits_for((long long)q.key_tiles * q.probs, q.R);
+  q.fwd_splits = splits_for<T>((long long)q.row_tiles * q.probs, g->Tk);
+  q.gkv_splits = splits_for<T>((long long)q.key_tiles * q.probs, q.R);
   return q;
 }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -705,12 +804,13 @@ size_t fwd_bytes(const vg_attention_geom* g, const Plan& q) {
   const size_t rows = (size_t)q.probs * q.fwd_splits * q.R;
   return align256(rows * padded_width(g->D) * 4) + rows * 8;
 }
+// delta, partial queries' rows, partial keys and values
+size_t gq_bytes(const vg_attention_geom* g, const Plan& q) {
+  return q.fwd_splits == 1 ? 0 : align256((size_t)q.probs * q.fwd_splits * q.R * padded_width(g->D) * 4);
+}
 size_t bwd_bytes(const vg_attention_geom* g, const Plan& q) {
-  const size_t dp = padded_width(g->D);
-  size_t a = q.fwd_splits == 1 ? 0 : (size_t)q.probs * q.fwd_splits * q.R * dp * 4;
-  const size_t b = q.gkv_splits == 1 ? 0 : 2 * (size_t)q.probs * q.gkv_splits * g->Tk * dp * 4;
-  if (b > a) a = b;       // one after the other on one stream: they share the space
-  return align256((size_t)q.probs * q.R * 4) + a;
+  const size_t kv = q.gkv_splits == 1 ? 0 : 2 * (size_t)q.probs * q.gkv_splits * g->Tk * padded_width(g->D) * 4;
+  return align256((size_t)q.probs * q.R * 4) + gq_bytes(g, q) + kv;
 }
 
 AttnParams params_of(const vg_attention_geom* g, const Plan& q) {
@@ -726,53 +826,58 @@ AttnParams params_of(const vg_attention_geom* g, const Plan& q) {
 }
 int chunk_of(int len, int splits) { return ((len + splits - 1) / splits + 63) & ~63; }
 
-template <class T, int DP>
-void launch_fwd(AttnParams& p, const Plan& q, hipStream_t st) {
+// bf16: a probability's (ds's) rounding is one of very many that average out in a result, and costs it 0.4 of its own
+// rounding. In a small call they are too few for that; there both terms are taken, at no visible cost (up to 2^20
+// probabilities the products take a few microseconds).
+template <class T>
+bool fine(const vg_attention_geom& g) {
+  return sizeof(T) == 2 && (double)g.B * g.Hq * g.Tq * g.Tk < (double)(1 << 20);
+}
+template <class T, int DP, bool FINE>
+void launch_fwd_of(AttnParams& p, const Plan& q, hipStream_t st) {
   p.splits = q.fwd_splits;
   p.chunk = chunk_of(p.g.Tk, p.splits);
   const int grid = q.row_tiles * p.splits * q.probs;
   if (p.splits == 1) {
-    attn_fwd_kernel<T, DP, false><<<grid, 256, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, false, FINE><<<grid, 256, 0, st>>>(p);
   } else {
-    attn_fwd_kernel<T, DP, true><<<grid, 256, 0, st>>>(p);
-    attn_join_kernel<T, DP><<<ceil_div((long long)q.probs * q.R, 256 / (DP / 4)), 256, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, true, FINE><<<grid, 256, 0, st>>>(p);
+    int per_row = 1;           // four splits a group of lanes
+    while (per_row < 256 / (DP / 4) && per_row * 4 < p.splits) per_row *= 2;
+    attn_join_kernel<T, DP><<<ceil_div((long long)q.probs * q.R * per_row, 256 / (DP / 4)), 256, 0, st>>>(p, per_row);
   }
 }
 template <class T, int DP>
+void launch_fwd(AttnParams& p, const Plan& q, hipStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (fine<T>(p.g)) return launch_fwd_of<T, DP, true>(p, q, st);
+  launch_fwd_of<T, DP, false>(p, q, st);
+}
+template <class T, int DP>
 void launch_bwd(AttnParams& p, const Plan& q, float* delta, hipStream_t st) {
-  if (q.probs * (long long)q.R > 0) attn_delta_kernel<T><<<ceil_div((long long)q.probs * q.R, 32), 256, 0, st>>>(p, delta);
-  if (q.row_tiles > 0 && p.gq) {
-    p.splits = q.fwd_splits;
-    p.chunk = chunk_of(p.g.Tk, p.splits);
-    const int grid = q.row_tiles * p.splits * q.probs;
-    if (p.splits == 1) {
-      attn_gq_kernel<T, DP, false><<<grid, 256, 0, st>>>(p);
-    } else {
-      attn_gq_kernel<T, DP, true><<<grid, 256, 0, st>>>(p);
-      attn_sum_kernel<T, DP><<<ceil_div((long long)q.probs * q.R, 256 / (DP / 4)), 256, 0, st>>>(p, p.part, 0);
-    }
+  if (q.R > 0) attn_delta_kernel<T><<<ceil_div((long long)q.probs * q.R, 32), 256, 0, st>>>(p, delta);
+  p.splits = p.gq ? q.fwd_splits : 1;
+  p.chunk = chunk_of(p.g.Tk, p.splits);
+  p.r_splits = p.gk ? q.gkv_splits : 1;
+  p.r_chunk = chunk_of(q.R, p.r_splits);
+  p.gkv_blocks = p.gk ? q.key_tiles * p.r_splits * q.probs : 0;
+  const int gq_blocks = p.gq ? q.row_tiles * p.splits * q.probs : 0;
+  if (p.gkv_blocks + gq_blocks > 0) {
+    auto kernel = attn_bwd_kernel<T, DP, false>;
+    if constexpr (sizeof(T) == 2)
+      if (fine<T>(p.g)) kernel = attn_bwd_kernel<T, DP, true>;
+    kernel<<<p.gkv_blocks + gq_blocks, 256, 0, st>>>(p);
   }
-  if (q.key_tiles > 0 && p.gk) {
-    p.splits = q.gkv_splits;
-    p.chunk = chunk_of(q.R, p.splits);
-    const int grid = q.key_tiles * p.splits * q.probs;
-    if (p.splits == 1) {
-      attn_gkv_kernel<T, DP, false><<<grid, 256, 0, st>>>(p);
-    } else {
-      attn_gkv_kernel<T, DP, true><<<grid, 256, 0, st>>>(p);
-      const int blocks = ceil_div((long long)q.probs * p.g.Tk, 256 / (DP / 4));
-      attn_sum_kernel<T, DP><<<blocks, 256, 0, st>>>(p, p.part, 1);
-      attn_sum_kernel<T, DP><<<blocks, 256, 0, st>>>(p, p.part + (size_t)q.probs * p.splits * p.g.Tk * DP, 2);
-    }
-  }
+  const long long rows = (p.splits > 1 ? (long long)q.probs * q.R : 0) + (p.r_splits > 1 ? 2ll * q.probs * p.g.Tk : 0);
+  if (rows > 0) attn_sum_kernel<T, DP><<<ceil_div(rows, 256 / (DP / 4)), 256, 0, st>>>(p);
 }
 
 template <class T>
 int attention_fwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len,
-                  void* o, float* lse, void* ws, size_t ws_bytes, void* stream) {
+                  void* o, void* low, float* lse, void* ws, size_t ws_bytes, void* stream) {
   const int rc = check_geom(g);
   if (rc) return rc;
-  const Plan pl = plan_of(g);
+  const Plan pl = plan_of<T>(g);
   if (pl.probs == 0 || pl.R == 0) return VG_OK;
   VG_REQUIRE(q && o && (g->Tk == 0 || (k && v)), "attention: null tensor");
   VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->Tq, g->Hq) && tok_layout_ok<T>(g->o, o, g->B, g->Tq, g->Hq) &&
@@ -788,6 +893,7 @@ int attention_fwd(const vg_attention_geom* g, const void* q, const void* k, cons
   p.k = k;
   p.v = v;
   p.out = o;
+  p.low = (__bf16*)low;
   p.lse = lse;
   p.q_len = q_len;
   p.k_len = k_len;
@@ -804,11 +910,11 @@ int attention_fwd(const vg_attention_geom* g, const void* q, const void* k, cons
 }
 
 template <class T>
-int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* go,
+int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const void* low, const float* lse, const void* go,
                   const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* ws, size_t ws_bytes, void* stream) {
   const int rc = check_geom(g);
   if (rc) return rc;
-  const Plan pl = plan_of(g);
+  const Plan pl = plan_of<T>(g);
   if (pl.probs == 0 || (pl.R == 0 && g->Tk == 0)) return VG_OK;
   VG_REQUIRE((pl.R == 0 || (q && o && lse && go)) && (g->Tk == 0 || (k && v)) && !gk == !gv, "attention backward: null tensor");
   VG_REQUIRE(tok_layout_ok<T>(g->q, q, g->B, g->Tq, g->Hq) && tok_layout_ok<T>(g->o, o, g->B, g->Tq, g->Hq) &&
@@ -828,6 +934,7 @@ int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, cons
   p.v = v;
   p.o = o;
   p.go = go;
+  p.low = (__bf16*)const_cast<void*>(low);
   p.lse_in = lse;
   p.q_len = q_len;
   p.k_len = k_len;
@@ -837,6 +944,7 @@ int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, cons
   float* delta = (float*)ws;
   p.delta = delta;
   p.part = (float*)((char*)ws + align256((size_t)pl.probs * pl.R * 4));
+  p.part_kv = (float*)((char*)p.part + gq_bytes(g, pl));
   hipStream_t st = (hipStream_t)stream;
   switch (padded_width(g->D)) {
     case 32: launch_bwd<T, 32>(p, pl, delta, st); break;
@@ -851,29 +959,31 @@ int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, cons
 
 extern "C" {
 
-size_t vg_attention_workspace_bytes(const vg_attention_geom* g, int backward) {
+size_t vg_attention_workspace_bytes(const vg_attention_geom* g, int backward, int half) {
   if (check_geom(g)) return 0;
-  const Plan q = plan_of(g);
+  const Plan q = half ? plan_of<__bf16>(g) : plan_of<float>(g);
   if (q.probs == 0) return 0;
   return backward ? bwd_bytes(g, q) : fwd_bytes(g, q);
 }
 int vg_attention_fwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const int32_t* q_len, const int32_t* k_len,
                      float* o, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  return attention_fwd<float>(g, q, k, v, q_len, k_len, o, lse, workspace, workspace_bytes, stream);
+  return attention_fwd<float>(g, q, k, v, q_len, k_len, o, nullptr, lse, workspace, workspace_bytes, stream);
 }
 int vg_attention_fwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len,
-                       void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  return attention_fwd<__bf16>(g, q, k, v, q_len, k_len, o, lse, workspace, workspace_bytes, stream);
+                       void* o, void* o_low, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  VG_REQUIRE(vg_aligned16(o_low), "attention: a tensor does not start on a 16-byte border");
+  return attention_fwd<__bf16>(g, q, k, v, q_len, k_len, o, o_low, lse, workspace, workspace_bytes, stream);
 }
 int vg_attention_bwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const float* o, const float* lse,
                      const float* go, const int32_t* q_len, const int32_t* k_len, float* gq, float* gk, float* gv, void* workspace,
                      size_t workspace_bytes, void* stream) {
-  return attention_bwd<float>(g, q, k, v, o, lse, go, q_len, k_len, gq, gk, gv, workspace, workspace_bytes, stream);
+  return attention_bwd<float>(g, q, k, v, o, nullptr, lse, go, q_len, k_len, gq, gk, gv, workspace, workspace_bytes, stream);
 }
-int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                       const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* workspace,
-                       size_t workspace_bytes, void* stream) {
-  return attention_bwd<__bf16>(g, q, k, v, o, lse, go, q_len, k_len, gq, gk, gv, workspace, workspace_bytes, stream);
+int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const void* o_low,
+                       const float* lse, const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  VG_REQUIRE(vg_aligned16(o_low), "attention backward: a tensor does not start on a 16-byte border");
+  return attention_bwd<__bf16>(g, q, k, v, o, o_low, lse, go, q_len, k_len, gq, gk, gv, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -21,9 +21,9 @@ struct GatedParams {
   void* h;               // forward: [M][F]
   float* z;              // forward: [M][2F] or null
   const void* gh;        // recomputing backward: [M][F]
-  void* gz;              // [M][2F]
+  void* gz;              // [M][2F], two of them where `terms` is 2: the rounded gradient and what the rounding left
   float* gb_part;        // [row tiles][2F] or null
-  int M, C, F, act, row_tiles, col_tiles;
+  int M, C, F, act, row_tiles, col_tiles, terms;
 };
 
 // The gates. f32 takes the library's exponential and error function. bf16 results keep 8 bits: the hardware's exponential
@@ -186,6 +186,16 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gated_kernel(const 
         if constexpr (BWD) {
           store16((T*)p.gz + at2, left, gg);
           store16((T*)p.gz + at2 + p.F, left, gu);
+          if (sizeof(T) == 2 && p.terms == 2) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              gg[e] -= (float)(T)gg[e];
+              gu[e] -= (float)(T)gu[e];
+            }
+            T* low = (T*)p.gz + (size_t)p.M * 2 * p.F + at2;
+            store16(low, left, gg);
+            store16(low + p.F, left, gu);
+          }
         } else {
           store16((T*)p.h + at, left, gg);
           if (p.z) {
@@ -347,12 +357,20 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
         su[e] += gu[e];
       }
       T* out = (T*)p.gz + (size_t)m * 2 * p.F + f;
-      if constexpr (V == 4) {
-        tok_store4(out, gg[0], gg[1], gg[2], gg[3]);
-        tok_store4(out + p.F, gu[0], gu[1], gu[2], gu[3]);
-      } else {
-        out[0] = (T)gg[0];
-        out[p.F] = (T)gu[0];
+      for (int t = 0; t < p.terms; ++t) {
+        if constexpr (V == 4) {
+          tok_store4(out, gg[0], gg[1], gg[2], gg[3]);
+          tok_store4(out + p.F, gu[0], gu[1], gu[2], gu[3]);
+        } else {
+          out[0] = (T)gg[0];
+          out[p.F] = (T)gu[0];
+        }
+        out += (size_t)p.M * 2 * p.F;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          gg[e] -= (float)(T)gg[e];
+          gu[e] -= (float)(T)gu[e];
+        }
       }
     }
   }
@@ -378,22 +396,23 @@ struct ProductParams {
   int64_t lda, ldb;
   int M, N, K;
   void* out;            // [M][N], or splits slabs of it (f32)
-  int out_f32, col_tiles, tiles, splits, chunk;
+  int64_t a_term;       // elements from the first term of a to the second
+  int out_f32, col_tiles, tiles, splits, chunk;     // splits: of each term
 };
 template <class T, bool ARC, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) product_kernel(const ProductParams p) {
   using G = TokGemm<T, ARC, true, BM, BN, WM, WN>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
   const int id = tok_xcd_order(blockIdx.x, gridDim.x);
-  const int sp = id / p.tiles, t = id - sp * p.tiles;
+  const int slab_id = id / p.tiles, t = id - slab_id * p.tiles, term = slab_id / p.splits, sp = slab_id - term * p.splits;
   const int mt = t / p.col_tiles, nt = t - mt * p.col_tiles;
   const int m0 = mt * BM, n0 = nt * BN, kbeg = sp * p.chunk, kend = min(p.K, kbeg + p.chunk);
   f32x16 acc[G::TM][G::TN];
-  const TokOperand<T> A = {(const T*)p.a, p.lda, p.M, 0}, B = {(const T*)p.b, p.ldb, p.N, 0};
+  const TokOperand<T> A = {(const T*)p.a + term * p.a_term, p.lda, p.M, 0}, B = {(const T*)p.b, p.ldb, p.N, 0};
   G::run(A, B, m0, n0, kbeg, kend, reinterpret_cast<T*>(smem_raw), acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
   const int wm = wid / WN, wn = wid % WN;
-  const size_t slab = (size_t)sp * p.M * p.N;
+  const size_t slab = (size_t)slab_id * p.M * p.N;
 #pragma unroll
   for (int j = 0; j < G::TN; ++j) {
     const int n = n0 + (wn * G::TN + j) * 32 + c;
@@ -529,27 +548,27 @@ ProductPlan product_plan(int M, int N, int K) {
   return best;
 }
 template <class T>
-size_t product_bytes(int M, int N, int K) {
-  const int s = product_plan<T>(M, N, K).splits;
+size_t product_bytes(int M, int N, int K, int terms) {
+  const int s = product_plan<T>(M, N, K).splits * terms;
   return s == 1 ? 0 : (size_t)s * M * N * 4;
 }
 
 template <class T, bool ARC, int BMN, int WM, int WN>
-int launch_product(ProductParams& p, hipStream_t st) {
+int launch_product(ProductParams& p, int slabs, hipStream_t st) {
   using G = TokGemm<T, ARC, true, BMN, BMN, WM, WN>;
   p.col_tiles = ceil_div(p.N, BMN);
   p.tiles = ceil_div(p.M, BMN) * p.col_tiles;
   auto kernel = product_kernel<T, ARC, BMN, BMN, WM, WN>;
   const int rc = allow_lds(kernel, G::LDS_BYTES);
   if (rc) return rc;
-  kernel<<<p.tiles * p.splits, G::NT, G::LDS_BYTES, st>>>(p);
+  kernel<<<p.tiles * slabs, G::NT, G::LDS_BYTES, st>>>(p);
   return VG_OK;
 }
 template <class T, bool ARC>
-int product(const void* a, int64_t lda, const void* b, int64_t ldb, int M, int N, int K, void* out, int out_f32, void* ws, size_t ws_bytes,
-            hipStream_t st) {
+int product(const void* a, int64_t lda, int terms, int64_t a_term, const void* b, int64_t ldb, int M, int N, int K, void* out, int out_f32,
+            void* ws, size_t ws_bytes, hipStream_t st) {
   const ProductPlan plan = product_plan<T>(M, N, K);
-  const size_t need = product_bytes<T>(M, N, K);
+  const size_t need = product_bytes<T>(M, N, K, terms);
   if (need && (!ws || ws_bytes < need)) return vg_fail(VG_ERR_WORKSPACE, "gated backward: workspace of %zu bytes, %zu are needed", ws_bytes, need);
   ProductParams p = {};
   p.a = a;
@@ -561,20 +580,22 @@ int product(const void* a, int64_t lda, const void* b, int64_t ldb, int M, int N
   p.K = K;
   p.splits = plan.splits;
   p.chunk = plan.chunk;
-  p.out = p.splits > 1 ? ws : out;
-  p.out_f32 = p.splits > 1 ? 1 : out_f32;
+  p.a_term = a_term;
+  const int slabs = plan.splits * terms;
+  p.out = slabs > 1 ? ws : out;
+  p.out_f32 = slabs > 1 ? 1 : out_f32;
   int rc;
   if constexpr (sizeof(T) == 2)
-    rc = plan.tile == 256 ? launch_product<T, ARC, 256, 2, 4>(p, st) : launch_product<T, ARC, 128, 2, 2>(p, st);
+    rc = plan.tile == 256 ? launch_product<T, ARC, 256, 2, 4>(p, slabs, st) : launch_product<T, ARC, 128, 2, 2>(p, slabs, st);
   else
-    rc = launch_product<T, ARC, 128, 2, 4>(p, st);
+    rc = launch_product<T, ARC, 128, 2, 4>(p, slabs, st);
   if (rc) return rc;
-  if (p.splits > 1) {
+  if (slabs > 1) {
     const size_t n = (size_t)M * N;
     if (out_f32)
-      slab_sum_kernel<float><<<vg_stream_grid(n, 256), 256, 0, st>>>((const float*)ws, p.splits, n, (float*)out);
+      slab_sum_kernel<float><<<vg_stream_grid(n, 256), 256, 0, st>>>((const float*)ws, slabs, n, (float*)out);
     else
-      slab_sum_kernel<__bf16><<<vg_stream_grid(n, 256), 256, 0, st>>>((const float*)ws, p.splits, n, (__bf16*)out);
+      slab_sum_kernel<__bf16><<<vg_stream_grid(n, 256), 256, 0, st>>>((const float*)ws, slabs, n, (__bf16*)out);
   }
   VG_CHECK_LAUNCH("gated backward product");
   return VG_OK;
@@ -588,6 +609,12 @@ bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 768; 
 
 // Scratch of the backward pass, one piece after the other: [gg gu], partial column sums and their reduction's scratch,
 // slabs of the two products (one after the other on one stream: they share the space).
+// bf16: [gg gu] is rounded to bf16 for the two products; of the many roundings in a sum most averages out, and what stays
+// costs a result 0.4 of its own rounding. In a small call (under 2^19 of them) they are too few for that: there what the
+// rounding left is multiplied too, as a second term, at no visible cost.
+template <class T>
+int gz_terms(int M, int F) { return sizeof(T) == 2 && (long long)M * 2 * F < (1 << 19) ? 2 : 1; }
+
 struct BwdSpace {
   size_t gz, part, colsum, slabs, total;
   int rows;          // of partial column sums
@@ -598,10 +625,11 @@ BwdSpace bwd_space(int M, int C, int F) {
   BwdSpace s;
   s.rows = ceil_div(M, keeps_z<T>(M, C) ? kRowsBlock : large_tiles<T>(M, 2ll * F) ? 256 : 128);
   s.gz = 0;
-  s.part = align256((size_t)M * 2 * F * sizeof(T));
+  s.part = align256((size_t)M * 2 * F * sizeof(T) * gz_terms<T>(M, F));
   s.colsum = s.part + align256((size_t)s.rows * 2 * F * 4);
   s.slabs = s.colsum + align256(vg_colsum_workspace_bytes(s.rows, 2 * F));
-  const size_t a = product_bytes<T>(M, C, 2 * F), b = product_bytes<T>(2 * F, C, M);
+  const int terms = gz_terms<T>(M, F);
+  const size_t a = product_bytes<T>(M, C, 2 * F, terms), b = product_bytes<T>(2 * F, C, M, terms);
   s.total = s.slabs + (a > b ? a : b);
   return s;
 }
@@ -613,7 +641,7 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (M == 0) {        // sums over no rows
-    if (gw) rc = product<T, true>(gh, 2 * (int64_t)F, x, C, 2 * F, C, 0, gw, gw_f32, nullptr, 0, st);
+    if (gw) rc = product<T, true>(gh, 2 * (int64_t)F, 1, 0, x, C, 2 * F, C, 0, gw, gw_f32, nullptr, 0, st);
     if (!rc && gb) rc = vg_fill(gb, 0.f, 2 * (size_t)F, stream);
     return rc;
   }
@@ -635,6 +663,7 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
   p.C = C;
   p.F = F;
   p.act = act;
+  p.terms = gz_terms<T>(M, F);
   if (keeps_z<T>(M, C)) {
     p.z = const_cast<float*>(z);
     const bool wide = F % 4 == 0 && vg_aligned16(z) && vg_aligned16(gh);
@@ -653,10 +682,10 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
     if (rc) return rc;
   }
   if (gx) {
-    rc = product<T, false>(p.gz, 2 * (int64_t)F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, at + s.slabs, s.total - s.slabs, st);
+    rc = product<T, false>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, at + s.slabs, s.total - s.slabs, st);
     if (rc) return rc;
   }
-  if (gw) rc = product<T, true>(p.gz, 2 * (int64_t)F, x, C, 2 * F, C, M, gw, gw_f32, at + s.slabs, s.total - s.slabs, st);
+  if (gw) rc = product<T, true>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, x, C, 2 * F, C, M, gw, gw_f32, at + s.slabs, s.total - s.slabs, st);
   return rc;
 }
 

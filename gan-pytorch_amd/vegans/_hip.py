@@ -186,11 +186,11 @@ SIGNATURES = {
     "vg_qk_norm_rotary_fwd_h": (c_int, [_RG] + [_P] * 8),
     "vg_qk_norm_rotary_bwd": (c_int, [_RG] + [_P] * 12 + [c_size_t, _P]),
     "vg_qk_norm_rotary_bwd_h": (c_int, [_RG] + [_P] * 12 + [c_size_t, _P]),
-    "vg_attention_workspace_bytes": (c_size_t, [_AG, c_int]),
+    "vg_attention_workspace_bytes": (c_size_t, [_AG, c_int, c_int]),
     "vg_attention_fwd": (c_int, [_AG] + [_P] * 8 + [c_size_t, _P]),
-    "vg_attention_fwd_h": (c_int, [_AG] + [_P] * 8 + [c_size_t, _P]),
+    "vg_attention_fwd_h": (c_int, [_AG] + [_P] * 9 + [c_size_t, _P]),
     "vg_attention_bwd": (c_int, [_AG] + [_P] * 12 + [c_size_t, _P]),
-    "vg_attention_bwd_h": (c_int, [_AG] + [_P] * 12 + [c_size_t, _P]),
+    "vg_attention_bwd_h": (c_int, [_AG] + [_P] * 13 + [c_size_t, _P]),
     "vg_gated_linear_fwd": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
     "vg_gated_linear_fwd_h": (c_int, [c_int] * 3 + [_P] * 5 + [c_int, _P]),
     "vg_gated_linear_keeps_z": (c_int, [c_int] * 4),

@@ -2125,22 +2125,27 @@ class _AttentionPlan:
             g.gv = gv_layout
         self.fwd_name, self.bwd_name = _A("vg_attention_fwd", q), _A("vg_attention_bwd", q)
         self.fwd, self.bwd = getattr(lib, self.fwd_name), getattr(lib, self.bwd_name)
-        self.fwd_scratch, self.bwd_scratch = (lib.vg_attention_workspace_bytes(ctypes.byref(g), i) for i in (0, 1))
+        self.fwd_scratch, self.bwd_scratch = (lib.vg_attention_workspace_bytes(ctypes.byref(g), i, int(q.dtype == BF16)) for i in (0, 1))
         self.lse_shape = (g.B, g.Hk, g.Tq * (g.Hq // g.Hk))
+        self.half = q.dtype == BF16
 
     def forward(self, q, k, v, q_lengths, k_lengths, o, save, stream):
-        """(q, k, v: addresses.) Writes o; returns the row sums' logarithms when `save`."""
+        """(q, k, v: addresses.) Writes o; returns what the backward pass needs besides it when `save`: the row sums'
+        logarithms and, of a bf16 o, what its rounding left."""
         lse = torch.empty(self.lse_shape, dtype=F32, device=o.device) if save else None
+        low = torch.empty_like(o) if save and self.half else None
         space = _scratch(self.fwd_scratch, o)
-        rc = self.fwd(self.geom, q, k, v, _at(q_lengths), _at(k_lengths), o.data_ptr(), _at(lse), _at(space), self.fwd_scratch, stream)
+        outs = (o.data_ptr(), _at(low), _at(lse)) if self.half else (o.data_ptr(), _at(lse))
+        rc = self.fwd(self.geom, q, k, v, _at(q_lengths), _at(k_lengths), *outs, _at(space), self.fwd_scratch, stream)
         if rc:
             _hip._check(rc, self.fwd_name)
-        return lse
+        return lse, low
 
-    def backward(self, q, k, v, o, lse, go, q_lengths, k_lengths, gq, gk, gv, stream):
+    def backward(self, q, k, v, o, lse, low, go, q_lengths, k_lengths, gq, gk, gv, stream):
         """(q, k, v, gq, gk, gv: addresses.)"""
         space = _scratch(self.bwd_scratch, o)
-        rc = self.bwd(self.geom, q, k, v, o.data_ptr(), lse.data_ptr(), go.data_ptr(), _at(q_lengths), _at(k_lengths), gq, gk, gv,
+        outs = (o.data_ptr(), _at(low), lse.data_ptr()) if self.half else (o.data_ptr(), lse.data_ptr())
+        rc = self.bwd(self.geom, q, k, v, *outs, go.data_ptr(), _at(q_lengths), _at(k_lengths), gq, gk, gv,
                       _at(space), self.bwd_scratch, stream)
         if rc:
             _hip._check(rc, self.bwd_name)
@@ -2157,15 +2162,15 @@ class AttentionFn(Function):
     def forward(ctx, q, k, v, q_lengths, k_lengths, plan):
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         with _on(q):
-            lse = plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, True, _raw_stream(q))
+            saved = plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, True, _raw_stream(q))
         ctx.plan = plan
-        ctx.save_for_backward(q, k, v, o, lse, q_lengths, k_lengths)
+        ctx.save_for_backward(q, k, v, o, *saved, q_lengths, k_lengths)
         return o
 
     @staticmethod
     @_first_order
     def backward(ctx, go):
-        q, k, v, o, lse, q_lengths, k_lengths = ctx.saved_tensors
+        q, k, v, o, lse, low, q_lengths, k_lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
         go = go.contiguous()
         gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need[0] else None
@@ -2173,7 +2178,7 @@ class AttentionFn(Function):
         if need[1] or need[2]:
             gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
         with _on(q):
-            ctx.plan.backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), o, lse, go, q_lengths, k_lengths, _at(gq), _at(gk), _at(gv),
+            ctx.plan.backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), o, lse, low, go, q_lengths, k_lengths, _at(gq), _at(gk), _at(gv),
                               _raw_stream(q))
         return gq, gk if need[1] else None, gv if need[2] else None, None, None, None
 
@@ -2227,22 +2232,22 @@ class _SelfAttentionPlan:
         with _on(qkv):
             stream = _raw_stream(qkv)
             self.rotary.forward(at, at + self.k_at, wq, wk, pos, yq, yk, stream)
-            lse = self.attention.forward(yq.data_ptr(), yk.data_ptr(), at + self.v_at, lengths, lengths, o, save, stream)
-        return yq, yk, o, lse
+            lse, low = self.attention.forward(yq.data_ptr(), yk.data_ptr(), at + self.v_at, lengths, lengths, o, save, stream)
+        return yq, yk, o, lse, low
 
 
 class SelfAttentionFn(Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, pos, lengths, plan):
-        yq, yk, o, lse = plan.forward(qkv, wq, wk, pos, lengths, True)
+        yq, yk, o, lse, low = plan.forward(qkv, wq, wk, pos, lengths, True)
         ctx.plan, ctx.label = plan, grads.ticket()
-        ctx.save_for_backward(qkv, wq, wk, pos, yq, yk, o, lse, lengths)
+        ctx.save_for_backward(qkv, wq, wk, pos, yq, yk, o, lse, low, lengths)
         return o
 
     @staticmethod
     @_first_order
     def backward(ctx, go):
-        qkv, wq, wk, pos, yq, yk, o, lse, lengths = ctx.saved_tensors
+        qkv, wq, wk, pos, yq, yk, o, lse, low, lengths = ctx.saved_tensors
         plan, lab, need = ctx.plan, ctx.label, ctx.needs_input_grad
         go = go.contiguous()
         gqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
@@ -2251,7 +2256,7 @@ class SelfAttentionFn(Function):
         at, gat = qkv.data_ptr(), gqkv.data_ptr()
         with _on(qkv):
             stream = _raw_stream(qkv)
-            plan.attention.backward(yq.data_ptr(), yk.data_ptr(), at + plan.v_at, o, lse, go, lengths, lengths, gyq.data_ptr(),
+            plan.attention.backward(yq.data_ptr(), yk.data_ptr(), at + plan.v_at, o, lse, low, go, lengths, lengths, gyq.data_ptr(),
                                     gyk.data_ptr(), gat + plan.gv_at, stream)
             gwq, gwk = plan.rotary.backward(at, at + plan.k_at, wq, wk, pos, gyq, gyk, gat, gat + plan.gk_at,
                                             (params and need[1], params and need[2]), stream)

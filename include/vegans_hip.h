@@ -500,6 +500,7 @@ int vg_qk_norm_rotary_bwd_h(const vg_rotary_geom* g, const void* q, const void* 
  * nullable (all): queries and keys at or past them take no part and may hold anything; rows without a key, and rows past
  * q_len, are zero, as are the gradients of everything that takes no part. Lengths outside 0..T are clamped. lse [B][Hk]
  * [Tq * Hq / Hk] f32 (log2 of the row sums; nullable in the forward pass) is what the backward pass needs besides o.
+ * bf16: o_low [B][Tq][Hq][D] (dense, nullable) is what the rounding of o left; with it the backward pass loses nothing to it.
  * Backward: gq, and gk with gv, may be null (not wanted).
  * D is a multiple of 8 up to 128; scale is finite and not zero. */
 typedef struct vg_attention_geom {
@@ -507,17 +508,17 @@ typedef struct vg_attention_geom {
   float scale;
   vg_heads_layout q, k, v, o, go, gq, gk, gv;
 } vg_attention_geom;
-size_t vg_attention_workspace_bytes(const vg_attention_geom* g, int backward);
+size_t vg_attention_workspace_bytes(const vg_attention_geom* g, int backward, int half);
 int vg_attention_fwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const int32_t* q_len, const int32_t* k_len,
                      float* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 int vg_attention_fwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len,
-                       void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+                       void* o, void* o_low, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 int vg_attention_bwd(const vg_attention_geom* g, const float* q, const float* k, const float* v, const float* o, const float* lse,
                      const float* go, const int32_t* q_len, const int32_t* k_len, float* gq, float* gk, float* gv, void* workspace,
                      size_t workspace_bytes, void* stream);
-int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                       const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* workspace,
-                       size_t workspace_bytes, void* stream);
+int vg_attention_bwd_h(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const void* o_low,
+                       const float* lse, const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gated linear layer h[M][F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M][C], w [2F][C] (gate rows first), bias [2F] nullable.
  * fwd: z [M][2F] f32 nullable: the pre-activations, which the backward pass of the sizes that vg_gated_linear_keeps_z names

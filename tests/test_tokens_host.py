@@ -77,12 +77,12 @@ def test_attention_arguments_are_checked_before_any_launch():
                     (_attention(Tq=1 << 29, Hq=4), "too many"), (_attention(Tk=1 << 30), "too many"),
                     (_attention(B=1 << 20, Tq=1 << 14), "too many")):
         assert fwd(g) == -1 and word in _text(lib), _text(lib)
-        assert lib.vg_attention_workspace_bytes(ctypes.byref(g), 0) == 0
+        assert lib.vg_attention_workspace_bytes(ctypes.byref(g), 0, 0) == 0
     assert fwd(_attention(), q=None) == -1 and "null" in _text(lib)
     assert fwd(_attention(), q=ctypes.c_void_p(8)) == -1 and "16-byte" in _text(lib)
     # one query over many keys: the keys are split, and the partial results need space
     g = _attention(B=1, Tq=1, Tk=1 << 14)
-    need = lib.vg_attention_workspace_bytes(ctypes.byref(g), 0)
+    need = lib.vg_attention_workspace_bytes(ctypes.byref(g), 0, 0)
     assert need > 0
     assert fwd(g, ws=DUMMY, size=need - 1) == -3 and "are needed" in _text(lib)
     assert fwd(g, ws=ctypes.c_void_p(264), size=need) == -1 and "aligned" in _text(lib)

@@ -2373,3 +2373,51 @@ def gated_linear(x, w, bias=None, act="silu"):
     if not _recording(x, w, bias):
         return plan.forward(*_gated_operands(x, w), bias, code, False)[0]
     return _recorded(GatedLinearFn.apply(x, w, bias, code, plan))
+
+
+class TokensFn(Function):
+    """[N, C, H, W] -> [N * H * W, C]: the feature map's memory as it lies (NHWC)."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.shape = tuple(x.shape)
+        n, c, h, w = x.shape
+        return to_nhwc(x).permute(0, 2, 3, 1).reshape(n * h * w, c)
+
+    @staticmethod
+    def backward(ctx, g):
+        return FeatureMapFn.apply(g, ctx.shape)
+
+
+class FeatureMapFn(Function):
+    """[N * H * W, C] -> [N, C, H, W] (NHWC memory)."""
+
+    @staticmethod
+    def forward(ctx, t, shape):
+        n, c, h, w = shape
+        return to_nhwc(t).view(n, h, w, c).permute(0, 3, 1, 2)
+
+    @staticmethod
+    def backward(ctx, g):
+        return TokensFn.apply(g), None
+
+
+def tokens(x):
+    """The pixels of feature map x [N, C, H, W] as rows [N * H * W, C] (no copy of an NHWC map)."""
+    return TokensFn.apply(x)
+
+
+def feature_map(t, shape):
+    """Rows [N * H * W, C] as a feature map of `shape` (N, C, H, W) (no copy)."""
+    return FeatureMapFn.apply(t, tuple(shape))
+
+
+def add(a, b):
+    """a + b of two activations of one shape, in the storage type of a."""
+    return AddFn.apply(a, b if b.dtype == a.dtype else CastFn.apply(b, a.dtype))
+
+
+def as_feature(x):
+    """Rows x in the type the engine stores activations of that many channels in."""
+    kind = _feature_dtype(x.shape[1])
+    return x if x.dtype == kind else CastFn.apply(x, kind)

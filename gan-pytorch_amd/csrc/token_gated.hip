@@ -271,20 +271,25 @@ __global__ void __launch_bounds__(64 * kFewWaves) gated_few_kernel(const GatedPa
 #pragma unroll
         for (int i = 0; i < 8; ++i) b[n][i] = S::whole(reinterpret_cast<const char*>(x[n] + k + i * V));
     } else {
+      auto first = [&](const T* at, int left) {
+        const char* c = reinterpret_cast<const char*>(at);
+        return p.C >= V ? S::first(c, left) : S::part(c, left);
+      };
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int left = p.C - k - h * HALF - i * V;
-        a[i] = left >= V ? S::whole(reinterpret_cast<const char*>(w + k + i * V)) : S::part(reinterpret_cast<const char*>(w + k + i * V), left);
+        a[i] = first(w + k + i * V, left);
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-          b[n][i] = left >= V ? S::whole(reinterpret_cast<const char*>(x[n] + k + i * V))
-                              : S::part(reinterpret_cast<const char*>(x[n] + k + i * V), left);
+        for (int n = 0; n < NB; ++n) b[n][i] = first(x[n] + k + i * V, left);
       }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int n = 0; n < NB; ++n) acc[n] = tok_mma(__builtin_bit_cast(Frag, a[i]), __builtin_bit_cast(Frag, b[n][i]), acc[n]);
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < tok_parts<T>(); ++e)
+          acc[n] = tok_mma(__builtin_bit_cast(Frag, a[i]), __builtin_bit_cast(Frag, b[n][i]), acc[n], e);
   }
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -311,7 +316,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) gated_few_kernel(const GatedPa
   }
 }
 
-// [gg gu] from z and gh, elementwise; a block covers 256 columns (4 a thread, V = 4; 1 a thread: 64) and kRowsBlock rows
+// [gg gu] from z and gh, elementwise: V neighbouring columns a thread (one 16-byte vector of T, or 1 where the rows do not
+// start on 16-byte borders), 64 V columns and kRowsBlock rows a block. Bound by HBM: 8 + 3 sizeof(T) bytes an element.
 constexpr int kRowsBlock = 64;
 template <class T, int V>
 __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
@@ -322,26 +328,22 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
 #pragma unroll
   for (int e = 0; e < V; ++e) sg[e] = su[e] = 0.f;
   if (f < p.F) {
+#pragma unroll 2
     for (int m = r0 + rl; m < r1; m += 4) {
       const float* zg = p.z + (size_t)m * 2 * p.F + f;
       const T* gh = (const T*)p.gh + (size_t)m * p.F + f;
       float g[V], u[V], x[V], gg[V], gu[V];
-      if constexpr (V == 4) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(zg), b = *reinterpret_cast<const f32x4*>(zg + p.F);
+      if constexpr (V > 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] = a[e];
-          u[e] = b[e];
+        for (int e = 0; e < V; e += 4) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(zg + e), b = *reinterpret_cast<const f32x4*>(zg + p.F + e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            g[e + k] = a[k];
+            u[e + k] = b[k];
+          }
         }
-        if constexpr (sizeof(T) == 4) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(gh);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = y[e];
-        } else {
-          const u32x2 y = *reinterpret_cast<const u32x2*>(gh);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(float, (unsigned)(e % 2 ? y[e / 2] & 0xffff0000u : y[e / 2] << 16));
-        }
+        tok_widen(*reinterpret_cast<const u32x4*>(gh), x);
       } else {
         g[0] = zg[0];
         u[0] = zg[p.F];
@@ -358,9 +360,9 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
       }
       T* out = (T*)p.gz + (size_t)m * 2 * p.F + f;
       for (int t = 0; t < p.terms; ++t) {
-        if constexpr (V == 4) {
-          tok_store4(out, gg[0], gg[1], gg[2], gg[3]);
-          tok_store4(out + p.F, gu[0], gu[1], gu[2], gu[3]);
+        if constexpr (V > 1) {
+          *reinterpret_cast<u32x4*>(out) = tok_narrow(gg);
+          *reinterpret_cast<u32x4*>(out + p.F) = tok_narrow(gu);
         } else {
           out[0] = (T)gg[0];
           out[p.F] = (T)gu[0];
@@ -387,6 +389,23 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
     if (ff < p.F)
       p.gb_part[(size_t)blockIdx.x * 2 * p.F + which * p.F + ff] =
           (red[which][0][col] + red[which][1][col]) + (red[which][2][col] + red[which][3][col]);
+  }
+}
+// gb = sum of the partial sums' rows, in a fixed order: 32 columns and 32 row lanes a block
+__global__ void __launch_bounds__(1024) gated_bias_kernel(const float* part, int rows, int n, float* gb) {
+  __shared__ float red[32][33];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + col;
+  float v = 0.f;
+  if (i < n) {
+#pragma unroll 8
+    for (int r = row; r < rows; r += 32) v += part[(size_t)r * n + i];
+  }
+  red[row][col] = v;
+  __syncthreads();
+  if (row == 0 && i < n) {
+#pragma unroll
+    for (int r = 1; r < 32; ++r) v += red[r][col];
+    gb[i] = v;
   }
 }
 
@@ -527,7 +546,8 @@ struct ProductPlan {
 };
 // A product with few tiles is split along k, each split into a slab of its own (f32), summed in order. With n blocks on
 // the busiest compute unit the time goes as n (K / splits + 128): 128 k for a block's start, its stores and its share of
-// the slab sum. No split under 256 k.
+// the slab sum. No split under 128 k (a block of few k is bound by the latency of its loads, one k-step after the other:
+// 1554 x 333 x 1001 in splits of 334 k 22 us, of 167 17).
 template <class T>
 ProductPlan product_plan(int M, int N, int K) {
   ProductPlan best = {128, 1, K};
@@ -535,7 +555,7 @@ ProductPlan product_plan(int M, int N, int K) {
   for (int tile = 128; tile <= (sizeof(T) == 2 ? 256 : 128); tile *= 2) {
     const long long tiles = (long long)ceil_div(M, tile) * ceil_div(N, tile);
     if (tile == 256 && (M < 256 || N < 256)) break;
-    for (int s = 1; s <= 64 && (s == 1 || K / s >= 256); ++s) {
+    for (int s = 1; s <= 64 && (s == 1 || K / s >= 128); ++s) {
       const long long n = (tiles * s + 255) / 256;
       const double t = (double)n * ((double)K / s + 128) * (tile == 256 ? kLarge : 1);
       if (t < least * (s > 1 ? 0.97 : 1.0)) {
@@ -607,8 +627,7 @@ int product(const void* a, int64_t lda, int terms, int64_t a_term, const void* b
 template <class T>
 bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 768; }
 
-// Scratch of the backward pass, one piece after the other: [gg gu], partial column sums and their reduction's scratch,
-// slabs of the two products (one after the other on one stream: they share the space).
+// Scratch of the backward pass, one piece after the other: [gg gu], partial column sums, slabs of the two products (one after the other on one stream: they share the space).
 // bf16: [gg gu] is rounded to bf16 for the two products; of the many roundings in a sum most averages out, and what stays
 // costs a result 0.4 of its own rounding. In a small call (under 2^19 of them) they are too few for that: there what the
 // rounding left is multiplied too, as a second term, at no visible cost.
@@ -616,7 +635,7 @@ template <class T>
 int gz_terms(int M, int F) { return sizeof(T) == 2 && (long long)M * 2 * F < (1 << 19) ? 2 : 1; }
 
 struct BwdSpace {
-  size_t gz, part, colsum, slabs, total;
+  size_t gz, part, slabs, total;
   int rows;          // of partial column sums
 };
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -626,8 +645,7 @@ BwdSpace bwd_space(int M, int C, int F) {
   s.rows = ceil_div(M, keeps_z<T>(M, C) ? kRowsBlock : large_tiles<T>(M, 2ll * F) ? 256 : 128);
   s.gz = 0;
   s.part = align256((size_t)M * 2 * F * sizeof(T) * gz_terms<T>(M, F));
-  s.colsum = s.part + align256((size_t)s.rows * 2 * F * 4);
-  s.slabs = s.colsum + align256(vg_colsum_workspace_bytes(s.rows, 2 * F));
+  s.slabs = s.part + align256((size_t)s.rows * 2 * F * 4);
   const int terms = gz_terms<T>(M, F);
   const size_t a = product_bytes<T>(M, C, 2 * F, terms), b = product_bytes<T>(2 * F, C, M, terms);
   s.total = s.slabs + (a > b ? a : b);
@@ -666,10 +684,11 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
   p.terms = gz_terms<T>(M, F);
   if (keeps_z<T>(M, C)) {
     p.z = const_cast<float*>(z);
-    const bool wide = F % 4 == 0 && vg_aligned16(z) && vg_aligned16(gh);
-    const dim3 grid(ceil_div(M, kRowsBlock), ceil_div(F, wide ? 256 : 64));
+    constexpr int V = TokNum<T>::V;
+    const bool wide = F % V == 0 && vg_aligned16(z) && vg_aligned16(gh);
+    const dim3 grid(ceil_div(M, kRowsBlock), ceil_div(F, wide ? 64 * V : 64));
     if (wide)
-      gated_bwd_kernel<T, 4><<<grid, 256, 0, st>>>(p);
+      gated_bwd_kernel<T, V><<<grid, 256, 0, st>>>(p);
     else
       gated_bwd_kernel<T, 1><<<grid, 256, 0, st>>>(p);
     VG_CHECK_LAUNCH("gated backward");
@@ -678,8 +697,8 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
     if (rc) return rc;
   }
   if (gb) {
-    rc = vg_colsum((const float*)(at + s.part), gb, s.rows, 2 * F, at + s.colsum, s.slabs - s.colsum, stream);
-    if (rc) return rc;
+    gated_bias_kernel<<<ceil_div(2ll * F, 32), 1024, 0, st>>>(p.gb_part, s.rows, 2 * F, gb);
+    VG_CHECK_LAUNCH("gated backward bias");
   }
   if (gx) {
     rc = product<T, false>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, at + s.slabs, s.total - s.slabs, st);

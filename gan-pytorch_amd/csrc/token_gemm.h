@@ -35,8 +35,7 @@ struct TokStage {
   u32x4 r[N];
   unsigned off[N];      // bytes from the base
   const char* base;     // first row of the operand (KC) or first row of the tile (RC), at the current k
-  unsigned ragged;      // RC: vectors of this thread that are not 16 bytes inside the operand's rows, one bit each
-  bool edge;            // ... of any thread of the block
+  bool edge;            // RC: vectors of the tile cross the operand's last row
 
   static __device__ __forceinline__ u32x4 whole(const char* p) {
     u32x4 v;
@@ -57,14 +56,12 @@ struct TokStage {
   }
   // rows row0.. of the operand, from k
   __device__ __forceinline__ void place(const TokOperand<T>& a, int row0, int k) {
-    ragged = 0;
     base = reinterpret_cast<const char*>(a.p + (RC ? k * a.ld + row0 : k + (a.split ? 0 : row0 * a.ld)));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = threadIdx.x + i * NT, lr = id / VPR, lv = (id % VPR) * V;
       if constexpr (RC) {
         const int left = a.rows - row0 - lv;
-        if (left < V && (left > 0 || a.rows - row0 < V)) ragged |= 1u << i;
         off[i] = (unsigned)(((int64_t)lr * a.ld + (left > 0 ? lv : 0)) * (int)sizeof(T));
       } else {
         int row = lr;
@@ -85,23 +82,40 @@ struct TokStage {
     for (int i = 0; i < N; ++i) r[i] = whole(base + off[i]);
     base += (RC ? BK * a.ld : BK) * (int64_t)sizeof(T);
   }
+  // The first `left` elements at p, zeros behind them: the 16 bytes that end with them, shifted down (`left` may be
+  // negative: zeros; the V elements before p + left are readable).
+  static __device__ __forceinline__ u32x4 first(const char* p, int left) {
+    const int s = left >= V ? 0 : left <= 0 ? V : V - left;
+    u32x4 w = whole(p + (left < V ? left - V : 0) * (int)sizeof(T));
+    const int bytes = s * (int)sizeof(T);
+    if (bytes & 4) w = u32x4{w[1], w[2], w[3], 0u};
+    if (bytes & 8) w = u32x4{w[2], w[3], 0u, 0u};
+    if (sizeof(T) == 2 && (bytes & 2))
+      w = u32x4{__builtin_amdgcn_alignbyte(w[1], w[0], 2), __builtin_amdgcn_alignbyte(w[2], w[1], 2), __builtin_amdgcn_alignbyte(w[3], w[2], 2),
+                w[3] >> 16};
+    return bytes >= 16 ? u32x4{0, 0, 0, 0} : w;
+  }
   // the k-step that starts at k, whatever lies outside
   __device__ __forceinline__ void load(const TokOperand<T>& a, int row0, int k, int kend) {
     if (k + BK <= kend && !edge) {
       load_inside(a);
       return;
     }
+    const bool roomy = RC ? a.rows >= V : kend >= V;       // a row has the 16 bytes that first() reads
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = threadIdx.x + i * NT, lr = id / VPR, lv = (id % VPR) * V;
-      int left;
       if constexpr (RC) {
-        left = k + lr < kend ? a.rows - row0 - lv : 0;
-        if (k + lr < kend && left <= 0 && !(ragged >> i & 1)) left = V;      // (clamped: its values are not used)
+        // (past the last row: what lies at the clamped offset, it is not used)
+        const int inside = a.rows - row0 - lv, left = k + lr < kend ? (inside > 0 ? inside : a.rows - row0) : 0;
+        if (left <= 0)
+          r[i] = u32x4{0, 0, 0, 0};
+        else
+          r[i] = roomy ? first(base + off[i], left) : part(base + off[i], left);
       } else {
-        left = kend - k - lv;
+        const int left = kend - k - lv;
+        r[i] = roomy ? first(base + off[i], left) : part(base + off[i], left);
       }
-      r[i] = left >= V ? whole(base + off[i]) : part(base + off[i], left);
     }
     base += (RC ? BK * a.ld : BK) * (int64_t)sizeof(T);
   }
@@ -136,13 +150,14 @@ struct TokStage {
   }
 };
 
-__device__ __forceinline__ f32x16 tok_mma(bf16x8 a, bf16x8 b, f32x16 c) {
+// One product of two fragments is kParts matrix instructions (f32: a fragment's 4 k, two at a time over the lane halves).
+template <class T>
+constexpr int tok_parts() { return sizeof(T) == 2 ? 1 : 4; }
+__device__ __forceinline__ f32x16 tok_mma(bf16x8 a, bf16x8 b, f32x16 c, int) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 tok_mma(f32x4 a, f32x4 b, f32x16 c) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-  return c;
+__device__ __forceinline__ f32x16 tok_mma(f32x4 a, f32x4 b, f32x16 c, int e) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
 }
 
 template <class T, bool ARC, bool BRC, int BM, int BN, int WM, int WN>
@@ -193,9 +208,11 @@ struct TokGemm {
           for (int j = 0; j < TN; ++j) fb[(s + 1) & 1][j] = SB::frag(tb, nw + 32 * j, s + 1, lane);
         }
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int e = 0; e < tok_parts<T>(); ++e)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = tok_mma(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = tok_mma(fa[s & 1][i], fb[s & 1][j], acc[i][j], e);
         if (s == 0) {
           T* next = smem + (buf ^ 1) * BUF;
           if constexpr (decltype(inside)::value) {

@@ -107,13 +107,12 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
     sq[e] = sk[e] = 0.f;
   }
   const float inv_d = 1.f / (float)g.D;
-  const long long tokens = (long long)g.B * g.T;
-  const long long stride = (long long)gridDim.x * 4 * p.wave_tokens;
+  const unsigned tokens = (unsigned)g.B * (unsigned)g.T, stride = gridDim.x * 4 * p.wave_tokens;
   const int q_steps = (g.Hq + p.hps - 1) / p.hps, steps = q_steps + (g.Hk + p.hps - 1) / p.hps;
-  for (long long base = ((long long)blockIdx.x * 4 + wid) * p.wave_tokens; base < tokens; base += stride) {
-    const long long token = base + sub;
+  for (unsigned base = (blockIdx.x * 4 + wid) * p.wave_tokens; base < tokens; base += stride) {
+    const unsigned token = base + sub;
     const bool tok = token < tokens;
-    const int b = tok ? (int)(token / g.T) : 0, t = tok ? (int)(token - (long long)b * g.T) : 0;
+    const int b = tok ? (int)(token / (unsigned)g.T) : 0, t = tok ? (int)(token - (unsigned)b * g.T) : 0;
     float c[V / 2], s[V / 2];
     for (int s0 = 0; s0 < steps; s0 += kUnroll) {
       u32x4 rx[kUnroll], rg[kUnroll];
@@ -232,6 +231,7 @@ __global__ void __launch_bounds__(1024) rotary_weight_kernel(const float* part, 
 int check_geom(const vg_rotary_geom* g, const void* pos) {
   VG_REQUIRE(g, "rotary: null geometry");
   VG_REQUIRE(g->B >= 0 && g->T >= 0 && g->Hq >= 1 && g->Hk >= 0, "rotary: bad sizes B=%d T=%d Hq=%d Hk=%d", g->B, g->T, g->Hq, g->Hk);
+  VG_REQUIRE((long long)g->B * g->T < (1ll << 31), "rotary: %lld tokens are too many", (long long)g->B * g->T);
   VG_REQUIRE(g->D >= 8 && g->D <= 256 && g->D % 8 == 0, "rotary: head width %d is not a multiple of 8 from 8 to 256", g->D);
   VG_REQUIRE(g->axes >= 0 && g->axes <= 4, "rotary: %d axes, 0 to 4 are supported", g->axes);
   VG_REQUIRE(g->axes == 0 || pos, "rotary: null positions");

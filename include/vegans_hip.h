@@ -474,7 +474,7 @@ typedef struct vg_heads_layout {
  *   pair (2i, 2i+1) turns by pos[b][t][a] * base^(-2i / width[a]); elements behind the sections are not turned.
  * pos: int32, or int64 where pos_wide, [B][T][axes], batch stride pos_sb elements (0: one grid for the whole batch).
  * Forward: inputs at layouts q, k, outputs at oq, ok. Backward: inputs at q, k, output gradients at gq, gk, input
- * gradients written at oq, ok; gwq, gwk [D] nullable. Hk may be 0. D is a multiple of 8 up to 256. */
+ * gradients written at oq, ok; gwq, gwk [D] nullable. Hk may be 0. D is a multiple of 8 up to 256; B T < 2^31. */
 typedef struct vg_rotary_geom {
   int32_t B, T, Hq, Hk, D;
   int32_t axes, width[4];
@@ -502,7 +502,8 @@ int vg_qk_norm_rotary_bwd_h(const vg_rotary_geom* g, const void* q, const void* 
  * [Tq * Hq / Hk] f32 (log2 of the row sums; nullable in the forward pass) is what the backward pass needs besides o.
  * bf16: o_low [B][Tq][Hq][D] (dense, nullable) is what the rounding of o left; with it the backward pass loses nothing to it.
  * Backward: gq, and gk with gv, may be null (not wanted).
- * D is a multiple of 8 up to 128; scale is finite and not zero. */
+ * D is a multiple of 8 up to 128; scale is finite and not zero; with G = Hq / Hk, (Tq G + 128) G < 2^32 and Tk < 2^30;
+ * strides between tokens stay under 2^30 / 66 bytes (gradients' and outputs': any). */
 typedef struct vg_attention_geom {
   int32_t B, Tq, Tk, Hq, Hk, D;
   float scale;

@@ -155,7 +155,7 @@ def _attention_case(case, dtype, seed=0):
         kl = torch.randint(0, tk + 1, (b,), generator=gen, dtype=torch.int32)
         kl[0] = max(1, tk // 3)
         if b > 1:
-            kl[-1] = 0                       # an element without keys
+            kl[-1] = -3                      # an element without keys (below zero: clamped)
             ql[0], kl[0] = tq, tk + 50       # beyond the tensor: clamped
     return q, k, v, ql, kl, go
 
@@ -388,6 +388,68 @@ def test_gated_f32_master_weight(gpu):
     assert torch.equal(h, h2)
     g, g2 = torch.autograd.grad(h, (xd, wd), gh.cuda()), torch.autograd.grad(h2, (xd, wh), gh.cuda())
     assert torch.equal(g[0], g2[0]) and g[1].dtype == F32 and torch.equal(g[1].to(BF16), g2[1])
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# beyond 32-bit offsets
+# ------------------------------------------------------------------------------------------------------------------
+def test_attention_over_a_cache_of_four_gigabytes(gpu):
+    """2^24 + 77 keys of 128 bf16: everything that counts lies in the last key and in one near the 2^31st element."""
+    n, d = (1 << 24) + 77, 128
+    k = torch.zeros(1, n, 1, d, dtype=BF16, device="cuda")
+    v = torch.zeros(1, n, 1, d, dtype=BF16, device="cuda")
+    q = torch.zeros(1, 3, 1, d, dtype=BF16, device="cuda")
+    q[0, :, 0, 0] = 16.0
+    places = (n - 1, (1 << 31) // d + 5)
+    for i, at in enumerate(places):
+        k[0, at, 0, 0] = 64.0                      # score 1024 / sqrt(128) = 90.5: all others together weigh 2^24 e^-90
+        v[0, at, 0, i] = 2.0
+    go = torch.ones(1, 3, 1, d, dtype=BF16, device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = _ops().attention(*leaves)
+    assert (o[0, :, 0, :2] == 1).all() and not o[0, :, 0, 2:].any()
+    gq, gk, gv = torch.autograd.grad(o, leaves, go)
+    for i, at in enumerate(places):
+        assert (gv[0, at, 0] == 1.5).all()         # three rows with weight 1/2 each
+    assert not gv[0, :1000].any() and gv.count_nonzero() == 2 * d
+    # go v^T is 2 at both places and delta is 2: no gradient of scores
+    assert not gq.any() and not gk.any()
+
+
+def test_strides_of_four_gigabytes(gpu):
+    """Batch elements 2^31 elements apart."""
+    store = torch.zeros((1 << 31) + 4096, dtype=BF16, device="cuda")
+    gen = torch.Generator().manual_seed(8)
+    x = _rand(gen, 2, 9, 4, 32, dtype=BF16).cuda()
+    far = store.as_strided((2, 9, 4, 32), (1 << 31, 128, 32, 1))
+    far.copy_(x)
+    ops, w, pos = _ops(), torch.ones(32, device="cuda"), torch.arange(9, device="cuda")[:, None]
+    with torch.no_grad():
+        assert torch.equal(ops.attention(far, far, far), ops.attention(x, x, x))
+        for a, b in zip(ops.qk_norm_rotary(far, far, w, w, pos, (32,)), ops.qk_norm_rotary(x, x, w, w, pos, (32,))):
+            assert torch.equal(a, b)
+
+
+def test_gated_rows_beyond_two_gigabytes(gpu):
+    """2^20 + 3 rows of 2 x 1100 pre-activations: the last rows are what they are alone."""
+    m, c, f = (1 << 20) + 3, 8, 1100
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(m, c, generator=gen, device="cuda").to(BF16).requires_grad_()
+    w = torch.randn(2 * f, c, generator=gen, device="cuda").to(BF16).requires_grad_()
+    gh = torch.randn(m, f, generator=gen, device="cuda").to(BF16)
+    h = _ops().gated_linear(x, w)
+    gx, gw = torch.autograd.grad(h, (x, w), gh)
+    last = slice(m - 300, m)
+    xl = x.detach()[last].clone().requires_grad_()
+    hl = _ops().gated_linear(xl, w)
+    (gxl,) = torch.autograd.grad(hl, xl, gh[last])
+    assert torch.equal(h[last], hl)
+    # the alone rows' products are split (and small enough for two terms): the same up to the roundings of [gg gu] and gx
+    want = oracle.gated(xl.detach().cpu().double(), w.detach().cpu().double(), None, "silu", gh[last].cpu().double())
+    for got in (gx[last], gxl):
+        allowed = (c + 2 * f + 32) * U32 * want["abs"]["gx"] + UBF * (1 + UBF) * want["gz_abs"]["gx"] + UBF * want["gx"].abs() * 1.01
+        _within(got, want["gx"], allowed, "gx")
+    assert torch.isfinite(gw).all()
 
 
 # ------------------------------------------------------------------------------------------------------------------

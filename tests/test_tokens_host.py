@@ -41,7 +41,7 @@ def test_rotary_arguments_are_checked_before_any_launch():
         return lib.vg_qk_norm_rotary_fwd(ctypes.byref(g), q, DUMMY, DUMMY, DUMMY, pos, DUMMY, DUMMY, None)
 
     for g, word in ((_rotary(D=12), "head width"), (_rotary(D=264), "head width"), (_rotary(axes=5), "axes"), (_rotary(Hq=0), "bad sizes"),
-                    (_rotary(T=-1), "bad sizes"), (_rotary(base=0.0), "base")):
+                    (_rotary(T=-1), "bad sizes"), (_rotary(B=1 << 16, T=1 << 15), "too many"), (_rotary(base=0.0), "base")):
         assert fwd(g) == -1 and word in _text(lib), _text(lib)
         assert lib.vg_qk_norm_rotary_workspace_bytes(ctypes.byref(g)) == 0
     g = _rotary()
@@ -87,6 +87,9 @@ def test_attention_arguments_are_checked_before_any_launch():
     assert fwd(g, ws=DUMMY, size=need - 1) == -3 and "are needed" in _text(lib)
     assert fwd(g, ws=ctypes.c_void_p(264), size=need) == -1 and "aligned" in _text(lib)
     assert fwd(_attention(B=0), q=None) == 0
+    g = _attention()
+    g.k.st = 1 << 26
+    assert fwd(g) == -1 and "stride" in _text(lib)
     rc = lib.vg_attention_bwd(ctypes.byref(_attention()), *[DUMMY] * 8, DUMMY, DUMMY, None, DUMMY, 1 << 20, None)
     assert rc == -1 and "null" in _text(lib)                 # keys' gradient without values'
     rc = lib.vg_attention_bwd(ctypes.byref(_attention()), *[DUMMY] * 8, DUMMY, DUMMY, DUMMY, None, 0, None)

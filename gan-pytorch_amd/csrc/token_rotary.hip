@@ -29,11 +29,10 @@ struct RotaryParams {
   double decay[4];        // log2 of the ratio of neighbouring elements' frequencies on an axis
 };
 
-constexpr int kUnroll = 4;          // head steps whose loads are in flight together
 // Blocks of four waves: as many as run at once (registers: four waves a SIMD forward, three backward), so that a wave's
 // start (frequencies in 64 bits) is spread over as many tokens as can be. Measured on 4 x 8192 tokens, 20 heads of 128, bf16
-// (336 MB forward, 503 MB backward): forward 1024 blocks 81 us (4.1 TB/s), 2048 86, 512 108; backward 768 blocks 128 us
-// (3.9 TB/s), 512 at two waves a SIMD 141.
+// (336 MB forward, 503 MB backward): forward 70 us (4.8 TB/s; half the blocks 94), backward 121 us (4.2 TB/s; half 163);
+// twice the blocks take the same.
 constexpr int kBlocks = 1024;
 constexpr int kBwdBlocks = 768;     // rows of partial weight-gradient sums at most
 
@@ -70,6 +69,8 @@ __device__ __forceinline__ float head_sum(float v, int lanes) {
 template <class T, bool BWD>
 __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryParams p) {
   constexpr int V = TokNum<T>::V;
+  constexpr int kUnroll = BWD ? 5 : 6;     // head steps whose loads are in flight together (what the registers hold)
+  __shared__ float weight[2][256];
   const vg_rotary_geom& g = p.g;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int lh = lane & (p.lph - 1);                   // lane in the head
@@ -99,13 +100,15 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
     freq[i] = g.axes ? exp2(e) * 0.15915494309189533577 : 0.0;
     if (!in) axis[i] = -1;
   }
-  float wq[V], wk[V], sq[V], sk[V];                    // weights, and (backward) sums of their gradients
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    wq[e] = in && p.wq ? p.wq[d0 + e] : 1.f;
-    wk[e] = in && p.wk ? p.wk[d0 + e] : 1.f;
-    sq[e] = sk[e] = 0.f;
+  {
+    const int d = threadIdx.x;
+    weight[0][d] = d < g.D && p.wq ? p.wq[d] : 1.f;
+    weight[1][d] = d < g.D && p.wk ? p.wk[d] : 1.f;
   }
+  __syncthreads();
+  float sq[V], sk[V];                                  // (backward) sums of the weights' gradients
+#pragma unroll
+  for (int e = 0; e < V; ++e) sq[e] = sk[e] = 0.f;
   const float inv_d = 1.f / (float)g.D;
   const unsigned tokens = (unsigned)g.B * (unsigned)g.T, stride = gridDim.x * 4 * p.wave_tokens;
   const int q_steps = (g.Hq + p.hps - 1) / p.hps, steps = q_steps + (g.Hk + p.hps - 1) / p.hps;
@@ -139,8 +142,10 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
         const bool ok = tok && in && h < (isq ? g.Hq : g.Hk);
         const vg_heads_layout& lo = isq ? g.oq : g.ok;
         T* out = (T*)(isq ? p.oq : p.ok) + b * lo.sb + t * lo.st + h * lo.sh + d0;
-        auto one = [&](const float (&w)[V], bool normed, float (&sum)[V]) {
-          float xv[V], y[V];
+        auto one = [&](int which, bool normed, float (&sum)[V]) {
+          float xv[V], y[V], w[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) w[e] = weight[which][d0 + e];
           tok_widen(rx[u], xv);
           float r = 1.f;
           if (normed) {
@@ -181,9 +186,9 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
           if (ok) *reinterpret_cast<u32x4*>(out) = tok_narrow(y);
         };
         if (isq)
-          one(wq, p.wq != nullptr, sq);
+          one(0, p.wq != nullptr, sq);
         else
-          one(wk, p.wk != nullptr, sk);
+          one(1, p.wk != nullptr, sk);
       }
     }
   }

@@ -2053,7 +2053,7 @@ class QkNormRotaryFn(Function):
         q, k, wq, wk, pos = ctx.saved_tensors
         lab, need = ctx.label, ctx.needs_input_grad
         gyq, gyk = gyq.contiguous(), gyk.contiguous()
-        gq, gk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        gq, gk = q.new_empty(q.shape), k.new_empty(k.shape)
         params = not inputs_only.active
         with _on(q):
             gwq, gwk = ctx.plan.backward(q.data_ptr(), k.data_ptr(), wq, wk, pos, gyq, gyk, gq.data_ptr(), gk.data_ptr(),
@@ -2063,7 +2063,7 @@ class QkNormRotaryFn(Function):
 
 
 def _rotate(plan, q, k, wq, wk, pos):
-    yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
     with _on(q):
         plan.forward(q.data_ptr(), k.data_ptr(), wq, wk, pos, yq, yk, _raw_stream(q))
     return yq, yk
@@ -2160,7 +2160,7 @@ def _check_lengths(n, q, what):
 class AttentionFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, q_lengths, k_lengths, plan):
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o = q.new_empty(q.shape)
         with _on(q):
             saved = plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, True, _raw_stream(q))
         ctx.plan = plan
@@ -2173,10 +2173,10 @@ class AttentionFn(Function):
         q, k, v, o, lse, low, q_lengths, k_lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
         go = go.contiguous()
-        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need[0] else None
+        gq = q.new_empty(q.shape) if need[0] else None
         gk = gv = None
         if need[1] or need[2]:
-            gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+            gk, gv = (k.new_empty(k.shape) for _ in range(2))
         with _on(q):
             ctx.plan.backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), o, lse, low, go, q_lengths, k_lengths, _at(gq), _at(gk), _at(gv),
                               _raw_stream(q))
@@ -2201,7 +2201,7 @@ def attention(q, k, v, q_lengths=None, k_lengths=None, scale=None):
     _check_lengths(q_lengths, q, "q_lengths")
     _check_lengths(k_lengths, q, "k_lengths")
     if not _recording(q, k, v):
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o = q.new_empty(q.shape)
         with _on(q):
             plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, False, _raw_stream(q))
         return o

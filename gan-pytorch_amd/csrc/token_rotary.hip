@@ -31,8 +31,9 @@ struct RotaryParams {
 
 // Blocks of four waves: as many as run at once (registers: four waves a SIMD forward, three backward), so that a wave's
 // start (frequencies in 64 bits) is spread over as many tokens as can be. Measured on 4 x 8192 tokens, 20 heads of 128, bf16
-// (336 MB forward, 503 MB backward): forward 70 us (4.8 TB/s; half the blocks 94), backward 121 us (4.2 TB/s; half 163);
-// twice the blocks take the same.
+// (336 MB forward, 503 MB backward): forward 67 us (5.0 TB/s; half the blocks 94), backward 106 us (4.8 TB/s; half 163);
+// twice the blocks take the same. The outputs are written past the caches, which leaves those to the reads: 70 and 119 us
+// without; 3 x 777 tokens of 8 heads of 72 in f32 (27 MB both ways) take 8 + 11 us so, 10 + 12 without.
 constexpr int kBlocks = 1024;
 constexpr int kBwdBlocks = 768;     // rows of partial weight-gradient sums at most
 
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
               for (int e = 0; e < V; ++e) y[e] = r * __builtin_fmaf(-xv[e], inner, y[e]);
             }
           }
-          if (ok) *reinterpret_cast<u32x4*>(out) = tok_narrow(y);
+          if (ok) __builtin_nontemporal_store(tok_narrow(y), reinterpret_cast<u32x4*>(out));
         };
         if (isq)
           one(0, p.wq != nullptr, sq);

@@ -104,23 +104,43 @@ __device__ __forceinline__ void load16(const T* p, int n, float (&v)[16]) {
     for (int e = 0; e < 16; ++e) v[e] = e < n ? (float)p[e] : 0.f;
   }
 }
-template <class T>
-__device__ __forceinline__ void store16(T* p, int n, const float (&v)[16]) {
-  constexpr int V = TokNum<T>::V;
-  if (n >= 16) {
+// A 32 x 32 tile of a result, `rows` x `cols` of it inside. A lane holds 16 neighbouring columns of row lane % 32: stored
+// from there, every lane of a 16-byte store would be in a line of its own. The wave turns the tile in LDS (its own kTurn
+// floats) and stores whole runs of 128 bytes (f32) or 64 (bf16): 16384 x 1024 x 4096 with z (671 MB of results) 565 -> 490
+// us, 4096 x 512 x 1408 in f32 132 -> 121.
+constexpr int kTurnLd = 36, kTurn = 32 * kTurnLd;
+template <class O>
+__device__ __forceinline__ void store_tile(float* mine, O* out, size_t ld, int rows, int cols, const float (&v)[16], int lane) {
+  constexpr int V = TokNum<O>::V, LANES = 32 / V;      // lanes of a row
 #pragma unroll
-    for (int i = 0; i < 16 / V; ++i) {
-      float f[V];
+  for (int e = 0; e < 16; e += 4)
+    *reinterpret_cast<f32x4*>(mine + (lane & 31) * kTurnLd + 16 * (lane >> 5) + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const int r0 = lane / LANES, col = lane % LANES * V;
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = v[i * V + e];
-      const u32x4 raw = tok_narrow(f);
-      __builtin_memcpy(p + i * V, &raw, 16);
+  for (int r = r0; r < 32 + r0; r += 64 / LANES) {
+    float f[V];
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(mine + r * kTurnLd + col + e);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[e + k] = a[k];
     }
-  } else {
+    O* to = out + (size_t)r * ld + col;
+    if (r < rows) {
+      if (col + V <= cols) {
+        const u32x4 raw = tok_narrow(f);
+        __builtin_memcpy(to, &raw, 16);
+      } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (e < n) p[e] = (T)v[e];
+        for (int e = 0; e < V; ++e)
+          if (col + e < cols) to[e] = (O)f[e];
+      }
+    }
   }
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Tile order: runs of kGroup row tiles walk the column tiles together, so that the tiles in flight on an XCD share rows of
@@ -149,6 +169,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gated_kernel(const 
   constexpr int LDR = 68;                                       // a lane column of partial sums, padded
   float* red = reinterpret_cast<float*>(smem_raw);              // [wave][32][LDR], then [WN][BF] sums behind it
   float* total = red + WM * WN * 32 * LDR;
+  float* mine = red + wid * 32 * LDR;                           // the wave's own space: no barrier needed
+  static_assert(kTurn <= 32 * LDR, "a tile to be turned fits it");
   static_assert((WM * WN * 32 * LDR + WN * BF) * 4 <= G::LDS_BYTES, "the sums fit the tiles' space");
 #pragma unroll
   for (int i = 0; i < G::TM; i += 2) {
@@ -162,52 +184,53 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gated_kernel(const 
     }
 #pragma unroll
     for (int j = 0; j < G::TN; ++j) {
-      const int m = m0 + (wn * G::TN + j) * 32 + c;
-      if (m < p.M && left > 0) {
-        float g[16], u[16], gg[16], gu[16];
-        [[maybe_unused]] float x[16];
-        const size_t at = (size_t)m * p.F + f, at2 = (size_t)m * 2 * p.F + f;
-        if constexpr (BWD) load16((const T*)p.gh + at, left, x);
+      const int mt0 = m0 + (wn * G::TN + j) * 32, m = mt0 + c, ft = f - 16 * h, rows = p.M - mt0, cols = p.F - ft;
+      if (rows <= 0 || cols <= 0) continue;      // uniform
+      const bool ok = m < p.M && left > 0;
+      float g[16], u[16], gg[16], gu[16];
+      [[maybe_unused]] float x[16];
+      const size_t at = (size_t)mt0 * p.F + ft, at2 = (size_t)mt0 * 2 * p.F + ft;
+      if constexpr (BWD) load16((const T*)p.gh + (size_t)m * p.F + f, ok ? left : 0, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          g[e] = acc[i][j][e] + bg[e];
-          u[e] = acc[i + 1][j][e] + bu[e];
-          float a, d;
-          gate_both<sizeof(T) == 2>(g[e], p.act, a, d);
-          if constexpr (BWD) {
-            gg[e] = x[e] * u[e] * d;
-            gu[e] = x[e] * a;
+      for (int e = 0; e < 16; ++e) {
+        g[e] = acc[i][j][e] + bg[e];
+        u[e] = acc[i + 1][j][e] + bu[e];
+        float a, d;
+        gate_both<sizeof(T) == 2>(g[e], p.act, a, d);
+        if constexpr (BWD) {
+          gg[e] = x[e] * u[e] * d;
+          gu[e] = x[e] * a;
+          if (ok) {
             sg[e] += gg[e];
             su[e] += gu[e];
-          } else {
-            gg[e] = a * u[e];
-          }
-        }
-        if constexpr (BWD) {
-          store16((T*)p.gz + at2, left, gg);
-          store16((T*)p.gz + at2 + p.F, left, gu);
-          if (sizeof(T) == 2 && p.terms == 2) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              gg[e] -= (float)(T)gg[e];
-              gu[e] -= (float)(T)gu[e];
-            }
-            T* low = (T*)p.gz + (size_t)p.M * 2 * p.F + at2;
-            store16(low, left, gg);
-            store16(low + p.F, left, gu);
           }
         } else {
-          store16((T*)p.h + at, left, gg);
-          if (p.z) {
-            store16(p.z + at2, left, g);
-            store16(p.z + at2 + p.F, left, u);
+          gg[e] = a * u[e];
+        }
+      }
+      if constexpr (BWD) {
+        store_tile(mine, (T*)p.gz + at2, 2 * p.F, rows, cols, gg, lane);
+        store_tile(mine, (T*)p.gz + at2 + p.F, 2 * p.F, rows, cols, gu, lane);
+        if (sizeof(T) == 2 && p.terms == 2) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            gg[e] -= (float)(T)gg[e];
+            gu[e] -= (float)(T)gu[e];
           }
+          T* low = (T*)p.gz + (size_t)p.M * 2 * p.F + at2;
+          store_tile(mine, low, 2 * p.F, rows, cols, gg, lane);
+          store_tile(mine, low + p.F, 2 * p.F, rows, cols, gu, lane);
+        }
+      } else {
+        store_tile(mine, (T*)p.h + at, p.F, rows, cols, gg, lane);
+        if (p.z) {
+          store_tile(mine, p.z + at2, 2 * p.F, rows, cols, g, lane);
+          store_tile(mine, p.z + at2 + p.F, 2 * p.F, rows, cols, u, lane);
         }
       }
     }
     if constexpr (BWD) {
-      if (p.gb_part) {       // column sums: the wave's 32 rows of x in a fixed order (its own space: no barrier needed)
-        float* mine = red + wid * 32 * LDR;
+      if (p.gb_part) {       // column sums: the wave's 32 rows of x in a fixed order
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           *reinterpret_cast<f32x4*>(mine + c * LDR + 32 * h + e) = f32x4{sg[e], sg[e + 1], sg[e + 2], sg[e + 3]};
@@ -504,7 +527,7 @@ int check_sizes(int M, int C, int F, int act) {
 // Products are cut into 256 x 256 tiles (bf16: eight waves of 128 x 64, one block a CU) or 128 x 128 (two blocks a CU). The
 // large tile reads its operands half as often from the caches and takes 0.65 of the time of four small ones (16384 x 1024
 // x 8192: 284 us against 416); the small one wins where too few large ones are there for 256 compute units. f32 products
-// are bound by the matrix cores with either and take the small one, by eight waves of 64 x 32 (132 us against 139 with four
+// are bound by the matrix cores with either and take the small one, by eight waves of 64 x 32 (before the results were turned, 132 us against 139 with four
 // of 64 x 64, 4096 x 512 x 2816).
 constexpr double kLarge = 4 * 0.65;
 template <class T>
@@ -640,10 +663,11 @@ int product(const void* a, int64_t lda, int terms, int64_t a_term, const void* b
 }
 
 // What the backward pass of these sizes runs on: pre-activations kept by the forward pass in f32 (8 bytes written and read
-// an element), or, with bf16 operands, computed again. 16384 x C x 4096, forward and backward: C = 256 623 us again, 742
-// kept; 512 829 and 884; 1024 1249 and 1198. (Up to 64 rows the forward kernel has no backward twin.)
+// an element), or, with bf16 operands, computed again. Forward and backward, again / kept: 16384 x C x 4096: C = 256 622 /
+// 651 us, 512 814 / 782, 768 1168 / 1079, 1024 1242 / 1107; 16384 x C x 1024: 256 184 / 209, 512 236 / 256, 768 375 / 353,
+// 1024 352 / 329. (Up to 64 rows the forward kernel has no backward twin.)
 template <class T>
-bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 768; }
+bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 512; }
 
 // Scratch of the backward pass, one piece after the other: [gg gu], partial column sums, slabs of the two products (one after the other on one stream: they share the space).
 // bf16: [gg gu] is rounded to bf16 for the two products; of the many roundings in a sum most averages out, and what stays

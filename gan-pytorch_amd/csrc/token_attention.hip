@@ -17,6 +17,12 @@
 // they are, if the keys of a k-slice are numbered in the order in which the lane holds them - which only says which
 // rows of V the A operand reads. bf16 reads them with the transposing LDS load (4 keys of one column per lane), f32 with
 // 4-byte loads. Queries' gradients use the same shape; the gradients of keys and values its mirror image (column = key).
+//
+// Bound by the SIMDs: the vector instructions of the softmax (one exponential, two to four others an element) add to the
+// matrix instructions instead of hiding under them, so heads of 128 come nearer the matrix rate than heads of 64. Measured,
+// bf16: 8192 queries and keys, 2 x 16 query and 4 key heads of 128 ("the long case" below) forward 1.20 ms (0.92 PFLOP/s; a
+// library product of 8192^3 reaches 1.28), backward 3.61 ms (0.76 on its five products, 1.07 with the two that both walks
+// rebuild); 1024 queries and keys, 8 x 16 heads of 64 59 and 149 us (0.58 PFLOP/s both).
 #include <float.h>
 #include <math.h>
 
@@ -466,7 +472,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p, flo
 }
 
 // Queries' gradient: the forward kernel's walk with p rebuilt from lse. Heads of 128 take their keys 32 at a time (fewer
-// staging registers: at 64 the kernel spills, video case 1993 us).
+// staging registers: at 64 the kernel spills).
 template <class T, int DP>
 struct GqTiles {
   static constexpr int KT = DP >= 128 ? 32 : tile_len<T, DP>();
@@ -557,7 +563,8 @@ __device__ __forceinline__ void queries_gradient(const AttnParams& p, int id, Gq
 
 // Gradients of keys and values: a block owns kTileRows keys (32 a wave, in registers) and walks the problem's rows. bf16
 // heads of 128: the values of the block's keys stay in LDS instead and the rows come 32 at a time, which brings the kernel
-// under 256 registers, i.e. to two waves a SIMD (video case 3138 us with all in registers, 2350 so).
+// under 256 registers, i.e. to two waves a SIMD (this walk of the long case: 3138 us with
+// all in registers, 2350 so).
 template <class T, int DP>
 constexpr int row_len() {
   return sizeof(T) == 2 && DP < 128 ? 64 : 32;
@@ -910,8 +917,8 @@ int attention_fwd(const vg_attention_geom* g, const void* q, const void* k, cons
 }
 
 template <class T>
-int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const void* low, const float* lse, const void* go,
-                  const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* ws, size_t ws_bytes, void* stream) {
+int attention_bwd(const vg_attention_geom* g, const void* q, const void* k, const void* v, const void* o, const void* low,
+                  const float* lse, const void* go, const int32_t* q_len, const int32_t* k_len, void* gq, void* gk, void* gv, void* ws, size_t ws_bytes, void* stream) {
   const int rc = check_geom(g);
   if (rc) return rc;
   const Plan pl = plan_of<T>(g);

@@ -1853,9 +1853,12 @@ class _FirstOrderFn(Function):
 # instead. (Inside a training iteration the gradient ledger takes the parameters' gradients and no such node runs.)
 def _recorded(out):
     """`out` (a tensor, or several of one operator) after its operator was recorded: marks the accumulation nodes of leaves."""
+    captured = None
     for node, _ in (out if torch.is_tensor(out) else out[0]).grad_fn.next_functions:
         if type(node) is _AccumulateGrad:
-            node.metadata.setdefault("vg_captured", torch.cuda.is_current_stream_capturing())
+            if captured is None:
+                captured = torch.cuda.is_current_stream_capturing()
+            node.metadata.setdefault("vg_captured", captured)
     return out
 
 
@@ -1925,6 +1928,11 @@ def _raw_stream(t):
 def _scratch(nbytes, like):
     """Buffer of `nbytes` for one call (None for none)."""
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _new_dense(t):
+    """New tensor of the shape and type of `t`, dense whatever the strides of `t` are."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _at(t):
@@ -2053,7 +2061,7 @@ class QkNormRotaryFn(Function):
         q, k, wq, wk, pos = ctx.saved_tensors
         lab, need = ctx.label, ctx.needs_input_grad
         gyq, gyk = gyq.contiguous(), gyk.contiguous()
-        gq, gk = q.new_empty(q.shape), k.new_empty(k.shape)
+        gq, gk = _new_dense(q), _new_dense(k)
         params = not inputs_only.active
         with _on(q):
             gwq, gwk = ctx.plan.backward(q.data_ptr(), k.data_ptr(), wq, wk, pos, gyq, gyk, gq.data_ptr(), gk.data_ptr(),
@@ -2063,7 +2071,7 @@ class QkNormRotaryFn(Function):
 
 
 def _rotate(plan, q, k, wq, wk, pos):
-    yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
+    yq, yk = _new_dense(q), _new_dense(k)
     with _on(q):
         plan.forward(q.data_ptr(), k.data_ptr(), wq, wk, pos, yq, yk, _raw_stream(q))
     return yq, yk
@@ -2132,7 +2140,7 @@ class _AttentionPlan:
     def forward(self, q, k, v, q_lengths, k_lengths, o, save, stream):
         """(q, k, v: addresses.) Writes o; returns what the backward pass needs besides it when `save`: the row sums'
         logarithms and, of a bf16 o, what its rounding left."""
-        lse = torch.empty(self.lse_shape, dtype=F32, device=o.device) if save else None
+        lse = o.new_empty(self.lse_shape, dtype=F32) if save else None
         low = torch.empty_like(o) if save and self.half else None
         space = _scratch(self.fwd_scratch, o)
         outs = (o.data_ptr(), _at(low), _at(lse)) if self.half else (o.data_ptr(), _at(lse))
@@ -2160,7 +2168,7 @@ def _check_lengths(n, q, what):
 class AttentionFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, q_lengths, k_lengths, plan):
-        o = q.new_empty(q.shape)
+        o = _new_dense(q)
         with _on(q):
             saved = plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, True, _raw_stream(q))
         ctx.plan = plan
@@ -2173,10 +2181,10 @@ class AttentionFn(Function):
         q, k, v, o, lse, low, q_lengths, k_lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
         go = go.contiguous()
-        gq = q.new_empty(q.shape) if need[0] else None
+        gq = _new_dense(q) if need[0] else None
         gk = gv = None
         if need[1] or need[2]:
-            gk, gv = (k.new_empty(k.shape) for _ in range(2))
+            gk, gv = _new_dense(k), _new_dense(k)
         with _on(q):
             ctx.plan.backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), o, lse, low, go, q_lengths, k_lengths, _at(gq), _at(gk), _at(gv),
                               _raw_stream(q))
@@ -2201,7 +2209,7 @@ def attention(q, k, v, q_lengths=None, k_lengths=None, scale=None):
     _check_lengths(q_lengths, q, "q_lengths")
     _check_lengths(k_lengths, q, "k_lengths")
     if not _recording(q, k, v):
-        o = q.new_empty(q.shape)
+        o = _new_dense(q)
         with _on(q):
             plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, False, _raw_stream(q))
         return o
@@ -2226,8 +2234,7 @@ class _SelfAttentionPlan:
         self.gk_at, self.gv_at = (h * d * size for h in (heads, heads + kv_heads))
 
     def forward(self, qkv, wq, wk, pos, lengths, save):
-        new = lambda shape: torch.empty(shape, dtype=qkv.dtype, device=qkv.device)  # noqa: E731
-        yq, yk, o = new(self.q_shape), new(self.k_shape), new(self.q_shape)
+        yq, yk, o = qkv.new_empty(self.q_shape), qkv.new_empty(self.k_shape), qkv.new_empty(self.q_shape)
         at = qkv.data_ptr()
         with _on(qkv):
             stream = _raw_stream(qkv)
@@ -2250,7 +2257,7 @@ class SelfAttentionFn(Function):
         qkv, wq, wk, pos, yq, yk, o, lse, low, lengths = ctx.saved_tensors
         plan, lab, need = ctx.plan, ctx.label, ctx.needs_input_grad
         go = go.contiguous()
-        gqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        gqkv = _new_dense(qkv)
         gyq, gyk = torch.empty_like(yq), torch.empty_like(yk)
         params = not inputs_only.active
         at, gat = qkv.data_ptr(), gqkv.data_ptr()
@@ -2303,8 +2310,8 @@ class _GatedPlan:
 
     def forward(self, x, w, bias, act, save):
         """Returns the output and, when `save` and the backward pass wants them, the pre-activations."""
-        h = torch.empty((self.m, self.f), dtype=x.dtype, device=x.device)
-        z = torch.empty((self.m, 2 * self.f), dtype=F32, device=x.device) if save and self.keeps_z else None
+        h = x.new_empty((self.m, self.f))
+        z = x.new_empty((self.m, 2 * self.f), dtype=F32) if save and self.keeps_z else None
         with _on(x):
             rc = self.fwd(self.m, self.c, self.f, x.data_ptr(), w.data_ptr(), _at(bias), h.data_ptr(), _at(z), act, _raw_stream(x))
             if rc:
@@ -2339,10 +2346,9 @@ class GatedLinearFn(Function):
         plan, lab, need = ctx.plan, ctx.label, ctx.needs_input_grad
         gh = _cast_raw(gh.contiguous(), xm.dtype)
         params = not inputs_only.active
-        dev = xm.device
-        gx = torch.empty((plan.m, plan.c), dtype=xm.dtype, device=dev) if _wants_input_grad(ctx, x) else None
-        gw = torch.empty((2 * plan.f, plan.c), dtype=w.dtype, device=dev) if params and need[1] else None
-        gb = torch.empty(2 * plan.f, dtype=F32, device=dev) if params and bias is not None and need[2] else None
+        gx = torch.empty_like(xm) if _wants_input_grad(ctx, x) else None
+        gw = torch.empty_like(wm, dtype=w.dtype) if params and need[1] else None
+        gb = torch.empty_like(bias) if params and bias is not None and need[2] else None
         if gx is not None or gw is not None or gb is not None:
             with _on(xm):
                 space = _scratch(plan.scratch, xm)

@@ -8,8 +8,8 @@
 // element end in the same lane's accumulators, sixteen neighbouring elements of one row of h a lane, so the epilogue
 // needs no other lane's values. Bound by the matrix cores (4 M C F flops forward, twice that backward) and, behind them, by
 // what is written. Measured, bf16, 16384 x 1024 x 4096: forward 490 us (671 MB written behind 290 us of product), backward
-// 191 us elementwise (4.9 TB/s) and two products of 300 us (0.92 PFLOP/s; a library product of 8192^3 reaches 1.28). f32,
-// 4096 x 512 x 1408: forward 121 us, products 109 and 124 us (a library product of these sizes: 108, 98 and 101 us).
+// 191 us elementwise (4.9 TB/s) and 598 us for the two products (0.92 PFLOP/s; a library product of 8192^3 reaches 1.28). f32,
+// 4096 x 512 x 1408: forward 121 us, products 231 us (library products of these sizes: 108, 98 and 101 us).
 //
 // What the backward pass needs of g and u is either written by the forward pass in f32 (z) or, with bf16 operands and
 // few input features, computed again: a product of C terms per element against 8 bytes written and read. z is never
@@ -435,23 +435,6 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const GatedParams p) {
           (red[which][0][col] + red[which][1][col]) + (red[which][2][col] + red[which][3][col]);
   }
 }
-// gb = sum of the partial sums' rows, in a fixed order: 32 columns and 32 row lanes a block
-__global__ void __launch_bounds__(1024) gated_bias_kernel(const float* part, int rows, int n, float* gb) {
-  __shared__ float red[32][33];
-  const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + col;
-  float v = 0.f;
-  if (i < n) {
-#pragma unroll 8
-    for (int r = row; r < rows; r += 32) v += part[(size_t)r * n + i];
-  }
-  red[row][col] = v;
-  __syncthreads();
-  if (row == 0 && i < n) {
-#pragma unroll
-    for (int r = 1; r < 32; ++r) v += red[r][col];
-    gb[i] = v;
-  }
-}
 
 // ---- products of the backward pass -----------------------------------------------------------------------------
 struct ProductParams {
@@ -462,17 +445,16 @@ struct ProductParams {
   int64_t a_term;       // elements from the first term of a to the second
   int out_f32, col_tiles, tiles, splits, chunk;     // splits: of each term
 };
-template <class T, bool ARC, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) product_kernel(const ProductParams p) {
-  using G = TokGemm<T, ARC, true, BM, BN, WM, WN>;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
-  const int id = tok_xcd_order(blockIdx.x, gridDim.x);
+template <class T, bool ARC, int BMN, int WM, int WN>
+__device__ __forceinline__ void product_tile(const ProductParams& p, int id, T* smem) {
+  using G = TokGemm<T, ARC, true, BMN, BMN, WM, WN>;
+  constexpr int BM = BMN, BN = BMN;
   const int slab_id = id / p.tiles, t = id - slab_id * p.tiles, term = slab_id / p.splits, sp = slab_id - term * p.splits;
   const int mt = t / p.col_tiles, nt = t - mt * p.col_tiles;
   const int m0 = mt * BM, n0 = nt * BN, kbeg = sp * p.chunk, kend = min(p.K, kbeg + p.chunk);
   f32x16 acc[G::TM][G::TN];
   const TokOperand<T> A = {(const T*)p.a + term * p.a_term, p.lda, p.M, 0}, B = {(const T*)p.b, p.ldb, p.N, 0};
-  G::run(A, B, m0, n0, kbeg, kend, reinterpret_cast<T*>(smem_raw), acc);
+  G::run(A, B, m0, n0, kbeg, kend, smem, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
   const int wm = wid / WN, wn = wid % WN;
   const size_t slab = (size_t)slab_id * p.M * p.N;
@@ -493,13 +475,53 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) product_kernel(cons
       }
   }
 }
-// out = sum of the slabs in order
-template <class O>
-__global__ void __launch_bounds__(256) slab_sum_kernel(const float* slabs, int splits, size_t n, O* out) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-    float v = slabs[i];
-    for (int s = 1; s < splits; ++s) v += slabs[(size_t)s * n + i];
-    out[i] = (O)v;
+// gx = [gg gu] w (the first blocks) and gw = [gg gu]^T x in one launch: neither waits for the other's last blocks (1001 rows,
+// 333 x 777, bf16: 18 us, one after the other 17 + 17)
+template <class T, int BMN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) products_kernel(const ProductParams gx, const ProductParams gw, int gx_blocks) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+  const int id = (int)blockIdx.x - gx_blocks;
+  if (id < 0)
+    product_tile<T, false, BMN, WM, WN>(gx, tok_xcd_order(blockIdx.x, gx_blocks), reinterpret_cast<T*>(smem_raw));
+  else
+    product_tile<T, true, BMN, WM, WN>(gw, tok_xcd_order(id, gridDim.x - gx_blocks), reinterpret_cast<T*>(smem_raw));
+}
+
+// What is left to add up, in one launch: the slabs of gx and gw, elementwise and in order, and gb, the partial column sums'
+// rows in a fixed order (32 columns and 32 row lanes a block).
+struct SlabSum {
+  const float* slabs;
+  void* out;
+  size_t n;
+  int splits, out_f32, blocks;
+};
+__global__ void __launch_bounds__(1024) gated_sums_kernel(const SlabSum gx, const SlabSum gw, const float* part, int rows, int n, float* gb) {
+  const int id = blockIdx.x;
+  if (id < gx.blocks + gw.blocks) {
+    const SlabSum& p = id < gx.blocks ? gx : gw;
+    for (size_t i = (size_t)(id < gx.blocks ? id : id - gx.blocks) * 1024 + threadIdx.x; i < p.n; i += (size_t)p.blocks * 1024) {
+      float v = p.slabs[i];
+      for (int s = 1; s < p.splits; ++s) v += p.slabs[(size_t)s * p.n + i];
+      if (p.out_f32)
+        ((float*)p.out)[i] = v;
+      else
+        ((__bf16*)p.out)[i] = (__bf16)v;
+    }
+    return;
+  }
+  __shared__ float red[32][33];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = (id - gx.blocks - gw.blocks) * 32 + col;
+  float v = 0.f;
+  if (i < n) {
+#pragma unroll 8
+    for (int r = row; r < rows; r += 32) v += part[(size_t)r * n + i];
+  }
+  red[row][col] = v;
+  __syncthreads();
+  if (row == 0 && i < n) {
+#pragma unroll
+    for (int r = 1; r < 32; ++r) v += red[r][col];
+    gb[i] = v;
   }
 }
 
@@ -617,52 +639,58 @@ size_t product_bytes(int M, int N, int K, int terms) {
   return s == 1 ? 0 : (size_t)s * M * N * 4;
 }
 
-template <class T, bool ARC, int BMN, int WM, int WN>
-int launch_product(ProductParams& p, int slabs, hipStream_t st) {
-  using G = TokGemm<T, ARC, true, BMN, BMN, WM, WN>;
-  p.col_tiles = ceil_div(p.N, BMN);
-  p.tiles = ceil_div(p.M, BMN) * p.col_tiles;
-  auto kernel = product_kernel<T, ARC, BMN, BMN, WM, WN>;
-  const int rc = allow_lds(kernel, G::LDS_BYTES);
+// One of the two products: how it is cut, and its kernel's arguments.
+struct Product {
+  ProductPlan plan;
+  ProductParams p;
+  SlabSum sum;
+  int blocks;
+};
+template <class T>
+Product product(const void* a, int64_t lda, int terms, int64_t a_term, const void* b, int64_t ldb, int M, int N, int K, void* out, int out_f32,
+                void* slabs) {
+  Product q = {product_plan<T>(M, N, K)};
+  const int count = q.plan.splits * terms;
+  q.p.a = a;
+  q.p.b = b;
+  q.p.lda = lda;
+  q.p.ldb = ldb;
+  q.p.M = M;
+  q.p.N = N;
+  q.p.K = K;
+  q.p.splits = q.plan.splits;
+  q.p.chunk = q.plan.chunk;
+  q.p.a_term = a_term;
+  q.p.col_tiles = ceil_div(N, q.plan.tile);
+  q.p.tiles = ceil_div(M, q.plan.tile) * q.p.col_tiles;
+  q.p.out = count > 1 ? slabs : out;
+  q.p.out_f32 = count > 1 ? 1 : out_f32;
+  q.blocks = q.p.tiles * count;
+  if (count > 1) q.sum = {(const float*)slabs, out, (size_t)M * N, count, out_f32, vg_stream_grid((size_t)M * N, 1024)};
+  return q;
+}
+template <class T, int BMN, int WM, int WN>
+int launch_products_of(const Product& gx, const Product& gw, hipStream_t st) {
+  constexpr int A = TokGemm<T, false, true, BMN, BMN, WM, WN>::LDS_BYTES, B = TokGemm<T, true, true, BMN, BMN, WM, WN>::LDS_BYTES;
+  auto kernel = products_kernel<T, BMN, WM, WN>;
+  const int rc = allow_lds(kernel, A > B ? A : B);
   if (rc) return rc;
-  kernel<<<p.tiles * slabs, G::NT, G::LDS_BYTES, st>>>(p);
+  kernel<<<gx.blocks + gw.blocks, 64 * WM * WN, A > B ? A : B, st>>>(gx.p, gw.p, gx.blocks);
+  VG_CHECK_LAUNCH("gated backward products");
   return VG_OK;
 }
-template <class T, bool ARC>
-int product(const void* a, int64_t lda, int terms, int64_t a_term, const void* b, int64_t ldb, int M, int N, int K, void* out, int out_f32,
-            void* ws, size_t ws_bytes, hipStream_t st) {
-  const ProductPlan plan = product_plan<T>(M, N, K);
-  const size_t need = product_bytes<T>(M, N, K, terms);
-  if (need && (!ws || ws_bytes < need)) return vg_fail(VG_ERR_WORKSPACE, "gated backward: workspace of %zu bytes, %zu are needed", ws_bytes, need);
-  ProductParams p = {};
-  p.a = a;
-  p.b = b;
-  p.lda = lda;
-  p.ldb = ldb;
-  p.M = M;
-  p.N = N;
-  p.K = K;
-  p.splits = plan.splits;
-  p.chunk = plan.chunk;
-  p.a_term = a_term;
-  const int slabs = plan.splits * terms;
-  p.out = slabs > 1 ? ws : out;
-  p.out_f32 = slabs > 1 ? 1 : out_f32;
-  int rc;
-  if constexpr (sizeof(T) == 2)
-    rc = plan.tile == 256 ? launch_product<T, ARC, 256, 2, 4>(p, slabs, st) : launch_product<T, ARC, 128, 2, 2>(p, slabs, st);
-  else
-    rc = launch_product<T, ARC, 128, 2, 4>(p, slabs, st);
-  if (rc) return rc;
-  if (slabs > 1) {
-    const size_t n = (size_t)M * N;
-    if (out_f32)
-      slab_sum_kernel<float><<<vg_stream_grid(n, 256), 256, 0, st>>>((const float*)ws, slabs, n, (float*)out);
-    else
-      slab_sum_kernel<__bf16><<<vg_stream_grid(n, 256), 256, 0, st>>>((const float*)ws, slabs, n, (__bf16*)out);
+// either may have no blocks
+template <class T>
+int launch_products(const Product& gx, const Product& gw, hipStream_t st) {
+  if constexpr (sizeof(T) == 4) {
+    return launch_products_of<T, 128, 2, 4>(gx, gw, st);
+  } else {
+    if (gx.blocks && gw.blocks && gx.plan.tile != gw.plan.tile) {
+      const int rc = launch_products<T>(gx, Product{}, st);
+      return rc ? rc : launch_products<T>(Product{}, gw, st);
+    }
+    return (gx.blocks ? gx : gw).plan.tile == 256 ? launch_products_of<T, 256, 2, 4>(gx, gw, st) : launch_products_of<T, 128, 2, 2>(gx, gw, st);
   }
-  VG_CHECK_LAUNCH("gated backward product");
-  return VG_OK;
 }
 
 // What the backward pass of these sizes runs on: pre-activations kept by the forward pass in f32 (8 bytes written and read
@@ -672,8 +700,7 @@ int product(const void* a, int64_t lda, int terms, int64_t a_term, const void* b
 template <class T>
 bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 512; }
 
-// Scratch of the backward pass, one piece after the other: [gg gu], partial column sums, slabs of the two products (one after
-// the other on one stream: they share the space).
+// Scratch of the backward pass, one piece after the other: [gg gu], partial column sums, slabs of the two products.
 // bf16: [gg gu] is rounded to bf16 for the two products; of the many roundings in a sum most averages out, and what stays
 // costs a result 0.4 of its own rounding. In a small call (under 2^19 of them) they are too few for that: there what the
 // rounding left is multiplied too, as a second term, at no visible cost.
@@ -681,7 +708,7 @@ template <class T>
 int gz_terms(int M, int F) { return sizeof(T) == 2 && (long long)M * 2 * F < (1 << 19) ? 2 : 1; }
 
 struct BwdSpace {
-  size_t gz, part, slabs, total;
+  size_t gz, part, gx_slabs, gw_slabs, total;
   int rows;          // of partial column sums
 };
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -691,10 +718,10 @@ BwdSpace bwd_space(int M, int C, int F) {
   s.rows = ceil_div(M, keeps_z<T>(M, C) ? kRowsBlock : large_tiles<T>(M, 2ll * F) ? 256 : 128);
   s.gz = 0;
   s.part = align256((size_t)M * 2 * F * sizeof(T) * gz_terms<T>(M, F));
-  s.slabs = s.part + align256((size_t)s.rows * 2 * F * 4);
   const int terms = gz_terms<T>(M, F);
-  const size_t a = product_bytes<T>(M, C, 2 * F, terms), b = product_bytes<T>(2 * F, C, M, terms);
-  s.total = s.slabs + (a > b ? a : b);
+  s.gx_slabs = s.part + align256((size_t)s.rows * 2 * F * 4);
+  s.gw_slabs = s.gx_slabs + align256(product_bytes<T>(M, C, 2 * F, terms));
+  s.total = s.gw_slabs + product_bytes<T>(2 * F, C, M, terms);
   return s;
 }
 
@@ -705,7 +732,7 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (M == 0) {        // sums over no rows
-    if (gw) rc = product<T, true>(gh, 2 * (int64_t)F, 1, 0, x, C, 2 * F, C, 0, gw, gw_f32, nullptr, 0, st);
+    if (gw) rc = launch_products<T>(Product{}, product<T>(gh, 2 * (int64_t)F, 1, 0, x, C, 2 * F, C, 0, gw, gw_f32, nullptr), st);
     if (!rc && gb) rc = vg_fill(gb, 0.f, 2 * (size_t)F, stream);
     return rc;
   }
@@ -744,15 +771,16 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
     rc = launch_gated<T, true>(p, st);
     if (rc) return rc;
   }
-  if (gb) {
-    gated_bias_kernel<<<ceil_div(2ll * F, 32), 1024, 0, st>>>(p.gb_part, s.rows, 2 * F, gb);
-    VG_CHECK_LAUNCH("gated backward bias");
+  Product px = {}, pw = {};
+  if (gx) px = product<T>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, at + s.gx_slabs);
+  if (gw) pw = product<T>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, x, C, 2 * F, C, M, gw, gw_f32, at + s.gw_slabs);
+  if (gx || gw) rc = launch_products<T>(px, pw, st);
+  if (rc) return rc;
+  const int sums = px.sum.blocks + pw.sum.blocks + (gb ? ceil_div(2ll * F, 32) : 0);
+  if (sums) {
+    gated_sums_kernel<<<sums, 1024, 0, st>>>(px.sum, pw.sum, p.gb_part, s.rows, 2 * F, gb);
+    VG_CHECK_LAUNCH("gated backward sums");
   }
-  if (gx) {
-    rc = product<T, false>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, w, C, M, C, 2 * F, gx, sizeof(T) == 4, at + s.slabs, s.total - s.slabs, st);
-    if (rc) return rc;
-  }
-  if (gw) rc = product<T, true>(p.gz, 2 * (int64_t)F, p.terms, (int64_t)M * 2 * F, x, C, 2 * F, C, M, gw, gw_f32, at + s.slabs, s.total - s.slabs, st);
   return rc;
 }
 

@@ -390,6 +390,47 @@ def test_gated_f32_master_weight(gpu):
     assert torch.equal(g[0], g2[0]) and g[1].dtype == F32 and torch.equal(g[1].to(BF16), g2[1])
 
 
+@pytest.mark.parametrize("dtype, m, c, f, act", [
+    (BF16, 130, 600, 72, "gelu"),          # pre-activations kept, small tiles
+    (BF16, 200, 1024, 6400, "silu"),       # gx on small tiles, gw on large ones: two launches
+    (BF16, 4099, 264, 4096, "gelu"),       # large tiles, pre-activations computed again
+    (BF16, 4099, 520, 4720, "silu"),       # large tiles, pre-activations kept: over 256 MB, past the caches
+    (F32, 4099, 60, 3300, "gelu"),         # the same in f32
+], ids=str)
+def test_gated_large(gpu, dtype, m, c, f, act):
+    """What test_gated says, at the sizes where other tiles and the streaming kernels are chosen (the oracle on the GPU)."""
+    gen = torch.Generator().manual_seed(m + c + f)
+    x, w = _rand(gen, m, c, dtype=dtype).cuda(), _rand(gen, 2 * f, c, dtype=dtype, scale=c ** -0.5).cuda()
+    bias, gh = _rand(gen, 2 * f, scale=0.2).cuda(), _rand(gen, m, f, dtype=dtype).cuda()
+    leaves = [t.clone().requires_grad_() for t in (x, w, bias)]
+    h = _ops().gated_linear(*leaves, act=act)
+    got = dict(zip(("gx", "gw", "gb"), torch.autograd.grad(h, leaves, gh)))
+    got["h"] = h.detach()
+    want = oracle.gated(x.double(), w.double(), bias.double(), act, gh.double())
+    for n, terms in (("h", 0), ("gx", 2 * f), ("gw", m), ("gb", m)):
+        allowed = (c + terms + 32) * U32 * want["abs"][n] + 1e-30
+        if dtype == BF16 and n != "gb":
+            u = want["gz_abs"][n] * UBF * (1 + UBF) if n != "h" else 0
+            allowed = allowed + u + UBF * want[n].abs() * 1.01
+        _within(got[n].cpu(), want[n].cpu(), allowed.cpu(), n)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("m, c, f", [(17, 72, 1030), (1000, 96, 16), (257, 256, 200), (130, 600, 72)])
+def test_gated_gradients_of_a_part(gpu, dtype, m, c, f):
+    """Only what asks for a gradient gets one, and it is the same: alone, two together, with and without slabs to sum."""
+    gen = torch.Generator().manual_seed(8)
+    dev = [t.cuda() for t in (_rand(gen, m, c, dtype=dtype), _rand(gen, 2 * f, c, dtype=dtype), _rand(gen, 2 * f))]
+    gh = _rand(gen, m, f, dtype=dtype).cuda()
+    full = [t.clone().requires_grad_() for t in dev]
+    want = torch.autograd.grad(_ops().gated_linear(*full), full, gh)
+    for part in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        some = [t.clone().requires_grad_(j in part) for j, t in enumerate(dev)]
+        got = torch.autograd.grad(_ops().gated_linear(*some), [some[i] for i in part], gh)
+        for i, g in zip(part, got):
+            assert torch.equal(g, want[i]), (part, i)
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # beyond 32-bit offsets
 # ------------------------------------------------------------------------------------------------------------------

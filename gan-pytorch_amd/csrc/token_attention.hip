@@ -21,8 +21,8 @@
 // Bound by the SIMDs: the vector instructions of the softmax (one exponential, two to four others an element) add to the
 // matrix instructions instead of hiding under them, so heads of 128 come nearer the matrix rate than heads of 64. Measured,
 // bf16: 8192 queries and keys, 2 x 16 query and 4 key heads of 128 ("the long case" below) forward 1.20 ms (0.92 PFLOP/s; a
-// library product of 8192^3 reaches 1.28), backward 3.61 ms (0.76 on its five products, 1.07 with the two that both walks
-// rebuild); 1024 queries and keys, 8 x 16 heads of 64 59 and 149 us (0.58 PFLOP/s both).
+// library product of 8192^3 reaches 1.28), backward 3.57 ms (0.77 on its five products, 1.08 with the two that both walks
+// rebuild); 1024 queries and keys, 8 x 16 heads of 64 59 and 145 us (0.58 and 0.59 PFLOP/s).
 #include <float.h>
 #include <math.h>
 
@@ -545,7 +545,6 @@ __device__ __forceinline__ void queries_gradient(const AttnParams& p, int id, Gq
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= s[i];
-      if (kl == 1) dp = zero16();          // (the softmax of one key is constant)
       mul_cols<DP, FINE>(ktile[buf], dp, 32 * kk, lane, acc);
     }
     if (more) {
@@ -556,6 +555,10 @@ __device__ __forceinline__ void queries_gradient(const AttnParams& p, int id, Gq
     buf ^= 1;
   }
   if (r >= p.R) return;
+  if (kl == 1) {               // the softmax of one key is constant
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+  }
   if (p.splits > 1) {
     float* out = p.part + (((size_t)prob * p.splits + sp) * p.R + r) * DP;
 #pragma unroll
@@ -677,7 +680,6 @@ __device__ __forceinline__ void keys_gradient(const AttnParams& p, int id, GkvTi
         dp = mul_rows<DP, true>(smem[buf][1], vf, 32 * rr, c, h, dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= w[i];
-      if (kl == 1) dp = zero16();          // (the softmax of one key is constant)
       mul_cols<DP, FINE>(smem[buf][1], w, 32 * rr, lane, gv);
       __builtin_amdgcn_sched_barrier(0);     // (reads hoisted across this line spill)
       mul_cols<DP, FINE>(smem[buf][0], dp, 32 * rr, lane, gk);
@@ -691,6 +693,7 @@ __device__ __forceinline__ void keys_gradient(const AttnParams& p, int id, GkvTi
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) {
     if (key >= kl) gk[d] = gv[d] = zero16();
+    if (kl == 1) gk[d] = zero16();         // (the softmax of one key is constant)
     if (p.r_splits > 1) {
       const size_t at = (((size_t)prob * p.r_splits + sp) * g.Tk + key) * DP;
       const size_t half = (size_t)g.B * g.Hk * p.r_splits * g.Tk * DP;

@@ -3,7 +3,7 @@
 //   r = 1 / sqrt(mean(x^2) + eps)      n = x r w           (w null: n = x)
 //   section a of a head (width[a] elements, pairs (2i, 2i+1)):  theta = pos[a] base^(-2i / width[a])
 //   y0 = n0 cos - n1 sin    y1 = n0 sin + n1 cos           (elements behind the sections: y = n)
-// backward:  gn = R^T gy     gw = sum gn x r     gx = r (w gn - x r mean(w gn x r))
+// backward:  gn = R^T gy     gw = sum gn x r     gx = r (w gn - x r mean(w gn x r))     (heads with gy = 0: nothing)
 //
 // Bound by HBM: one read and one write per element forward, two reads and one write backward. A thread holds one
 // 16-byte vector of a head, a power of two of neighbouring lanes the head, and a wave one token (or several, where its
@@ -65,6 +65,13 @@ __device__ __forceinline__ float head_sum(float v, int lanes) {
   if (lanes >= 32) v += __shfl_xor(v, 16, 64);
   if (lanes >= 64) v += __shfl_xor(v, 32, 64);
   return v;
+}
+
+// Whether any of the head's gradients is not zero. A head without takes no part in the backward pass, whatever it holds: the
+// padding of a batch may be NaN, and 0 NaN would reach the weights' gradients.
+__device__ __forceinline__ bool head_any(u32x4 g, unsigned magnitude, int lane, int lanes) {
+  const unsigned long long some = __ballot(((g[0] | g[1] | g[2] | g[3]) & magnitude) != 0);
+  return (some >> (lane & -lanes) & (lanes == 64 ? ~0ull : (1ull << lanes) - 1)) != 0;
 }
 
 template <class T, bool BWD>
@@ -171,9 +178,10 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
               y[2 * i + 1] = gv[2 * i + 1] * c[i] - gv[2 * i] * s[i];
             }
             if (normed) {
+              const bool live = head_any(rg[u], sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu, lane, p.lph);
 #pragma unroll
               for (int e = 0; e < V; ++e) {
-                const float xh = xv[e] * r, wg = w[e] * y[e];
+                const float xh = live ? xv[e] * r : 0.f, wg = w[e] * y[e];
                 if (ok) sum[e] = __builtin_fmaf(y[e], xh, sum[e]);
                 inner = __builtin_fmaf(wg, xh, inner);
                 xv[e] = xh;
@@ -181,7 +189,7 @@ __global__ void __launch_bounds__(256, BWD ? 3 : 4) rotary_kernel(const RotaryPa
               }
               inner = head_sum(inner, p.lph) * inv_d;
 #pragma unroll
-              for (int e = 0; e < V; ++e) y[e] = r * __builtin_fmaf(-xv[e], inner, y[e]);
+              for (int e = 0; e < V; ++e) y[e] = live ? r * __builtin_fmaf(-xv[e], inner, y[e]) : 0.f;
             }
           }
           if (ok) __builtin_nontemporal_store(tok_narrow(y), reinterpret_cast<u32x4*>(out));
@@ -240,7 +248,7 @@ int check_geom(const vg_rotary_geom* g, const void* pos) {
   VG_REQUIRE((long long)g->B * g->T < (1ll << 31), "rotary: %lld tokens are too many", (long long)g->B * g->T);
   VG_REQUIRE(g->D >= 8 && g->D <= 256 && g->D % 8 == 0, "rotary: head width %d is not a multiple of 8 from 8 to 256", g->D);
   VG_REQUIRE(g->axes >= 0 && g->axes <= 4, "rotary: %d axes, 0 to 4 are supported", g->axes);
-  VG_REQUIRE(g->axes == 0 || pos, "rotary: null positions");
+  VG_REQUIRE(g->axes == 0 || pos || (long long)g->B * g->T == 0, "rotary: null positions");
   int64_t total = 0;
   for (int a = 0; a < g->axes; ++a) {
     VG_REQUIRE(g->width[a] >= 2 && g->width[a] % 2 == 0, "rotary: axis width %d is not even and positive", g->width[a]);

@@ -2084,7 +2084,10 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, axes=(), 
     q_weight / k_weight [width] (float32): scale of the norm, shared by the heads; None: that side is not normalised.
     positions [tokens, len(axes)] or [batch, tokens, len(axes)] (int32 / int64): a token's place on every axis (row and
     column of a feature map, frame of a clip). axes: how many elements of a head belong to each axis, in order; pair
-    (2i, 2i+1) of a section of width d turns by position * base^(-2i / d); elements behind the sections are not turned."""
+    (2i, 2i+1) of a section of width d turns by position * base^(-2i / d); elements behind the sections are not turned.
+
+    A head whose incoming gradient is zero (padding behind an attention with lengths) gets a zero gradient and adds nothing
+    to the weights', whatever it holds."""
     _token_tensor(q, "queries", 4)
     _token_tensor(k, "keys", 4)
     axes, base, eps = tuple(axes), float(base), float(eps)
@@ -2275,7 +2278,7 @@ def self_attention(qkv, heads, kv_heads=None, q_weight=None, k_weight=None, posi
                    eps=1e-6, scale=None):
     """`qk_norm_rotary` and `attention` of the tokens of each batch element among themselves. qkv [batch, tokens,
     heads + 2 * kv_heads, width]: queries, keys and values as one projection leaves them. lengths (int32 [batch]): tokens
-    of each batch element. Returns [batch, tokens, heads, width]."""
+    of each batch element; what lies behind them may hold anything, its result and its gradient are zero. Returns [batch, tokens, heads, width]."""
     _token_tensor(qkv, "packed queries, keys and values", 4)
     kv_heads = heads if kv_heads is None else kv_heads
     if heads < 1 or kv_heads < 1 or qkv.shape[2] != heads + 2 * kv_heads:

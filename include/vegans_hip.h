@@ -474,7 +474,8 @@ typedef struct vg_heads_layout {
  *   pair (2i, 2i+1) turns by pos[b][t][a] * base^(-2i / width[a]); elements behind the sections are not turned.
  * pos: int32, or int64 where pos_wide, [B][T][axes], batch stride pos_sb elements (0: one grid for the whole batch).
  * Forward: inputs at layouts q, k, outputs at oq, ok. Backward: inputs at q, k, output gradients at gq, gk, input
- * gradients written at oq, ok; gwq, gwk [D] nullable. Hk may be 0. D is a multiple of 8 up to 256; B T < 2^31. */
+ * gradients written at oq, ok; gwq, gwk [D] nullable; a normed head whose output gradient is zero gets a zero gradient and
+ * takes no part in gwq, gwk, whatever it holds. Hk may be 0. D is a multiple of 8 up to 256; B T < 2^31. */
 typedef struct vg_rotary_geom {
   int32_t B, T, Hq, Hk, D;
   int32_t axes, width[4];

@@ -553,6 +553,51 @@ def test_the_operators_together(gpu, dtype):
         assert off <= tol, (n, off.item(), tol)
 
 
+@pytest.mark.parametrize("packed", [True, False], ids=["packed", "separate"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_padding_holds_anything(gpu, dtype, packed, eps):
+    """Norm, rotation and attention of a padded batch whose padding is NaN, infinite or zero: results and gradients are those
+    of any other padding, bit for bit, the padding's own gradient is zero."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(12)
+    b, t, heads, kv, d = 4, 37, 4, 2, 24
+    lengths = torch.tensor([37, 9, 0, 30], dtype=torch.int32)
+    pad = torch.arange(t)[None, :] >= lengths[:, None]
+    base = _rand(gen, b, t, heads + 2 * kv, d, dtype=dtype)
+    wq, wk = (1 + 0.2 * torch.randn(d, generator=gen) for _ in range(2))
+    pos, go = torch.randint(0, 99, (b, t, 1), generator=gen), _rand(gen, b, t, heads, d, dtype=dtype)
+    found = []
+    for filling in (1.5, float("nan"), float("inf"), 0.0):
+        qkv = base.clone()
+        qkv[pad] = filling
+        leaves = [x.cuda().requires_grad_() for x in (qkv, wq, wk)]
+        n = lengths.cuda()
+        if packed:
+            o = ops.self_attention(leaves[0], heads, kv, leaves[1], leaves[2], pos.cuda(), (16,), n, eps=eps)
+        else:
+            q, k, v = leaves[0].split((heads, kv, kv), 2)
+            q, k = ops.qk_norm_rotary(q, k, leaves[1], leaves[2], pos.cuda(), (16,), eps=eps)
+            o = ops.attention(q, k, v, n, n)
+        found.append([o.detach()] + list(torch.autograd.grad(o, leaves, go.cuda())))
+    assert not found[0][0][pad.cuda()].any() and not found[0][1][pad.cuda()].any()
+    assert all(x.isfinite().all() and x.any() for x in found[0])
+    for other in found[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(found[0], other))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("b, t", [(2, 0), (0, 5), (1, 1)])
+def test_packed_of_nothing_and_one_token(gpu, dtype, b, t):
+    gen = torch.Generator().manual_seed(13)
+    leaves = [x.cuda().requires_grad_() for x in (_rand(gen, b, t, 4, 16, dtype=dtype), torch.ones(16), torch.ones(16))]
+    o = _ops().self_attention(leaves[0], 2, 1, leaves[1], leaves[2], torch.zeros(t, 1, dtype=torch.int32, device="cuda"), (16,))
+    assert o.shape == (b, t, 2, 16) and torch.equal(o, leaves[0][:, :, 3:].expand(b, t, 2, 16))
+    gx, gq, gk = torch.autograd.grad(o, leaves, torch.ones_like(o))
+    # one token attends to itself alone: its value's gradient is the sum over the heads, nothing else has one
+    assert gx.shape == leaves[0].shape and not gq.any() and not gk.any() and not gx[:, :, :3].any() and (gx[:, :, 3:] == 2).all()
+
+
 def test_on_other_streams_at_once(gpu):
     """Two streams run the operators at the same time (the second on other inputs): no scratch is shared."""
     sets = [_stage_inputs(F32, s) for s in (1, 2)]

@@ -1935,6 +1935,12 @@ def _new_dense(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _dense_grad(g):
+    """A result's gradient as the kernels read it: dense, from a 16-byte border on (autograd may hand over a slice)."""
+    g = g.contiguous()
+    return g if g.data_ptr() % 16 == 0 else g.clone()
+
+
 def _at(t):
     return t.data_ptr() if t is not None else None
 
@@ -2060,7 +2066,7 @@ class QkNormRotaryFn(Function):
     def backward(ctx, gyq, gyk):
         q, k, wq, wk, pos = ctx.saved_tensors
         lab, need = ctx.label, ctx.needs_input_grad
-        gyq, gyk = gyq.contiguous(), gyk.contiguous()
+        gyq, gyk = _dense_grad(gyq), _dense_grad(gyk)
         gq, gk = _new_dense(q), _new_dense(k)
         params = not inputs_only.active
         with _on(q):
@@ -2183,7 +2189,7 @@ class AttentionFn(Function):
     def backward(ctx, go):
         q, k, v, o, lse, low, q_lengths, k_lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
-        go = go.contiguous()
+        go = _dense_grad(go)
         gq = _new_dense(q) if need[0] else None
         gk = gv = None
         if need[1] or need[2]:
@@ -2259,7 +2265,7 @@ class SelfAttentionFn(Function):
     def backward(ctx, go):
         qkv, wq, wk, pos, yq, yk, o, lse, low, lengths = ctx.saved_tensors
         plan, lab, need = ctx.plan, ctx.label, ctx.needs_input_grad
-        go = go.contiguous()
+        go = _dense_grad(go)
         gqkv = _new_dense(qkv)
         gyq, gyk = torch.empty_like(yq), torch.empty_like(yk)
         params = not inputs_only.active

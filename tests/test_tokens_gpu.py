@@ -598,6 +598,31 @@ def test_packed_of_nothing_and_one_token(gpu, dtype, b, t):
     assert gx.shape == leaves[0].shape and not gq.any() and not gk.any() and not gx[:, :, :3].any() and (gx[:, :, 3:] == 2).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_gradients_at_any_address(gpu, dtype):
+    """The gradient of a result may be a slice of another tensor, off every 16-byte border (what a concatenation hands back),
+    or one number expanded."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(14)
+    qkv, x, w = _rand(gen, 2, 7, 4, 16, dtype=dtype), _rand(gen, 9, 24, dtype=dtype), _rand(gen, 32, 24, dtype=dtype)
+    scale, pos = torch.ones(16, device="cuda"), torch.arange(7, device="cuda")[:, None]
+    calls = [lambda t: ops.self_attention(t, 2, 1, scale, scale, pos, (16,)), lambda t: ops.attention(t[:, :, :2], t[:, :, 2:3], t[:, :, 3:]),
+             lambda t: ops.qk_norm_rotary(t[:, :, :2], t[:, :, 2:], scale, scale, pos, (16,))[0], lambda t: ops.gated_linear(t, w.cuda())]
+    for call, t in zip(calls, (qkv, qkv, qkv, x)):
+        leaf = t.cuda().requires_grad_()
+        out = call(leaf)
+        g = _rand(gen, *out.shape, dtype=dtype).cuda()
+        want = torch.autograd.grad(out, leaf, g, retain_graph=True)[0]
+        room = torch.zeros(g.numel() + 1, dtype=dtype, device="cuda")
+        room[1:] = g.flatten()
+        off = room[1:].view(g.shape)
+        assert off.data_ptr() % 16 and off.is_contiguous()
+        assert torch.equal(torch.autograd.grad(out, leaf, off, retain_graph=True)[0], want)
+        one = torch.ones(1, dtype=dtype, device="cuda")
+        want = torch.autograd.grad(out, leaf, torch.ones_like(out), retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(out, leaf, one.expand(out.shape))[0], want)
+
+
 def test_on_other_streams_at_once(gpu):
     """Two streams run the operators at the same time (the second on other inputs): no scratch is shared."""
     sets = [_stage_inputs(F32, s) for s in (1, 2)]

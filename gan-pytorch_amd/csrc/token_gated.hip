@@ -540,8 +540,7 @@ int allow_lds(K kernel, int bytes) {
 int check_sizes(int M, int C, int F, int act) {
   VG_REQUIRE(M >= 0 && C >= 1 && F >= 1, "gated: bad sizes rows=%d in=%d out=%d", M, C, F);
   VG_REQUIRE(act >= VG_GATE_SIGMOID && act <= VG_GATE_SILU, "gated: unknown activation %d", act);
-  // tile counts and row indices of 31 bits (element offsets are 64-bit)
-  // ... and byte offsets inside a tile of 32
+  // tile counts and row indices of 31 bits; byte offsets inside a tile (256 rows of C, 64 of 2F) of 32, all others of 64
   VG_REQUIRE(M < (1 << 30) && C < (1 << 21) && F < (1 << 20) &&
                  ((long long)M / 128 + 1) * ((long long)F * 2 / 128 + 1) < (1ll << 31) && ((long long)M / 128 + 1) * ((long long)C / 128 + 1) < (1ll << 31) / 64 &&
                  ((long long)F * 2 / 128 + 1) * ((long long)C / 128 + 1) < (1ll << 31) / 64,

@@ -33,8 +33,9 @@ struct TokStage {
   static constexpr int N = ROWS * BK / V / NT;
   static_assert(ROWS * BK / V % NT == 0, "whole vectors per thread");
   u32x4 r[N];
-  unsigned off[N];      // bytes from the base
-  const char* base;     // first row of the operand (KC) or first row of the tile (RC), at the current k
+  unsigned off[N];      // bytes from the base: inside the tile, i.e. at most 256 rows (k) of the operand
+  const char* base;     // first row of the tile at the current k (interleaved: the first of vector 0's half)
+  int64_t half;         // interleaved: bytes from one half of the operand to the other where a thread's vectors alternate
   bool edge;            // RC: vectors of the tile cross the operand's last row
 
   static __device__ __forceinline__ u32x4 whole(const char* p) {
@@ -54,9 +55,18 @@ struct TokStage {
     }
     return out;
   }
+  // An interleaved tile lies in two runs of rows, up to 2^40 bytes apart, so the way from one to the other is not part of
+  // the 32-bit offsets: 32 rows of one half are followed by 32 of the other, and a block's threads cover RPV rows with one
+  // vector each. Where that is 32 a thread's vectors alternate between the halves; where it is a multiple of 64 they all lie
+  // in one half, the same for a whole wave.
+  static constexpr int RPV = RC ? 64 : NT / VPR;
+  static_assert(RPV == 32 || RPV % 64 == 0, "a thread's vectors alternate between the halves or stay in one");
+  __device__ __forceinline__ const char* at(int i) const { return (RPV == 32 && i % 2 ? base + half : base) + off[i]; }
   // rows row0.. of the operand, from k
   __device__ __forceinline__ void place(const TokOperand<T>& a, int row0, int k) {
-    base = reinterpret_cast<const char*>(a.p + (RC ? k * a.ld + row0 : k + (a.split ? 0 : row0 * a.ld)));
+    half = a.split * a.ld * (int64_t)sizeof(T);
+    base = reinterpret_cast<const char*>(a.p + (RC ? k * a.ld + row0 : k + (a.split ? row0 / 2 : row0) * a.ld));
+    if (!RC && RPV != 32 && (__builtin_amdgcn_readfirstlane(threadIdx.x) / VPR >> 5) % 2) base += half;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = threadIdx.x + i * NT, lr = id / VPR, lv = (id % VPR) * V;
@@ -66,8 +76,8 @@ struct TokStage {
       } else {
         int row = lr;
         if (a.split) {       // 32 rows of the first half, the matching 32 of the second, ... (tok_split_row)
-          const int v = row0 + lr, f = (v >> 6) * 32 + tok_split_row(v & 31);
-          row = (f < a.split ? f : a.split - 1) + ((v >> 5) & 1) * a.split;
+          const int f = (lr >> 6) * 32 + tok_split_row(lr & 31), last = a.split - 1 - row0 / 2;
+          row = f < last ? f : last;
         } else if (row0 + row >= a.rows) {
           row = a.rows - 1 - row0;
         }
@@ -79,7 +89,7 @@ struct TokStage {
   // the k-step at the base, all of it inside the operand; then on to the next
   __device__ __forceinline__ void load_inside(const TokOperand<T>& a) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = whole(base + off[i]);
+    for (int i = 0; i < N; ++i) r[i] = whole(at(i));
     base += (RC ? BK * a.ld : BK) * (int64_t)sizeof(T);
   }
   // The first `left` elements at p, zeros behind them: the 16 bytes that end with them, shifted down (`left` may be
@@ -111,10 +121,10 @@ struct TokStage {
         if (left <= 0)
           r[i] = u32x4{0, 0, 0, 0};
         else
-          r[i] = roomy ? first(base + off[i], left) : part(base + off[i], left);
+          r[i] = roomy ? first(at(i), left) : part(at(i), left);
       } else {
         const int left = kend - k - lv;
-        r[i] = roomy ? first(base + off[i], left) : part(base + off[i], left);
+        r[i] = roomy ? first(at(i), left) : part(at(i), left);
       }
     }
     base += (RC ? BK * a.ld : BK) * (int64_t)sizeof(T);

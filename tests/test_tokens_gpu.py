@@ -493,6 +493,35 @@ def test_gated_rows_beyond_two_gigabytes(gpu):
     assert torch.isfinite(gw).all()
 
 
+@pytest.mark.parametrize("dtype, c, f", [(BF16, 16384, 65600), (F32, 8192, 65600)], ids=str)
+@pytest.mark.parametrize("m", [65, 400])          # small tiles, large tiles (bf16)
+def test_gated_weights_beyond_four_gigabytes(gpu, dtype, c, f, m):
+    """2 x 65600 rows of 32 KB: all weights are zero but some gate rows and the matching value rows, among them the last, whose
+    byte offsets pass 2^32. Those columns are the layer of these rows alone, all others and their gradients are zero."""
+    gen = torch.Generator().manual_seed(m)
+    rows = torch.tensor([0, 33, f // 2, f - 66, f - 2, f - 1])
+    x, small = _rand(gen, m, c, dtype=dtype), _rand(gen, 2 * len(rows), c, dtype=dtype, scale=c ** -0.5)
+    gh_small = _rand(gen, m, len(rows), dtype=dtype)
+    at = torch.cat((rows, f + rows)).cuda()
+    w = torch.zeros(2 * f, c, dtype=dtype, device="cuda")
+    w[at] = small.cuda()
+    gh = torch.ones(m, f, dtype=dtype, device="cuda")
+    gh[:, rows.cuda()] = gh_small.cuda()
+    leaves = [x.cuda().requires_grad_(), w.requires_grad_()]
+    h = _ops().gated_linear(*leaves)
+    gx, gw = torch.autograd.grad(h, leaves, gh)
+    want = oracle.gated(x.double(), small.double(), None, "silu", gh_small.double())
+    got = {"h": h[:, rows.cuda()], "gx": gx, "gw": gw[at]}
+    # as in test_gated: the other columns add zeros to these sums
+    for n, terms in (("h", 0), ("gx", 2 * len(rows)), ("gw", m)):
+        allowed = (c + terms + 32) * U32 * want["abs"][n] + 1e-30
+        if dtype == BF16:
+            u = want["gz_abs"][n] * UBF * (1 + UBF) if n != "h" else 0
+            allowed = allowed + u + UBF * want[n].abs() * 1.01
+        _within(got[n], want[n], allowed, n)
+    assert h.count_nonzero() == got["h"].count_nonzero() and gw.count_nonzero() == got["gw"].count_nonzero()
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # together, on streams and in graphs
 # ------------------------------------------------------------------------------------------------------------------

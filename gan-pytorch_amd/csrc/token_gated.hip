@@ -737,7 +737,6 @@ int gated_bwd(int M, int C, int F, const void* x, const void* w, const float* bi
   }
   VG_REQUIRE(x && w && gh, "gated backward: null tensor");
   VG_REQUIRE(!keeps_z<T>(M, C) || z, "gated backward: these sizes need the pre-activations of the forward pass");
-  VG_REQUIRE(ceil_div(F, 64) <= 65535, "gated backward: %d columns are too many", F);
   const BwdSpace s = bwd_space<T>(M, C, F);
   if (!ws || ws_bytes < s.total) return vg_fail(VG_ERR_WORKSPACE, "gated backward: workspace of %zu bytes, %zu are needed", ws_bytes, s.total);
   VG_REQUIRE(vg_aligned16(ws), "gated backward: workspace is not 16-byte aligned");

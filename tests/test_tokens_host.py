@@ -1,6 +1,10 @@
 """Token operators on the host: argument checks of the C entry points (nothing is launched) and of the Python operators
 without a GPU."""
 import ctypes
+import glob
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -124,3 +128,14 @@ def test_operators_refuse_cpu_tensors():
                  lambda: ops.gated_linear(torch.zeros(4, 8), torch.zeros(6, 8))):
         with pytest.raises(_hip.HipError, match="GPU"):
             call()
+
+
+@pytest.mark.skipif(shutil.which("make") is None, reason="no make here")
+def test_a_change_of_the_compiler_flags_compiles_every_kernel_again():
+    """(nothing is run: what make would do after an edit of its file) Objects built with other flags must not be kept: they
+    may hold the packed f32 instructions that the flags leave out."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gan-pytorch_amd", "csrc")
+    lines = subprocess.run(["make", "-n", "-C", csrc, "-W", "Makefile"], capture_output=True, text=True, check=True).stdout.splitlines()
+    compiled = {line.split(" -c ")[1].split()[0]: line for line in lines if " -c " in line}
+    assert sorted(compiled) == sorted(os.path.basename(p) for p in glob.glob(os.path.join(csrc, "*.hip")))
+    assert all("-packed-fp32-ops" in line for line in compiled.values())

@@ -1849,17 +1849,44 @@ class _FirstOrderFn(Function):
 # A gradient that autograd itself accumulates into a leaf goes through that leaf's accumulation node, which belongs to
 # the stream it was made on and lives as long as any graph over the leaf. A backward pass captured into a HIP graph
 # while an eager graph of the same leaf is alive would pull that eager stream into the capture, which ends the
-# process. The nodes are therefore marked when an operator first meets them (`_recorded`), and such a backward pass raises
-# instead. (Inside a training iteration the gradient ledger takes the parameters' gradients and no such node runs.)
-def _recorded(out):
-    """`out` (a tensor, or several of one operator) after its operator was recorded: marks the accumulation nodes of leaves."""
-    captured = None
+# process. So the operators record on which stream of a capture a node was made (`_birth`), and a captured backward pass
+# that would reach any other node raises instead. (Inside a training iteration the gradient ledger takes the parameters'
+# gradients and no such node runs.) A node does not tell who made it: one that is already there when an operator first
+# meets its leaf in a capture counts as eager, also if another operation of the same capture made it.
+def _record(fn, *args):
+    """fn.apply(*args), with the accumulation nodes of the leaves among `args` marked."""
+    if torch.cuda.is_current_stream_capturing():
+        nodes = [_birth(t) for t in args if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
+        out = fn.apply(*args)
+        del nodes         # (until here only this list kept a new node, and with it its mark, alive)
+        return out
+    out = fn.apply(*args)
     for node, _ in (out if torch.is_tensor(out) else out[0]).grad_fn.next_functions:
         if type(node) is _AccumulateGrad:
-            if captured is None:
-                captured = torch.cuda.is_current_stream_capturing()
-            node.metadata.setdefault("vg_captured", captured)
+            node.metadata.setdefault("vg_stream", None)
     return out
+
+
+def _birth(leaf):
+    """The accumulation node of `leaf`, marked at the first meeting: with the current, capturing stream if it was made just
+    now (a node keeps its leaf: one more reference), else with None."""
+    before = leaf._use_count()
+    node = torch.autograd.graph.get_gradient_edge(leaf).node
+    made = leaf._use_count() > before
+    if "vg_stream" not in node.metadata:
+        node.metadata["vg_stream"] = torch.cuda.current_stream(leaf.device) if made else None
+    return node
+
+
+def _born_in_capture(node):
+    """Whether the stream of accumulation node `node` takes part in a capture."""
+    stream = node.metadata.get("vg_stream")
+    if stream is None:
+        return False
+    if stream == torch.cuda.current_stream(node.variable.device):
+        return True
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _accumulate_grad_type():
@@ -1879,9 +1906,10 @@ def _first_order(backward):
     def run(ctx, *gouts):
         if torch.cuda.is_current_stream_capturing():
             for node, _ in ctx.next_functions:
-                if type(node) is _AccumulateGrad and not grads.accepts(node.variable) and not node.metadata.get("vg_captured", True):
+                if type(node) is _AccumulateGrad and not grads.accepts(node.variable) and not _born_in_capture(node):
                     raise _hip.HipError("backward pass captured while an eager graph of the same leaf tensor is alive: drop the "
-                                        "eager outputs (and losses) before the capture")
+                                        "eager outputs (and losses) before the capture (and let a token operator be the first "
+                                        "operation of the capture on its leaves)")
         if not torch.is_grad_enabled():
             return backward(ctx, *gouts)
         with torch.no_grad():
@@ -2107,7 +2135,7 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, axes=(), 
         positions = None
     if not _recording(q, k, q_weight, k_weight):
         return _rotate(plan, q, k, q_weight, k_weight, positions)
-    return _recorded(QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, plan))
+    return _record(QkNormRotaryFn, q, k, q_weight, k_weight, positions, plan)
 
 
 def _attention_geom(q, k, v, scale):
@@ -2222,7 +2250,7 @@ def attention(q, k, v, q_lengths=None, k_lengths=None, scale=None):
         with _on(q):
             plan.forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_lengths, k_lengths, o, False, _raw_stream(q))
         return o
-    return _recorded(AttentionFn.apply(q, k, v, q_lengths, k_lengths, plan))
+    return _record(AttentionFn, q, k, v, q_lengths, k_lengths, plan)
 
 
 class _SelfAttentionPlan:
@@ -2302,7 +2330,7 @@ def self_attention(qkv, heads, kv_heads=None, q_weight=None, k_weight=None, posi
         positions = None
     if not _recording(qkv, q_weight, k_weight):
         return plan.forward(qkv, q_weight, k_weight, positions, lengths, False)[2]
-    return _recorded(SelfAttentionFn.apply(qkv, q_weight, k_weight, positions, lengths, plan))
+    return _record(SelfAttentionFn, qkv, q_weight, k_weight, positions, lengths, plan)
 
 
 class _GatedPlan:
@@ -2387,7 +2415,7 @@ def gated_linear(x, w, bias=None, act="silu"):
     plan = _token_plan(("gated", m, c, f, dtype), lambda: _GatedPlan(m, c, f, dtype))
     if not _recording(x, w, bias):
         return plan.forward(*_gated_operands(x, w), bias, code, False)[0]
-    return _recorded(GatedLinearFn.apply(x, w, bias, code, plan))
+    return _record(GatedLinearFn, x, w, bias, code, plan)
 
 
 class TokensFn(Function):

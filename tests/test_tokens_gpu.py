@@ -724,6 +724,33 @@ def test_capture_over_a_live_eager_graph_is_refused(gpu):
     assert alive.shape == (4, 4)
 
 
+def test_capture_over_a_live_graph_of_another_operation_is_refused(gpu):
+    """The leaf's accumulation node was made by an eager operation that is none of the token operators."""
+    from vegans._hip import HipError
+    ops = _ops()
+    x = torch.ones(4, 8, device="cuda", requires_grad=True)
+    w = torch.ones(8, 8, device="cuda", requires_grad=True)
+    alive = x * 2
+    torch.cuda.synchronize()
+    with pytest.raises(HipError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            h = ops.gated_linear(x, w)
+            torch.autograd.grad(h, (x, w), torch.ones_like(h))
+    # without it the same capture works, and replays
+    del alive, h
+    want = torch.autograd.grad(ops.gated_linear(x, w), (x, w), torch.ones(4, 4, device="cuda"))
+    torch.cuda.synchronize()
+    graph, ones = torch.cuda.CUDAGraph(), torch.ones(4, 4, device="cuda")
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ops.gated_linear(x, w), (x, w), ones)
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_second_derivative_is_refused(gpu):
     """A gradient taken with create_graph=True raises when it is differentiated, also behind a constant output gradient."""
     from vegans._hip import HipError

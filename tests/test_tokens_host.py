@@ -130,6 +130,63 @@ def test_operators_refuse_cpu_tensors():
             call()
 
 
+class _Twice(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return 2 * x
+
+    @staticmethod
+    def backward(ctx, g):
+        return 2 * g
+
+
+def _checked():
+    """A toy operator whose backward pass is guarded as the token operators' are."""
+    from vegans.engine import ops
+
+    class Checked(_Twice):
+        backward = staticmethod(ops._first_order(_Twice.backward))
+
+    return lambda x: ops._record(Checked, x)
+
+
+def test_accumulation_nodes_from_outside_a_capture_are_refused(monkeypatch):
+    """The capture's state is made up, nothing runs on a GPU. Whoever made a leaf's accumulation node before the operator met
+    it in the capture, the captured backward pass is refused; a node that the operator itself makes there is fine, also
+    for its next calls, and after the capture."""
+    from vegans import _hip
+    state = {"capturing": False, "stream": "eager"}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: state["stream"])
+    op, one = _checked(), torch.ones(3)
+
+    def captured(x, calls=1):
+        state.update(capturing=True, stream="capture")
+        try:
+            return [torch.autograd.grad(y, x, one)[0].tolist() for y in [op(x) for _ in range(calls)]]
+        finally:
+            state.update(capturing=False, stream="eager")
+
+    def leaf():
+        return torch.nn.Parameter(torch.ones(3))
+
+    assert captured(leaf(), calls=2) == [[2.0] * 3] * 2
+    for eager in (op, lambda x: x * 3, lambda x: torch.autograd.graph.get_gradient_edge(x)):
+        x = leaf()
+        alive = eager(x)
+        with pytest.raises(_hip.HipError, match="eager graph"):
+            captured(x)
+        del alive
+        assert captured(x) == [[2.0] * 3]
+    # the captured graph lives on, an eager one joins it: the node is still the capture's
+    x = leaf()
+    state.update(capturing=True, stream="capture")
+    kept = op(x)
+    state.update(capturing=False, stream="eager")
+    assert torch.autograd.grad(op(x), x, one)[0].tolist() == [2.0] * 3 and captured(x) == [[2.0] * 3]
+    assert kept.requires_grad
+
+
 @pytest.mark.skipif(shutil.which("make") is None, reason="no make here")
 def test_a_change_of_the_compiler_flags_compiles_every_kernel_again():
     """(nothing is run: what make would do after an edit of its file) Objects built with other flags must not be kept: they

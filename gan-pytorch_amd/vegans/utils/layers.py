@@ -92,8 +92,9 @@ class LayerSelfAttention(_LayerOnTokens):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("LayerSelfAttention meets a grid of {} for the first time while a HIP graph is being captured: "
                                    "run it once before".format(grid))
-            axes = torch.meshgrid(*[torch.arange(n, dtype=torch.int32) for n in grid], indexing="ij")
-            got = self._places[(grid, device)] = torch.stack(axes, -1).reshape(-1, len(grid)).contiguous().to(device)
+            with torch.inference_mode(False):       # (a tensor made in inference mode cannot be saved for a backward pass)
+                axes = torch.meshgrid(*[torch.arange(n, dtype=torch.int32) for n in grid], indexing="ij")
+                got = self._places[(grid, device)] = torch.stack(axes, -1).reshape(-1, len(grid)).contiguous().to(device)
         return got
 
     def forward(self, x):

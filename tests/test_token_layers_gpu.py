@@ -111,6 +111,18 @@ def test_layers_take_tokens_and_rows(gpu):
         assert att(x[:, :, :1].contiguous(memory_format=torch.channels_last)).shape == (2, 32, 1, 4)
 
 
+def test_layers_train_after_inference_mode(gpu):
+    """Sampling under torch.inference_mode() first, then a training step on the same grid: what the layer keeps between calls
+    (the pixels' places) can be saved for the backward pass."""
+    att = _bound(_make("attention"))
+    x = torch.randn(2, 32, 3, 5, device="cuda").contiguous(memory_format=torch.channels_last)
+    with torch.inference_mode():
+        sampled = att(x)
+    y = att(x)
+    grads = torch.autograd.grad(y, list(att.parameters()), torch.ones_like(y))
+    assert torch.equal(sampled, y) and all(g.isfinite().all() for g in grads)
+
+
 def test_layers_refuse(gpu):
     layers = _layers()
     for bad in (lambda: layers.LayerSelfAttention(32, 3, 2), lambda: layers.LayerSelfAttention(30, 3), lambda: layers.LayerSelfAttention(512, 2),

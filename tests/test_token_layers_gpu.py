@@ -111,6 +111,60 @@ def test_layers_take_tokens_and_rows(gpu):
         assert att(x[:, :, :1].contiguous(memory_format=torch.channels_last)).shape == (2, 32, 1, 4)
 
 
+def _reference_of_tokens(layer, x, gy):
+    """What `_reference` gives, for a token tensor [batch, tokens, channels]: one axis, along the tokens."""
+    if isinstance(layer, _layers().LayerGatedFeedForward):         # (tokens do not meet: any feature map of them)
+        n, t, c = x.shape
+        y, gx, found = _reference(layer, x.transpose(1, 2).reshape(n, c, 1, t), gy.transpose(1, 2).reshape(n, c, 1, t))
+        return y.reshape(n, c, t).transpose(1, 2), gx.reshape(n, c, t).transpose(1, 2), found
+    P = {n: p.detach().cpu().double() for n, p in layer.named_parameters()}
+    H, K, D = layer.heads, layer.kv_heads, layer.width
+    n, t, c = x.shape
+    rows, grow = x.reshape(-1, c).double(), gy.reshape(-1, c).double()
+    pos = torch.arange(t).view(1, t, 1).expand(n, -1, -1)
+    q, k, v = (rows @ P["qkv.weight"].T).view(n, t, H + 2 * K, D).split((H, K, K), 2)
+    yq, yk = (oracle.rotary(a, s, pos, (D,), layer.base, layer.eps) for a, s in ((q, P["q_scale"]), (k, P["k_scale"])))
+    att = oracle.attention(yq, yk, v, go=(grow @ P["out.weight"]).view(n, t, H, D))
+    _, gq, gqs = oracle.rotary(q, P["q_scale"], pos, (D,), layer.base, layer.eps, att["gq"])
+    _, gk, gks = oracle.rotary(k, P["k_scale"], pos, (D,), layer.base, layer.eps, att["gk"])
+    gqkv, hidden = torch.cat((gq, gk, att["gv"]), 2).reshape(n * t, -1), att["o"].reshape(n * t, -1)
+    out, grows = hidden @ P["out.weight"].T + P["out.bias"], gqkv @ P["qkv.weight"]
+    if layer.residual:
+        out, grows = out + rows, grows + grow
+    return out.view(x.shape), grows.view(x.shape), {"q_scale": gqs, "k_scale": gks, "qkv.weight": gqkv.T @ rows, "out.weight": grow.T @ hidden,
+                                                   "out.bias": grow.sum(0)}
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["attention", "attention, no residual", "feed-forward"])
+@pytest.mark.parametrize("shape", ["tokens", "one row of pixels"])
+def test_layers_on_sequences_against_their_formulas(gpu, shape, kind, mode):
+    """Token tensors (one axis of rotation) and feature maps of one row (all rows' places are zero): values and gradients."""
+    from vegans.engine import ops
+    layer = _make(kind)
+    gen = torch.Generator().manual_seed(19)
+    size = (3, 29, layer.channels) if shape == "tokens" else (3, layer.channels, 1, 29)
+    x, gy = (torch.randn(size, generator=gen) for _ in range(2))
+    want, want_gx, want_p = (_reference_of_tokens if shape == "tokens" else _reference)(layer, x, gy)
+    previous = ops.set_matmul_precision(mode)
+    try:
+        layer = _bound(layer)
+        form = torch.contiguous_format if shape == "tokens" else torch.channels_last
+        xd = x.cuda().contiguous(memory_format=form).requires_grad_()
+        y = layer(xd)
+        assert y.shape == size
+        y = ops.as_f32(y) if shape != "tokens" else ops.as_f32(y.reshape(-1, size[-1])).reshape(size)
+        got = torch.autograd.grad(y, [xd] + list(layer.parameters()), gy.cuda().contiguous(memory_format=form))
+    finally:
+        ops.set_matmul_precision(previous)
+    # as in test_layer_against_its_formula
+    tol = 10 * UBF if mode == "bf16" else 10 * 64 * 8 * U32
+    names = [n for n, _ in layer.named_parameters()]
+    for a, b, n in [(y, want, "y"), (got[0], want_gx, "gx")] + [(g, want_p[n], n) for g, n in zip(got[1:], names)]:
+        off = ((a.detach().cpu().double() - b).norm() / b.norm()).item()
+        assert off <= tol, (n, off, tol)
+
+
 def test_layers_train_after_inference_mode(gpu):
     """Sampling under torch.inference_mode() first, then a training step on the same grid: what the layer keeps between calls
     (the pixels' places) can be saved for the backward pass."""

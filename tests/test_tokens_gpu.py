@@ -291,6 +291,41 @@ def test_attention_of_nothing(gpu, dtype):
     assert ops.attention(new(0, 3, 2, 16), new(0, 3, 2, 16), new(0, 3, 2, 16)).shape == (0, 3, 2, 16)
 
 
+@pytest.mark.parametrize("case", [
+    (2, 700, 900, 2, 2, 24, False),        # both walks split
+    (3, 640, 520, 4, 2, 64, True),
+    (1, 1100, 1030, 2, 1, 96, True),
+    (8, 300, 300, 16, 8, 32, False),       # keys whole, rows split
+    (16, 256, 260, 16, 16, 64, True),      # both whole
+    (8, 200, 200, 32, 32, 128, False),
+], ids=str)
+def test_attention_of_many_scores(gpu, case):
+    """bf16 beyond 2^20 scores, where probabilities and ds are rounded to one bf16 term for their products."""
+    assert case[0] * case[1] * case[2] * case[3] > 1 << 20
+    q, k, v, ql, kl, go = _attention_case(case, BF16)
+    want = oracle.attention(q.double(), k.double(), v.double(), ql, kl, None, go.double())
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    lens = [t.cuda() if t is not None else None for t in (ql, kl)]
+    o = _ops().attention(*leaves, *lens)
+    got = dict(zip(("o", "gq", "gk", "gv"), (o,) + torch.autograd.grad(o, leaves, go.cuda())))
+    for name in got:
+        _within(got[name], want[name], _attention_allowed(want, BF16, case, name), name)
+
+
+def test_attention_over_few_keys_in_a_large_batch(gpu):
+    """What test_attention_over_few_keys says, beyond 2^20 scores, for two and three keys."""
+    for tk in (2, 3):
+        case = (1024, 33, tk, 16, 16, 64, False)
+        q, k, v, _, _, go = (t.cuda() if t is not None else None for t in _attention_case(case, BF16))
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        got = dict(zip(("gq", "gk"), torch.autograd.grad(_ops().attention(*leaves), leaves[:2], go)))
+        some = slice(500, 503)
+        want = oracle.attention(*(t[some].cpu().double() for t in (q, k, v)), None, None, None, go[some].cpu().double())
+        for n in got:
+            off = (got[n][some].cpu().double() - want[n]).norm()
+            assert off <= 2 * UBF * want[n].norm() + 2.0 ** -15 * want["abs"][n].norm(), (tk, n, off / want[n].norm())
+
+
 def test_attention_gradients_of_a_part(gpu):
     """Only what asks for a gradient gets one, and it is the same."""
     q, k, v, ql, kl, go = _attention_case((2, 33, 65, 4, 2, 32, True), F32)
@@ -457,6 +492,30 @@ def test_attention_over_a_cache_of_four_gigabytes(gpu):
     assert not gq.any() and not gk.any()
 
 
+def test_attention_gradients_over_a_cache_of_four_gigabytes(gpu):
+    """As above, with output gradients under which the scores of the two keys have gradients: go v^T is 2 and -2, delta 0, ds
+    therefore 1 and -1 (p = 1/2), and components of the keys that the queries do not see tell them apart."""
+    n, d = (1 << 24) + 77, 128
+    k = torch.zeros(1, n, 1, d, dtype=BF16, device="cuda")
+    v = torch.zeros(1, n, 1, d, dtype=BF16, device="cuda")
+    q = torch.zeros(1, 3, 1, d, dtype=BF16, device="cuda")
+    q[0, :, 0, 0] = 16.0
+    places = (n - 1, (1 << 31) // d + 5)
+    for i, at in enumerate(places):
+        k[0, at, 0, 0], k[0, at, 0, 2 + i] = 64.0, 8.0
+        v[0, at, 0, i] = 2.0
+    go = torch.zeros(1, 3, 1, d, dtype=BF16, device="cuda")
+    go[..., 0], go[..., 1] = 1.0, -1.0
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    gq, gk, gv = torch.autograd.grad(_ops().attention(*leaves), leaves, go)
+    assert gv.count_nonzero() == 4 and gk.count_nonzero() == 2 and gq.count_nonzero() == 6
+    scale = torch.tensor(d ** -0.5)              # of three queries of 16, of keys of 8: far from a rounding border of bf16
+    for i, (at, sign) in enumerate(zip(places, (1, -1))):
+        assert gv[0, at, 0, :2].tolist() == [1.5, -1.5]
+        assert gk[0, at, 0, 0].item() == sign * (48 * scale).to(BF16).item()
+        assert gq[0, :, 0, 2 + i].tolist() == [sign * (8 * scale).to(BF16).item()] * 3
+
+
 def test_strides_of_four_gigabytes(gpu):
     """Batch elements 2^31 elements apart."""
     store = torch.zeros((1 << 31) + 4096, dtype=BF16, device="cuda")
@@ -491,6 +550,26 @@ def test_gated_rows_beyond_two_gigabytes(gpu):
         allowed = (c + 2 * f + 32) * U32 * want["abs"]["gx"] + UBF * (1 + UBF) * want["gz_abs"]["gx"] + UBF * want["gx"].abs() * 1.01
         _within(got, want["gx"], allowed, "gx")
     assert torch.isfinite(gw).all()
+
+
+def test_gated_weight_gradient_beyond_two_gigabytes(gpu):
+    """2^20 + 3 rows of 2 x 1100 pre-activations, output gradients around the 2^31st of them and in the last rows only: the
+    weight gradient is that of these rows alone."""
+    m, c, f = (1 << 20) + 3, 8, 1100
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(m, c, generator=gen, device="cuda").to(BF16).requires_grad_()
+    w = torch.randn(2 * f, c, generator=gen, device="cuda").to(BF16).requires_grad_()
+    border = (1 << 31) // (2 * f)
+    some = torch.cat((torch.arange(border - 20, border + 20), torch.arange(m - 100, m))).cuda()
+    gh = torch.zeros(m, f, dtype=BF16, device="cuda")
+    gh[some] = torch.randn(len(some), f, generator=gen, device="cuda").to(BF16)
+    gx, gw = torch.autograd.grad(_ops().gated_linear(x, w), (x, w), gh)
+    want = oracle.gated(x.detach()[some].cpu().double(), w.detach().cpu().double(), None, "silu", gh[some].cpu().double())
+    # as in test_gated: all other rows add zeros
+    for n, got, terms in (("gw", gw, len(some)), ("gx", gx[some], 2 * f)):
+        allowed = (c + terms + 32) * U32 * want["abs"][n] + UBF * (1 + UBF) * want["gz_abs"][n] + UBF * want[n].abs() * 1.01
+        _within(got, want[n], allowed, n)
+    assert gx.count_nonzero() == gx[some].count_nonzero()
 
 
 @pytest.mark.parametrize("dtype, c, f", [(BF16, 16384, 65600), (F32, 8192, 65600)], ids=str)

@@ -2400,7 +2400,8 @@ def gated_linear(x, w, bias=None, act="silu"):
     """act(x Wg^T + bg) * (x Wu^T + bu): the first half of a gated feed-forward block. x [rows, features], w
     [2 * out, features] with the gate's rows first, bias [2 * out] (float32) or None; act "silu", "gelu" (exact), "relu" or
     "sigmoid". With bfloat16 x, w may be bfloat16 or a float32 master (rounded to bfloat16 for the products; its gradient
-    is float32)."""
+    is float32). x and w are contiguous or a slice of columns of a contiguous tensor, which is copied (bfloat16: of an even
+    number of columns on a 4-byte border, rows an even number apart); other strides (transposed, expanded) are refused."""
     _token_tensor(x, "input", 2)
     _token_tensor(w, "weight", 2)
     if w.shape[0] < 2 or w.shape[0] % 2 or w.shape[1] != x.shape[1] or not x.shape[1]:

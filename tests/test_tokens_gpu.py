@@ -425,6 +425,26 @@ def test_gated_f32_master_weight(gpu):
     assert torch.equal(g[0], g2[0]) and g[1].dtype == F32 and torch.equal(g[1].to(BF16), g2[1])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_gated_takes_column_slices_and_refuses_other_strides(gpu, dtype):
+    from vegans._hip import HipError
+    gen = torch.Generator().manual_seed(6)
+    wide_x, wide_w, gh = (_rand(gen, n, c, dtype=dtype).cuda() for n, c in ((70, 96), (24, 64), (70, 12)))
+    x, w = wide_x[:, 16:64], wide_w[:, 2:50]
+    dense, sliced = ([t.requires_grad_() for t in ts] for ts in ((x.clone(), w.clone()), (x.detach(), w.detach())))
+    assert not sliced[0].is_contiguous() and not sliced[1].is_contiguous()
+    h, want = _ops().gated_linear(*sliced), _ops().gated_linear(*dense)
+    assert torch.equal(h, want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(h, sliced, gh), torch.autograd.grad(want, dense, gh)))
+    x, w = dense[0].detach(), dense[1].detach()
+    bad = [(x.T.contiguous().T, w), (x, w.T.contiguous().T), (x[:1].expand(70, -1), w), (x, w[:1].expand(24, -1)), (wide_x[:, :96:2], w)]
+    if dtype == BF16:
+        bad += [(wide_x[:, 1:49], w), (wide_x[:, :47], w[:, :47].contiguous())]
+    for operands in bad:
+        with pytest.raises(HipError):
+            _ops().gated_linear(*operands)
+
+
 @pytest.mark.parametrize("dtype, m, c, f, act", [
     (BF16, 130, 600, 72, "gelu"),          # pre-activations kept, small tiles
     (BF16, 200, 1024, 6400, "silu"),       # gx on small tiles, gw on large ones: two launches

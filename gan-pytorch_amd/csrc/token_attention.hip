@@ -303,7 +303,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
 #pragma unroll
   for (int j = 0; j < DP / 32; ++j) o[j] = zero16();
   float m = -FLT_MAX, l = 0.f;       // finite: a row whose scores are all -inf sums to zero, not to NaN
-  // split walks have few rows: a wave without any only loads (16 problems of 8 rows on 16384 keys of 64: 16.5 -> 13.6 us)
+  // Split walks have few rows: a wave without any only loads (16 problems of 8 rows on 16384 keys of 64, bf16: 16.5 -> 13.6 us
+  // where calls repeat on keys and values that stay in the last-level cache in part; 16.4, 4.1 TB/s, where they change). f32:
+  // 45.8 us either way, 2.9 TB/s; the one wave with rows takes 8192 cycles of f32 products for 64 keys of 64, most of them
+  // for empty rows of the 32.
   const bool idle = SPLIT && rt * kTileRows + __builtin_amdgcn_readfirstlane(wid) * 32 >= rows;
   int buf = 0;
   if (kbeg < kend) {
@@ -752,6 +755,8 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(const AttnParams p) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
+// Heads are worked on at the next width of these (zeros behind their own elements): 72 and 96 cost what 128 does (4 x 8 heads,
+// 2048 queries and keys, bf16: 86 us forward, 238 backward; 64: 61 and 137).
 int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
@@ -788,8 +793,10 @@ int check_strides(const vg_attention_geom* g, bool backward) {
 }
 
 // A walk over `len` (keys, or rows) is split where the blocks alone leave compute units idle: towards 512 blocks (two
-// for each of the 256), but no split shorter than two tiles of 64 (f32, whose products take eight times as long: one),
-// below which a split's own start and its partial results cost more than the walk it saves.
+// for each of the 256), but into no more than len / 128 splits (f32, whose products take eight times as long: len / 64),
+// beyond which a split's own start and its partial results cost more than the walk it saves. The splits' length is then
+// rounded up to whole tiles of 64 (chunk_of), so the last splits of some lengths are empty: of the 8 over 517 f32 keys, 128
+// each, three are. They write zeros, which the joining kernel adds like the others.
 template <class T>
 int splits_for(long long blocks, long long len) {
   if (blocks >= 256 || blocks == 0) return 1;
@@ -842,9 +849,13 @@ AttnParams params_of(const vg_attention_geom* g, const Plan& q) {
 }
 int chunk_of(int len, int splits) { return ((len + splits - 1) / splits + 63) & ~63; }
 
-// bf16: a probability's (ds's) rounding is one of very many that average out in a result, and costs it 0.4 of its own
-// rounding. In a small call they are too few for that; there both terms are taken, at no visible cost (up to 2^20
-// probabilities the products take a few microseconds).
+// bf16: probabilities and ds go into their products rounded to bf16. That costs a result up to 0.4 of its own rounding,
+// whatever the number of terms (l2 against 64 bits, heads of 64, 2 to 512 keys: o 1.8 to 2.3e-3, gradients 2.3 to 2.5e-3, the
+// results' rounding alone 1.7e-3), and the queries' gradient more where the keys have a part in common: ds sums to zero and
+// cancels it, the rounded ds do not (keys of mean 1 and deviation 1: 0.9 to 1.2e-2). Calls of under 2^20 scores take both as
+// two bf16 terms (2^-17) and come out at the results' rounding alone in all of these; there the products take a few
+// microseconds. In larger calls the second term would cost up to a fifth (64 x 16 heads of 128 of one query on 2048 keys:
+// forward 49 -> 60 us). The size is that of the whole call, so a batch element's last bits depend on the batch it is in.
 template <class T>
 bool fine(const vg_attention_geom& g) {
   return sizeof(T) == 2 && (double)g.B * g.Hq * g.Tq * g.Tk < (double)(1 << 20);

@@ -7,9 +7,11 @@
 // weight tile takes 32 gate rows, the matching 32 value rows, the next 32 gate rows, ...: gate and value of one output
 // element end in the same lane's accumulators, sixteen neighbouring elements of one row of h a lane, so the epilogue
 // needs no other lane's values. Bound by the matrix cores (4 M C F flops forward, twice that backward) and, behind them, by
-// what is written. Measured, bf16, 16384 x 1024 x 4096: forward 490 us (671 MB written behind 290 us of product), backward
-// 191 us elementwise (4.9 TB/s) and 598 us for the two products (0.92 PFLOP/s; a library product of 8192^3 reaches 1.28). f32,
-// 4096 x 512 x 1408: forward 121 us, products 231 us (library products of these sizes: 108, 98 and 101 us).
+// what is written. Measured in a loop of calls, bf16, 16384 x 1024 x 4096: forward 441 us where the pre-activations are kept
+// (671 MB written), 308 where not (134 MB); backward 679, of which 187 are the elementwise pass with the bias gradient (939 MB)
+// and 237 and 251 the products for the inputs' and the weights' gradients (1.16 and 1.10 PFLOP/s; library products of the same
+// operand orders take 218 and 255). f32, 4096 x 512 x 1408: forward 108 us, backward 236 (library products: 108, 98 and 101).
+// Launches under a profiler, with pauses between them, take up to a quarter longer.
 //
 // What the backward pass needs of g and u is either written by the forward pass in f32 (z) or, with bf16 operands and
 // few input features, computed again: a product of C terms per element against 8 bytes written and read. z is never
@@ -32,7 +34,8 @@ struct GatedParams {
 // The gates. f32 takes the library's exponential and error function. bf16 results keep 8 bits: the hardware's exponential
 // and reciprocal (one unit in the last place of f32) and, for the normal distribution's tail, formula 7.1.26 of
 // Abramowitz and Stegun, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by at most 1.5e-7 - the library's
-// error function took longer than the products of a tile.
+// error function took longer than the products of a tile. Far in the tail that is no longer small beside the value: off by
+// 0.05 % of it at g = -4, 0.3 % at -5.7, 1 % at -8, where gelu itself is -1e-4, -3e-8 and -5e-15 (half a step of bf16: 0.4 %).
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float g) {
   if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
@@ -700,9 +703,9 @@ template <class T>
 bool keeps_z(int M, int C) { return sizeof(T) == 4 || M <= kFewRows || C > 512; }
 
 // Scratch of the backward pass, one piece after the other: [gg gu], partial column sums, slabs of the two products.
-// bf16: [gg gu] is rounded to bf16 for the two products; of the many roundings in a sum most averages out, and what stays
-// costs a result 0.4 of its own rounding. In a small call (under 2^19 of them) they are too few for that: there what the
-// rounding left is multiplied too, as a second term, at no visible cost.
+// bf16: [gg gu] is rounded to bf16 for the two products, which costs a result 0.4 of its own rounding. In a small call (under
+// 2^19 of them) what the rounding left is multiplied too, as a second term, at no visible cost. The size is that of the
+// whole call, so a row's last bits depend on how many others come with it.
 template <class T>
 int gz_terms(int M, int F) { return sizeof(T) == 2 && (long long)M * 2 * F < (1 << 19) ? 2 : 1; }
 

@@ -504,7 +504,8 @@ int vg_qk_norm_rotary_bwd_h(const vg_rotary_geom* g, const void* q, const void* 
  * bf16: o_low [B][Tq][Hq][D] (dense, nullable) is what the rounding of o left; with it the backward pass loses nothing to it.
  * Backward: gq, and gk with gv, may be null (not wanted).
  * D is a multiple of 8 up to 128; scale is finite and not zero; with G = Hq / Hk, (Tq G + 128) G < 2^32 and Tk < 2^30;
- * strides between tokens stay under 2^30 / 66 bytes (gradients' and outputs': any). */
+ * strides of q, k, v and (backward) go between tokens stay under 2^30 / 66 bytes, of q and go between heads under 2^30 / G (all
+ * others: any). */
 typedef struct vg_attention_geom {
   int32_t B, Tq, Tk, Hq, Hk, D;
   float scale;

@@ -158,9 +158,10 @@ __device__ __forceinline__ f32x16 mul_tiles(const __bf16* tile, const __bf16* co
 }
 
 // acc[j] (rows d = 32 j + row) += sum over the 32 rows k0.. of a TR tile of tile[k][d] * w[k][column], w as a product left it.
-// bf16: w (probabilities, ds) is rounded to bf16 for this; FINE: taken as two bf16 terms, i.e. to 2^-17.
+// bf16: w (probabilities, ds) is rounded to bf16 for this; FINE: taken as two bf16 terms, i.e. to 2^-17. `total` (not with
+// FINE): every element += the sum over the 32 rows of the rounded w[column].
 template <int DP, bool FINE>
-__device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
+__device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32], f32x16* total = nullptr) {
   using L = Tile<__bf16, DP, true>;
   const int h = lane >> 5, q = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   // rows k0 + 16 s + 4 h + q and 8 further: bits 2-3 of the row are h and 2 + h
@@ -176,6 +177,9 @@ __device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, in
 #pragma unroll
       for (int i = 0; i < 8; ++i) left[i] -= (float)x[i];
       x2 = __builtin_bit_cast(bf16x8, tok_narrow(left));
+    } else if (total) {
+      const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+      *total = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ones, x, *total, 0, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) {
@@ -188,7 +192,7 @@ __device__ __forceinline__ void mul_cols(const __bf16* tile, const f32x16& w, in
   }
 }
 template <int DP, bool>
-__device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32]) {
+__device__ __forceinline__ void mul_cols(const float* tile, const f32x16& w, int k0, int lane, f32x16 (&acc)[DP / 32], f32x16* = nullptr) {
   constexpr int LD = Tile<float, DP, true>::LD;
   const int h = lane >> 5, c = lane & 31;
 #pragma unroll
@@ -303,6 +307,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
 #pragma unroll
   for (int j = 0; j < DP / 32; ++j) o[j] = zero16();
   float m = -FLT_MAX, l = 0.f;       // finite: a row whose scores are all -inf sums to zero, not to NaN
+  // Probabilities of one bf16 term are divided by the sum of what they were rounded to, not of what they were: their roundings
+  // then only move o among the values, and nothing of the values' common part reaches delta = go o, in which it would be
+  // many times the scores' gradients (values, keys and output gradients of mean 3 and deviation 1: queries' gradient off by
+  // 9 to 11 % so, 0.7 % here). The matrix cores form that sum (any element of `total`, over both lane halves) in the time that
+  // the additions would take: the long case 1.20 ms either way.
+  constexpr bool kRounded = sizeof(T) == 2 && !FINE;
+  f32x16 total = zero16();
   // Split walks have few rows: a wave without any only loads (16 problems of 8 rows on 16384 keys of 64, bf16: 16.5 -> 13.6 us
   // where calls repeat on keys and values that stay in the last-level cache in part; 16.4, 4.1 TB/s, where they change). f32:
   // 45.8 us either way, 2.9 TB/s; the one wave with rows takes 8192 cycles of f32 products for 64 keys of 64, most of them
@@ -344,6 +355,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
         const float alpha = __builtin_amdgcn_exp2f(m - top);
         m = top;
         l *= alpha;
+        total[0] *= alpha;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -354,10 +366,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[kk][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk][i], cs, -m));
-          l += s[kk][i];
+          if (!kRounded) l += s[kk][i];
         }
 #pragma unroll
-      for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP, FINE>(vtile[buf], s[kk], 32 * kk, lane, o);
+      for (int kk = 0; kk < KT / 32; ++kk) mul_cols<DP, FINE>(vtile[buf], s[kk], 32 * kk, lane, o, kRounded ? &total : nullptr);
     }
     if (more) {
       sk.store(ktile[buf ^ 1]);
@@ -366,7 +378,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
     __syncthreads();
     buf ^= 1;
   }
-  l += __shfl_xor(l, 32, 64);
+  l = kRounded ? total[0] : l + __shfl_xor(l, 32, 64);
   if (r >= rows) l = 0.f;       // (took part as a row of zeros)
   if (r >= p.R) return;
   if constexpr (SPLIT) {
@@ -852,7 +864,8 @@ int chunk_of(int len, int splits) { return ((len + splits - 1) / splits + 63) & 
 // bf16: probabilities and ds go into their products rounded to bf16. That costs a result up to 0.4 of its own rounding,
 // whatever the number of terms (l2 against 64 bits, heads of 64, 2 to 512 keys: o 1.8 to 2.3e-3, gradients 2.3 to 2.5e-3, the
 // results' rounding alone 1.7e-3), and the queries' gradient more where the keys have a part in common: ds sums to zero and
-// cancels it, the rounded ds do not (keys of mean 1 and deviation 1: 0.9 to 1.2e-2). Calls of under 2^20 scores take both as
+// cancels it, the rounded ds do not (keys, values and output gradients of deviation 1 and mean 1: 3.2 to 3.6e-3, mean 3: 6.4
+// to 7.3e-3). Calls of under 2^20 scores take both as
 // two bf16 terms (2^-17) and come out at the results' rounding alone in all of these; there the products take a few
 // microseconds. In larger calls the second term would cost up to a fifth (64 x 16 heads of 128 of one query on 2048 keys:
 // forward 49 -> 60 us). The size is that of the whole call, so a batch element's last bits depend on the batch it is in.

@@ -326,6 +326,37 @@ def test_attention_over_few_keys_in_a_large_batch(gpu):
             assert off <= 2 * UBF * want[n].norm() + 2.0 ** -15 * want["abs"][n].norm(), (tk, n, off / want[n].norm())
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("b, tq, tk", [(700, 33, 3), (64, 40, 37), (16, 130, 150), (64, 1, 1100)])
+def test_attention_of_a_common_part(gpu, b, tq, tk, d):
+    """bf16 beyond 2^20 scores, keys, values and output gradients of mean 3 and deviation 1. ds = p (go v^T - delta) is the small
+    difference of two numbers near 9 d that have the values' common part in common: delta must not carry it rounded.
+
+    In norm, independent roundings adding as squares: the result's (u of it), each ds' (u |ds_j| |k_j|), and each
+    probability's: e_j p_j, |e_j| <= u, moves o by sum_j e_j p_j (v_j - o), delta by sum_j e_j ds_j (u |ds| in norm) and gq by that
+    times the row's mean key. A rounding is at most u, 0.4 u in the mean: a factor of two to spare; f32 adds 64 half-steps
+    of |go| |v| in delta."""
+    gen = torch.Generator().manual_seed(d + tk)
+    h, scale = 16, 0.02
+    q, k, v, go = (_rand(gen, b, n, h, d) + mean for n, mean in ((tq, 0), (tk, 3), (tk, 3), (tq, 3)))
+    q, k, v, go = (t.to(BF16).cuda() for t in (q, k, v, go))
+    assert b * h * tq * tk >= 1 << 20
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = _ops().attention(*leaves, scale=scale)
+    gq, gk, gv = torch.autograd.grad(o, leaves, go)
+    Q, K, V, G = (t.double().transpose(1, 2).contiguous() for t in (q, k, v, go))
+    p = torch.softmax(scale * Q @ K.transpose(2, 3).contiguous(), -1)
+    O = p @ V
+    ds = p * (G @ V.transpose(2, 3).contiguous() - (G * O).sum(-1, keepdim=True))
+    want = scale * ds @ K
+    squares = ds.square() @ K.square().sum(-1, keepdim=True) + ds.square().sum(-1, keepdim=True) * (p @ K).square().sum(-1, keepdim=True)
+    delta = 64 * U32 * (G.abs() * (p @ V.abs())).sum(-1, keepdim=True) * (p @ K).norm(dim=-1, keepdim=True)
+    allowed = UBF * (want.square().sum() + scale ** 2 * squares.sum()).sqrt() + scale * delta.norm()
+    off = (gq.double().transpose(1, 2) - want).norm()
+    assert off <= allowed, ((off / want.norm()).item(), (allowed / want.norm()).item())
+    assert (o.double().transpose(1, 2) - O).norm() <= 1.5 * UBF * O.norm()
+
+
 def test_attention_gradients_of_a_part(gpu):
     """Only what asks for a gradient gets one, and it is the same."""
     q, k, v, ql, kl, go = _attention_case((2, 33, 65, 4, 2, 32, True), F32)

@@ -19,10 +19,10 @@
 // 4-byte loads. Queries' gradients use the same shape; the gradients of keys and values its mirror image (column = key).
 //
 // Bound by the SIMDs: the vector instructions of the softmax (one exponential, two to four others an element) add to the
-// matrix instructions instead of hiding under them, so heads of 128 come nearer the matrix rate than heads of 64. Measured,
-// bf16: 8192 queries and keys, 2 x 16 query and 4 key heads of 128 ("the long case" below) forward 1.20 ms (0.92 PFLOP/s; a
-// library product of 8192^3 reaches 1.28), backward 3.57 ms (0.77 on its five products, 1.08 with the two that both walks
-// rebuild); 1024 queries and keys, 8 x 16 heads of 64 59 and 145 us (0.58 and 0.59 PFLOP/s).
+// matrix instructions instead of hiding under them, so heads of 128 come nearer the matrix rate than heads of 64. Measured
+// in loops of calls, bf16: 8192 queries and keys, 2 x 16 query and 4 key heads of 128 ("the long case" below) forward 1.15 ms (0.96 PFLOP/s; a
+// library product of 8192^3 reaches 1.28), backward 3.51 ms (0.78 on its five products, 1.10 with the two that both walks
+// rebuild); 1024 queries and keys, 8 x 16 heads of 64 51 and 145 us (0.67 and 0.59 PFLOP/s).
 #include <float.h>
 #include <math.h>
 
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_fwd_kernel(c
   // Probabilities of one bf16 term are divided by the sum of what they were rounded to, not of what they were: their roundings
   // then only move o among the values, and nothing of the values' common part reaches delta = go o, in which it would be
   // many times the scores' gradients (values, keys and output gradients of mean 3 and deviation 1: queries' gradient off by
-  // 9 to 11 % so, 0.7 % here). The matrix cores form that sum (any element of `total`, over both lane halves) in the time that
-  // the additions would take: the long case 1.20 ms either way.
+  // 9 to 11 % so, 0.7 % here). The matrix cores form that sum (any element of `total`, over both lane halves) in little more
+  // time than the additions would take: the long case 1.12 -> 1.15 ms, the other 49.5 -> 51.2 us.
   constexpr bool kRounded = sizeof(T) == 2 && !FINE;
   f32x16 total = zero16();
   // Split walks have few rows: a wave without any only loads (16 problems of 8 rows on 16384 keys of 64, bf16: 16.5 -> 13.6 us

@@ -20,9 +20,9 @@
 //
 // Bound by the SIMDs: the vector instructions of the softmax (one exponential, two to four others an element) add to the
 // matrix instructions instead of hiding under them, so heads of 128 come nearer the matrix rate than heads of 64. Measured
-// in loops of calls, bf16: 8192 queries and keys, 2 x 16 query and 4 key heads of 128 ("the long case" below) forward 1.15 ms (0.96 PFLOP/s; a
-// library product of 8192^3 reaches 1.28), backward 3.51 ms (0.78 on its five products, 1.10 with the two that both walks
-// rebuild); 1024 queries and keys, 8 x 16 heads of 64 51 and 145 us (0.67 and 0.59 PFLOP/s).
+// in loops of calls, bf16: 8192 queries and keys, 2 x 16 query and 4 key heads of 128 ("the long case" below) forward 1.15 ms
+// (0.96 PFLOP/s; a library product of 8192^3 reaches 1.28), backward 3.51 ms (0.78 on its five products, 1.10 with the two
+// that both walks rebuild); 1024 queries and keys, 8 x 16 heads of 64 51 and 145 us (0.67 and 0.59 PFLOP/s).
 #include <float.h>
 #include <math.h>
 
@@ -865,10 +865,10 @@ int chunk_of(int len, int splits) { return ((len + splits - 1) / splits + 63) & 
 // whatever the number of terms (l2 against 64 bits, heads of 64, 2 to 512 keys: o 1.8 to 2.3e-3, gradients 2.3 to 2.5e-3, the
 // results' rounding alone 1.7e-3), and the queries' gradient more where the keys have a part in common: ds sums to zero and
 // cancels it, the rounded ds do not (keys, values and output gradients of deviation 1 and mean 1: 3.2 to 3.6e-3, mean 3: 6.4
-// to 7.3e-3). Calls of under 2^20 scores take both as
-// two bf16 terms (2^-17) and come out at the results' rounding alone in all of these; there the products take a few
-// microseconds. In larger calls the second term would cost up to a fifth (64 x 16 heads of 128 of one query on 2048 keys:
-// forward 49 -> 60 us). The size is that of the whole call, so a batch element's last bits depend on the batch it is in.
+// to 7.3e-3). Calls of under 2^20 scores take both as two bf16 terms (2^-17) and come out at the results' rounding alone in
+// all of these; there the products take a few microseconds. In larger calls the second term would cost up to a fifth (64 x
+// 16 heads of 128 of one query on 2048 keys: forward 49 -> 60 us). The size is that of the whole call, so a batch element's
+// last bits depend on the batch it is in.
 template <class T>
 bool fine(const vg_attention_geom& g) {
   return sizeof(T) == 2 && (double)g.B * g.Hq * g.Tq * g.Tk < (double)(1 << 20);
